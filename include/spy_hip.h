@@ -183,6 +183,65 @@ int spy_hip_set_exact_order(int on);
  * index of the FIRST maximum of n logits, written to *out_index (device int32) */
 int spy_hip_argmax(void *stream, const float *logits, int64_t n, int32_t *out_index);
 
+/* Sampling -- beside spy_hip_argmax, which takes the largest logit: a token drawn from each row of a batch, by given random numbers.  No counterpart in
+ * the reference (its one sampler is the greedy one).  For the logits l of a row, in 64 bits of the definition:
+ *   w_i = exp((l_i - max l) / temperature);  the tokens are ranked by l, the largest first, equal ones by index;
+ *   kept are the first tokens in that rank, as many as the strictest of these leaves, one at least:
+ *     top_k   that many (0 or less: any number)
+ *     min_p   those with w >= min_p (0 or less: all; more than 1 counts as 1)
+ *     top_p   the fewest whose w add up to top_p times the sum over the tokens that top_k leaves (1 or more: all)
+ *   the token drawn is, in order of index, the first kept one at which the running sum of w exceeds uniform * (sum of the kept w).
+ * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab < 2^19.  All five settings are device arrays with one value per
+ * row; NULL: temperature 1, no top_k, no min_p, no top_p.  uniform is required: numbers in [0, 1) (below 0 and NaN count as 0, 1 and above as the last number before 1).
+ * temperature <= 0 (or NaN) takes the first of the largest logits.  -inf and NaN logits are never drawn; where a logit is +inf, all that are +inf have w = 1 and
+ * the others 0.  A row without a logit above -inf gives token -1 and probability 0.
+ * tokens: n_row int32, device; probs: n_row floats or NULL: w of the token / sum of the kept w.
+ * Weights are held as multiples of 2^-44 of the largest and added as integers, so that a result depends on no order of additions; tokens whose w is below that
+ * have none.  scratch: device memory of spy_hip_sample_scratch_size bytes, 256-byte aligned, this call's alone until the stream has passed it. */
+typedef struct spy_hip_sample_param {
+    const float   *temperature;
+    const int32_t *top_k;
+    const float   *top_p, *min_p;
+    const float   *uniform;
+} spy_hip_sample_param;
+size_t spy_hip_sample_scratch_size(const spy_hip_tensor *logits);
+int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sample_param *param, int32_t *tokens, float *probs, void *scratch, size_t scratch_bytes);
+
+/* ---- a batch of sequences over a cache in pages: no counterpart in the reference, whose caches hold one sequence
+ *      (attention.cpp:180-265).  K pages are {hd, page_size, n_kv_head, n_page} and V^T pages {page_size, hd, n_kv_head, n_page}, F16, nb[0] = 2, the other
+ *      strides any multiples of 16 bytes, data 16-byte aligned: within a page the layouts of the caches above (rows of K, rows of V^T).  page_size is a power of
+ *      two from 16 to 1024, hd 64, 128 or 256, n_head a multiple of n_kv_head (query head h reads K/V head h / (n_head / n_kv_head)). ----------------- */
+typedef struct spy_hip_paged_batch {
+    int32_t n_seq;               /* sequences */
+    int32_t max_new, max_kv;     /* no sequence has more new / cached tokens than these (the launches are sized by them) */
+    const int32_t *row_start;    /* device, n_seq + 1 entries, ascending from 0: rows row_start[s] .. row_start[s+1] - 1 of q, k, v and out are the new tokens of
+                                    sequence s (none: the sequence takes no part); rows from row_start[n_seq] on are left alone */
+    const int32_t *kv_len;       /* device, n_seq entries: cached tokens of a sequence, its new ones included, so that new token i is at position
+                                    kv_len[s] - (row_start[s+1] - row_start[s]) + i */
+    const int32_t *pages;        /* device, n_seq rows: entry j is the page of positions j * page_size ..; entries past a sequence's last page are not read */
+    int64_t page_stride;         /* entries from one row of `pages` to the next; a sequence has at most that many pages */
+} spy_hip_paged_batch;
+/* Position rotation and the stores of new tokens into the cache: Rope of q and k, the fp16 rounding of q, and both cache copies
+ * (non-linear.cpp:270-371; view.cpp:83-227; attention.cpp:180-265) for the batch, in one launch.  q {hd, n_head, n_row}, k and v {hd, n_kv_head, n_row}: F32 or
+ * F16, one type, nb[0] = its size, the other strides any multiples of 16 bytes, data 16-byte aligned; q_out {hd, n_head, n_row} F16 likewise.  q and q_out may both be
+ * NULL.  rope: NULL or mode -1: no rotation; mode 0: pairs (2i, 2i + 1), mode 2: pairs (i, i + num_dim / 2), i < num_dim / 2, by the angle
+ * position * freq_scale * freq_base^(-2i / num_dim), cos and sin times attention_factor; elements from num_dim on (a multiple of 16, at most hd) stay as they are.
+ * Angles are reduced in 64 bits; the other fields of RopeParam are not looked at, but extend_factor and xpos_base have to be 0 (SPY_HIP_EUNSUPPORTED).  Other
+ * than spy_hip_op_rope it is the same in every summation order.  A token at a negative position, or whose page is not in 0 .. n_page - 1, has no place in
+ * the cache: the error flag of spy_hip_take_error is raised and its K and V are not stored.  q_out must not overlap q, k or v. */
+int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k, const spy_hip_tensor *v, const spy_hip_paged_batch *batch,
+                         const spy_hip_rope_param *rope, const spy_hip_tensor *q_out, const spy_hip_tensor *k_pages, const spy_hip_tensor *v_pages);
+/* Attention of the batch's new tokens over the pages (which hold them already): MatMul(K, q) -> Softmax(mask, scale) -> MatMul(V^T, P) per sequence and head
+ * (attention.cpp:25-302).  q {hd, n_head, n_row} F16, out the same shape F32 or F16, strides and alignment as above.  A token sees the positions below
+ * kv_len of its sequence; causal != 0: none behind its own; window > 0: of those the last `window` up to its own position only.  A token that sees no
+ * position gets zeros; what lies in the pages at positions it does not see, infinities and NaN too, does not reach its output.  Pages outside 0 .. n_page - 1 hold nothing
+ * and raise the error flag.  scale: finite.  Scores, sums and the product are fp32; probabilities enter the product as fp16 (a relative error of 2^-11 each) for
+ * F16 outputs and as two fp16 terms (2^-22) for F32 outputs.  scratch: device memory of spy_hip_paged_attention_scratch_size bytes, 256-byte aligned, this call's
+ * alone until the stream has passed it (a captured call: until its graph is done with); its contents need not be set. */
+size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch);
+int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *v_pages, const spy_hip_tensor *out,
+                            const spy_hip_paged_batch *batch, float scale, int32_t causal, int32_t window, void *scratch, size_t scratch_bytes);
+
 /* ---- kernel families used by the operators above and by the fused token loop --------------- */
 
 /* Quantizator<FP32,Q8_0>::transform (backend/host/include/simd/vec_convert.h:178-261):

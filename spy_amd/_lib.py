@@ -35,6 +35,17 @@ class RopeParam(C.Structure):
                 ("beta_slow", C.c_float), ("xpos_base", C.c_float), ("xpos_down", C.c_int32)]
 
 
+class SampleParam(C.Structure):
+    """spy_hip_sample_param: device arrays, one value per row"""
+    _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "uniform")]
+
+
+class PagedBatch(C.Structure):
+    """spy_hip_paged_batch"""
+    _fields_ = [("n_seq", C.c_int32), ("max_new", C.c_int32), ("max_kv", C.c_int32), ("row_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("pages", C.c_void_p), ("page_stride", C.c_int64)]
+
+
 class LlamaLayer(C.Structure):
     """spy_hip_llama_layer"""
     _fields_ = [(n, C.c_void_p) for n in ("attn_norm", "ffn_norm", "wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down")] + \
@@ -102,6 +113,11 @@ SIGNATURES = {
     "spy_hip_take_error": (_i32, [C.POINTER(_i32)]),
     "spy_hip_set_exact_order": (_i32, [_i32]),
     "spy_hip_argmax": (_i32, [_vp, _vp, _i64, _vp]),
+    "spy_hip_sample_scratch_size": (_sz, [_TP]),
+    "spy_hip_sample": (_i32, [_vp, _TP, C.POINTER(SampleParam), _vp, _vp, _vp, _sz]),
+    "spy_hip_paged_append": (_i32, [_vp, _TP, _TP, _TP, C.POINTER(PagedBatch), C.POINTER(RopeParam), _TP, _TP, _TP]),
+    "spy_hip_paged_attention_scratch_size": (_sz, [_TP, _TP, C.POINTER(PagedBatch)]),
+    "spy_hip_paged_attention": (_i32, [_vp, _TP, _TP, _TP, _TP, C.POINTER(PagedBatch), _f32, _i32, _i32, _vp, _sz]),
     "spy_hip_quantize_q8_0": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64]),
     "spy_hip_quantize_f16": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64]),
     "spy_hip_gemv_q8_0act": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64]),
