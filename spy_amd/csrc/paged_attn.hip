@@ -10,6 +10,8 @@
 // are what the next instruction, O^T = V^T P^T, wants from it.  P never leaves the registers; V^T pages give its other operand as 16 contiguous bytes.
 #include "paged.cuh"
 
+#include <type_traits>
+
 int *spy_hip_err_flag_ptr();
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -24,10 +26,33 @@ struct attn_args {
     int G, group;                        // K/V heads, query heads to one
     float c;                             // scale * log2(e)
     int causal, window;                  // window: 0 or how many positions back
-    int tiles, split;                    // tiles of 16 rows per sequence and K/V head; key tiles (of 32) per workgroup
-    int n_split;
-    float *part;                         // (o, m, l) of the workgroups that share rows
+    // Sequences of few rows: tiles of 16 rows per sequence and K/V head, key tiles (of 32) per workgroup, workgroups that share a row's keys at most.  The others:
+    // tiles of CHUNK_ROWS rows over all sequences, key tiles (of 64).
+    int few, few_tiles, few_split, few_pieces, few_blocks;
+    int chunk_tiles, chunk_split, chunk_pieces, chunk_blocks;
+    float *few_part, *chunk_part;        // (o, m, l) of the workgroups that share rows
     int *err;
+};
+
+#define CHUNK_ROWS 128
+
+// Rows of a tile: the query rows are (new token, query head of the group) pairs, token by token.  Which keys they see: a token t those in lo(t) .. hi(t) - 1.
+struct row_tile {
+    int rows, r0, n_row;                 // of the sequence and K/V head; first of the tile; in the tile
+    int past;                            // position of the sequence's token 0; negative where the cache holds less than the new tokens
+    int group, kv, causal, window;
+    __device__ __forceinline__ row_tile(const attn_args &a, const pg_seq &q, int tile, int per) {
+        rows = q.n_new * a.group; r0 = tile * per; n_row = min(per, rows - r0);
+        past = q.kv - q.n_new; group = a.group; kv = q.kv; causal = a.causal; window = a.window;
+    }
+    __device__ __forceinline__ int hi(int t) const { return causal ? max(past + t + 1, 0) : kv; }
+    __device__ __forceinline__ int lo(int t) const { return window > 0 ? max(past + t - window + 1, 0) : 0; }
+    __device__ __forceinline__ int first() const { return r0 / group; }
+    __device__ __forceinline__ int last() const { return (r0 + n_row - 1) / group; }
+    __device__ __forceinline__ int hi_all() const { return hi(first()); }           // every row sees lo_all .. hi_all - 1
+    __device__ __forceinline__ int lo_all() const { return lo(last()); }
+    __device__ __forceinline__ int end() const { return hi(last()); }               // no row sees a key outside lo_any .. end - 1
+    __device__ __forceinline__ int lo_any() const { return lo(first()); }
 };
 
 static __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -39,53 +64,78 @@ template <class Op> static __device__ __forceinline__ float quad_reduce(float v,
     return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 static __device__ __forceinline__ v8h halves(uint4 w) { return __builtin_bit_cast(v8h, w); }
-// whether any of the eight fp16 values is an infinity or NaN
-static __device__ __forceinline__ bool unbounded(uint4 w) {
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    bool any = false;
+// the first n of eight fp16 values (n <= 0: none), the others 0
+static __device__ __forceinline__ uint4 first_of(uint4 w, int n) {
+    uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) any |= (v[i] & 0x7C00u) == 0x7C00u || (v[i] & 0x7C000000u) == 0x7C000000u;
-    return any;
+    for (int i = 0; i < 4; i++) v[i] &= n >= 2 * i + 2 ? 0xFFFFFFFFu : n == 2 * i + 1 ? 0xFFFFu : 0u;
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
-// the values of positions j with bit j set, 0 for the others and -- bounded -- for infinities and NaN
-static __device__ __forceinline__ uint4 only(uint4 w, uint32_t mask, bool bounded) {
+// infinities and NaN among eight fp16 values taken as 0; any: whether there were some
+static __device__ __forceinline__ uint4 bounded(uint4 w, bool &any) {
     uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if (!(mask >> (2 * i) & 1) || (bounded && (v[i] & 0x7C00u) == 0x7C00u)) v[i] &= 0xFFFF0000u;
-        if (!(mask >> (2 * i + 1) & 1) || (bounded && (v[i] & 0x7C000000u) == 0x7C000000u)) v[i] &= 0x0000FFFFu;
+        const bool lo = (v[i] & 0x7C00u) == 0x7C00u, hi = (v[i] & 0x7C000000u) == 0x7C000000u;
+        any |= lo | hi;
+        v[i] = lo ? v[i] & 0xFFFF0000u : v[i];
+        v[i] = hi ? v[i] & 0x0000FFFFu : v[i];
     }
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
+// Where V holds infinities or NaN at positions that some rows of a tile see and others do not, a probability of 0 would not keep them out of the others' outputs (0 times
+// either is NaN).  There the product takes 0 in their place, and which of +inf, -inf and NaN a row sees in which dimension is counted by the same instruction
+// over indicators: w's elements that are of kind 0, 1, 2 as 1, the others as 0.
+static __device__ __forceinline__ v8h of_kind(uint4 w, int kind) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t out = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t b = v[i] >> (16 * h) & 0xFFFFu;
+            const bool is = kind == 2 ? (b & 0x7FFFu) > 0x7C00u : b == (kind ? 0xFC00u : 0x7C00u);
+            out |= is ? 0x3C00u << (16 * h) : 0u;
+        }
+        r[i] = out;
+    }
+    return halves(make_uint4(r[0], r[1], r[2], r[3]));
+}
+// 1 for bit j set, 0 else
+static __device__ __forceinline__ v8h ones(uint32_t bits) {
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = (bits >> (2 * i) & 1 ? 0x3C00u : 0u) | (bits >> (2 * i + 1) & 1 ? 0x3C000000u : 0u);
+    return halves(make_uint4(r[0], r[1], r[2], r[3]));
+}
+static __device__ __forceinline__ float kind_value(int kind) { return kind == 2 ? NAN : kind ? -INFINITY : INFINITY; }
 
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
 // Bound by the bytes of K and V.  The four waves take every fourth tile of 32 keys, straight from memory into the registers of the matrix instruction: nothing is
 // shared between waves before the end.
-template <int D, bool F32OUT>
-__global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
-    constexpr int KS = D / 32, DT = D / 16, HALF = D < 128 ? D : 128;
-    __shared__ float s_m[4][16], s_l[4][16];
-    __shared__ __attribute__((aligned(16))) float s_o[4][16][HALF + 4];
+template <int D> struct few_shared {
+    static constexpr int HALF = D < 128 ? D : 128;
+    float m[4][16], l[4][16];
+    __attribute__((aligned(16))) float o[4][16][HALF + 4];
+};
+template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(const attn_args &a, few_shared<D> &sh, int block) {
+    constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D>::HALF;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, quarter = lane >> 4;
-    const int unit = blockIdx.x, piece = blockIdx.y;
-    const int s = unit / (a.tiles * a.G), rest = unit - s * a.tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
+    const int units = a.b.n_seq * a.few_tiles * a.G, piece = block / units, unit = block - piece * units;
+    const int s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
     const pg_seq sq = pg_sequence(a.b, s, a.err);
     if (!sq.ok) return;
-    const int rows = sq.n_new * a.group, r0 = tile * 16;
-    if (r0 >= rows) return;
+    const row_tile rt(a, sq, tile, 16);
+    if (rt.n_row <= 0 || rt.rows > a.few) return;
+    const int rows = rt.rows, r0 = rt.r0;
     const int r = min(r0 + n, rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
-    const int past = sq.kv - sq.n_new;                                     // position of token 0; negative where the cache holds less than the new tokens
-    // keys that a token t sees: lo(t) <= j < hi(t)
-    auto hi_of = [&](int t) { return a.causal ? max(past + t + 1, 0) : sq.kv; };
-    auto lo_of = [&](int t) { return a.window > 0 ? max(past + t - a.window + 1, 0) : 0; };
-    const int t_first = r0 / a.group, t_last = min(r0 + 15, rows - 1) / a.group;
-    const int hi = hi_of(token), lo = lo_of(token), hi_all = hi_of(t_first), lo_all = lo_of(t_last);          // all rows see lo_all .. hi_all - 1
-    const int begin = lo_of(t_first) & ~31, end = hi_of(t_last);                                            // some row sees a key in begin .. end - 1
+    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all(), begin = rt.lo_any() & ~31, end = rt.end();
     const int n_tile = max((end - begin + 31) >> 5, 0);
-    if (piece > 0 && piece * a.split >= n_tile) return;
-    const int stop = min((piece + 1) * a.split, n_tile);
-    const bool whole = n_tile <= a.split;
+    if (piece > 0 && piece * a.few_split >= n_tile) return;
+    const int stop = min((piece + 1) * a.few_split, n_tile);
+    const bool whole = n_tile <= a.few_split;
 
     const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
     v8h fq[KS];
@@ -98,7 +148,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
     v4f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
-    for (int kt = piece * a.split + wave; kt < stop; kt += 4) {
+    for (int kt = piece * a.few_split + wave; kt < stop; kt += 4) {
         const int kb = begin + 32 * kt;
         // instruction row i of score tile t is key 8 (i / 4) + 4 t + i % 4: a lane's scores are then of keys 8 quarter + 4 t + 0 .. 3
         const int kk = kb + 8 * (n >> 2) + (n & 3), vk = kb + 8 * quarter;
@@ -125,28 +175,18 @@ __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
         float e[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
-        uint32_t seen = 0xFF;                                              // bit j: this lane's query sees key 8 quarter + j
         const bool masked = __any(kb + 32 > hi_all || kb < lo_all || vbad);
+        const int there = vbad ? 0 : end - vk;                             // positions of this lane's eight that the cache has, for this tile's rows
         bool fix = false;
         if (masked) {
-            seen = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = seen >> j & 1 ? e[j] : -INFINITY;
-            if (vbad && vk < end && vk + 8 > lo_of(t_first) && a.err) *a.err = 1;     // (a page before the window may be gone)
-            // positions behind the cache's last one hold anything: their V is taken as 0.  Infinities and NaN among the others, which some rows may see and
-            // others not, go the long way round
-            uint32_t there = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) there |= (uint32_t)(vk + j < end && !vbad) << j;
+            for (int j = 0; j < 8; j++) e[j] = vk + j >= lo && vk + j < hi && !vbad ? e[j] : -INFINITY;
+            if (vbad && vk < end && vk + 8 > rt.lo_any() && a.err) *a.err = 1;     // (a page before the window may be gone)
+            // what lies behind the cache's last position is taken as 0, and so are infinities and NaN, which some rows may see and others not
             bool any = false;
 #pragma unroll
-            for (int d = 0; d < DT; d++) { fv[d] = only(fv[d], there, false); any |= unbounded(fv[d]); }
+            for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), any);
             fix = __any(any);
-            if (fix)
-#pragma unroll
-                for (int d = 0; d < DT; d++) fv[d] = only(fv[d], 0xFF, true);
         }
         float top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
         top = fmaxf(m, quad_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
@@ -166,42 +206,37 @@ __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
             if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fv[d]), p2, o[d], 0, 0, 0);
         }
         if (fix) {
-            for (int j = 0; j < 32; j++) {                                 // key kb + j, held by the lanes of quarter j / 8
-                const int from = n + 16 * (j >> 3), key = kb + j;
-                float pj = 0.0f;
-                uint32_t sj = 0;
+            uint32_t seen = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) if (i == (j & 7)) pj = e[i];
-                pj = __shfl(pj, from, SPY_WAVE);
-                sj = (uint32_t)__shfl((int)seen, from, SPY_WAVE) >> (j & 7) & 1;
-                if (key >= end || !sj) continue;
-                const int page = table[key >> a.b.page_log2];              // in range: the key is seen
-                const uint8_t *v = a.vp + page * a.vp_g + head * a.vp_h + (key & pmask) * 2;
+            for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
+            const v8h see = ones(seen);
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+            for (int d = 0; d < DT; d++) {
+                const uint4 w = first_of(*(const uint4 *)(vr + 16 * d * a.vp_d), there);
+#pragma nounroll
+                for (int kind = 0; kind < 3; kind++) {
+                    const v4f n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), see, v4f{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint16_t b = *(const uint16_t *)(v + (16 * d + 4 * quarter + i) * a.vp_d);
-                        if ((b & 0x7C00u) == 0x7C00u) o[d][i] += pj * h2f(b);
-                    }
+                    for (int i = 0; i < 4; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
+                }
             }
         }
     }
     l = quad_reduce(l, [](float p, float q) { return p + q; });
-    if (quarter == 0) { s_m[wave][n] = m; s_l[wave][n] = l; }
+    if (quarter == 0) { sh.m[wave][n] = m; sh.l[wave][n] = l; }
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, s_m[w][n]);
+    for (int w = 0; w < 4; w++) top = fmaxf(top, sh.m[w][n]);
     const float shrink = exp2_(m - (top == -INFINITY ? 0.0f : top));
-    float *part = a.part + (int64_t)((int64_t)unit * a.n_split + piece) * 16 * (D + 2);
+    float *part = a.few_part + ((int64_t)unit * a.few_pieces + piece) * 16 * (D + 2);
 #pragma unroll
     for (int h = 0; h < D / HALF; h++) {
         if (h) __syncthreads();
 #pragma unroll
         for (int d = 0; d < HALF / 16; d++) {
             const v4f v = o[h * (HALF / 16) + d] * shrink;
-            *(v4f *)&s_o[wave][n][16 * d + 4 * quarter] = v;
+            *(v4f *)&sh.o[wave][n][16 * d + 4 * quarter] = v;
         }
         __syncthreads();
         for (int i = tid; i < 16 * (HALF / 4); i += 256) {
@@ -209,10 +244,10 @@ __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
             v4f v = v4f{0, 0, 0, 0};
             float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) { v += *(const v4f *)&s_o[w][row][d]; mx = fmaxf(mx, s_m[w][row]); }
+            for (int w = 0; w < 4; w++) { v += *(const v4f *)&sh.o[w][row][d]; mx = fmaxf(mx, sh.m[w][row]); }
             const float base = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-            for (int w = 0; w < 4; w++) sum += s_l[w][row] * exp2_(s_m[w][row] - base);
+            for (int w = 0; w < 4; w++) sum += sh.l[w][row] * exp2_(sh.m[w][row] - base);
             if (r0 + row >= rows) continue;
             const int dd = h * HALF + d;
             if (whole) {
@@ -231,33 +266,319 @@ __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
     }
 }
 
-// The rows whose keys several workgroups shared
-template <int D, bool F32OUT>
-__global__ __launch_bounds__(256) void attn_join_kernel(attn_args a) {
-    const int unit = blockIdx.x, s = unit / (a.tiles * a.G), rest = unit - s * a.tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
+// ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
+// Bound by the matrix cores and, beside them, by the vector instructions of the softmax: 64 keys by 32 rows take a wave 32 matrix instructions of 32 cycles, and
+// (D = 128) 32 exponentials of 16 cycles, 32 fmas and 32 additions of 4, 16 + 16 for maximum and conversion.  Two waves per SIMD, so that one's softmax runs beside the
+// other's products.  Each of the four waves has 32 rows; the 64 keys' K and V^T lie in LDS, requested straight from memory one tile ahead into the other of two
+// buffers.  An LDS row is a row of the matrix instruction's operand (K: instruction row i of 32 is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that
+// a lane's scores are those of 8 keys that follow each other, as the product wants its probabilities); its 16-byte pieces are stored at their index xor a number
+// of the row, so that the lanes of a read meet different banks.
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes per lane from memory to LDS, in lane order from byte `lds` (uniform) on; base uniform, or an address per lane.  Written as instructions so that the compiler does
+// not wait for them at the next LDS read; landed() does.
+static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(addr) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+static __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const uint8_t *)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
+}
+static __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int D> static __device__ __forceinline__ int swizzle_k(int row) { return D == 64 ? (row >> 1 & 3) | (((row ^ row >> 3) & 1) << 2) : row & 15; }
+static __device__ __forceinline__ int swizzle_v(int row) { return (row >> 1 & 3) | (((row ^ row >> 3) & 1) << 2); }
+
+// over the two lanes l, l ^ 32
+template <class Op> static __device__ __forceinline__ float pair_reduce(float v, Op op) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+
+// Tile `left` of the sequences of many rows, one after the other: its sequence and its number there.  64 sequences per round; every lane the same.
+static __device__ __forceinline__ int find_tile(const attn_args &a, int left, int &tile, int &count) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.b.n_seq; base += 64) {
+        int n = 0;
+        if (base + lane < a.b.n_seq) {
+            const pg_seq q = pg_sequence(a.b, base + lane, a.err);
+            const int rows = q.ok ? q.n_new * a.group : 0;
+            n = rows > a.few ? (rows + CHUNK_ROWS - 1) / CHUNK_ROWS : 0;
+        }
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(sum, o, SPY_WAVE); if (lane >= o) sum += v; }
+        const unsigned long long past = __ballot(sum > left);
+        if (past) {
+            const int at = __ffsll(past) - 1;
+            tile = __builtin_amdgcn_readfirstlane(left - __shfl(sum - n, at, SPY_WAVE));
+            count = __builtin_amdgcn_readfirstlane(__shfl(n, at, SPY_WAVE));
+            return __builtin_amdgcn_readfirstlane(base + at);
+        }
+        left -= __shfl(sum, 63, SPY_WAVE);
+    }
+    return -1;
+}
+
+template <int D> struct chunk_shared { __attribute__((aligned(1024))) uint8_t k[2][64 * D * 2], v[2][64 * D * 2]; };
+
+template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(const attn_args &a, chunk_shared<D> &sh, int block) {
+    constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
+    constexpr int KC = D / 8, KR = 64 / KC;                                // 16-byte pieces of a K row, K rows per request
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
+    // heads fastest: a head's tiles run on one XCD where the number of heads is a multiple of 8, and share its L2
+    const int per = a.chunk_tiles * a.G, piece = block / per, unit = block - piece * per, head = unit % a.G;
+    int tile, count;
+    const int s = find_tile(a, unit / a.G, tile, count);
+    if (s < 0) return;
+    tile = count - 1 - tile;                                               // late tiles, which see most keys, first
     const pg_seq sq = pg_sequence(a.b, s, nullptr);
-    if (!sq.ok) return;
-    const int rows = sq.n_new * a.group, r0 = tile * 16;
-    if (r0 >= rows) return;
-    const int past = sq.kv - sq.n_new, t_first = r0 / a.group, t_last = min(r0 + 15, rows - 1) / a.group;
-    const int begin = (a.window > 0 ? max(past + t_first - a.window + 1, 0) : 0) & ~31, end = a.causal ? max(past + t_last + 1, 0) : sq.kv;
-    const int n_tile = max((end - begin + 31) >> 5, 0), pieces = (n_tile + a.split - 1) / a.split;
-    if (pieces <= 1) return;
-    const float *part = a.part + (int64_t)unit * a.n_split * 16 * (D + 2);
+    const row_tile rt(a, sq, tile, CHUNK_ROWS);
+    const int begin = rt.lo_any() & ~63, end = rt.end(), n_tile = max((end - begin + 63) >> 6, 0);
+    const int from = piece * a.chunk_split, stop = min(from + a.chunk_split, n_tile);
+    if (piece > 0 && from >= n_tile) return;
+    const bool whole = n_tile <= a.chunk_split;
+    const int r = min(rt.r0 + wave * 32 + n, rt.rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
+    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all();
+    const bool idle = wave * 32 >= rt.n_row;                               // waves without rows fetch, and compute nothing
+
+    const float c = fabsf(a.c);
+    v8h fq[KS];
+    {
+        const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
+        const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u;               // a negative scale: -q, so that the largest product is the largest score
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            uint4 w = *(const uint4 *)(qrow + (16 * k + 8 * half) * 2);
+            w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+            fq[k] = halves(w);
+        }
+    }
+    const int32_t *table = a.b.pages + (int64_t)s * a.b.page_stride;
+    const int plog = a.b.page_log2, pmask = (1 << plog) - 1, last = (sq.kv - 1) >> plog;
+    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.k[0], lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.v[0];
+
+    // K request i of a wave: LDS rows KR (4 i + wave) .., which are keys of one group of 16.  V request: V^T rows 8 (4 i + wave) .., lane's piece: keys 8 vc .. of the tile
+    uint32_t koff[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int row = KR * (4 * i + wave) + lane / KC;
+        koff[i] = (uint32_t)((8 * (row >> 2 & 1) + 4 * (row >> 3 & 1) + (row & 3)) * (int)a.kp_p + (((lane % KC) ^ swizzle_k<D>(row)) * 16));
+    }
+    const int vrow = 8 * wave + (lane >> 3), vc = (lane & 7) ^ swizzle_v(vrow);
+    const uint8_t *kbase = a.kp + head * a.kp_h, *vbase = a.vp + head * a.vp_h;
+    // pages of the tile's four groups of 16 keys (all the same one, or two, where pages are larger); bit g of `bad`: group g's is not there
+    auto pages_of = [&](int kt) {
+        const int kb = begin + 64 * kt;
+        return make_int4(table[min(kb >> plog, last)], table[min((kb + 16) >> plog, last)], table[min((kb + 32) >> plog, last)], table[min((kb + 48) >> plog, last)]);
+    };
+    auto check = [&](int4 &pg) {
+        int id[4] = {pg.x, pg.y, pg.z, pg.w};
+        int bad = 0;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            id[g] = __builtin_amdgcn_readfirstlane(id[g]);
+            if (id[g] < 0 || id[g] >= a.b.n_page) { id[g] = 0; bad |= 1 << g; }
+        }
+        pg = make_int4(id[0], id[1], id[2], id[3]);
+        return bad;
+    };
+    auto request = [&](int kt, int4 pg, int buf) {
+        const int kb = begin + 64 * kt;
+        const int id[4] = {pg.x, pg.y, pg.z, pg.w};
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int g = D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1);
+            const int page = D == 64 ? (wave >> 1 ? id[(2 * i + 1) & 3] : id[(2 * i) & 3]) : id[g & 3];
+            to_lds(uniform(kbase + page * a.kp_g + ((kb + 16 * g) & pmask) * a.kp_p), koff[i], uniform(lds_k + buf * (64 * D * 2) + (4 * i + wave) * 1024));
+        }
+        if (plog >= 6) {
+            const uint8_t *b = vbase + id[0] * a.vp_g + (kb & pmask) * 2;
+#pragma unroll
+            for (int i = 0; i < NI; i++) to_lds(uniform(b + (int64_t)i * 32 * a.vp_d), (uint32_t)(vrow * (int)a.vp_d + vc * 16), uniform(lds_v + buf * (64 * D * 2) + (4 * i + wave) * 1024));
+        } else {
+            const int mine = vc & 4 ? (vc & 2 ? id[3] : id[2]) : (vc & 2 ? id[1] : id[0]);
+            const uint8_t *b = vbase + mine * a.vp_g + ((kb + 8 * vc) & pmask) * 2 + vrow * a.vp_d;
+#pragma unroll
+            for (int i = 0; i < NI; i++) to_lds(b + (int64_t)i * 32 * a.vp_d, uniform(lds_v + buf * (64 * D * 2) + (4 * i + wave) * 1024));
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    v16f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = v16f{0};
+    auto compute = [&](int kt, int buf, int bad, bool masked) {
+        const int kb = begin + 64 * kt;
+        v16f x[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            x[t] = v16f{0};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v8h fk = *(const v8h *)(sh.k[buf] + (32 * t + n) * (2 * D) + (((2 * k + half) ^ swizzle_k<D>(n)) * 16));
+                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, fq[k], x[t], 0, 0, 0);
+            }
+        }
+        // register 8 s + j of tile t: key 32 t + 16 s + 8 half + j.  This lane's query sees register i's where lies(i, first) holds, first: the register 0's from lo on
+        const int mine = kb + 8 * half;
+        const uint32_t span = max(hi - lo, 0);
+        const auto sees = [&](int i, int first) { return (uint32_t)(first + 16 * (i >> 3) + (i & 7)) < (bad >> (i >> 3) & 1 ? 0u : span); };
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i >> 4][i & 15] = sees(i, mine - lo) ? x[i >> 4][i & 15] : -INFINITY;
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; i++) top = fmaxf(top, x[i >> 4][i & 15]);
+        top = pair_reduce(top, [](float p, float q) { return fmaxf(p, q); }) * c;
+        // m may stay up to 8 below the largest x: probabilities up to 2^8 lose nothing, and o is seldom scaled
+        if (__any(top > m + 8.0f || (m == -INFINITY && top > -INFINITY))) {
+            const float next = fmaxf(m, top), shrink = exp2_(m - (next == -INFINITY ? 0.0f : next));
+            m = next;
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= shrink;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const float e = exp2_(fmaf(x[i >> 4][i & 15], c, -base));
+            x[i >> 4][i & 15] = e;
+            sum += e;
+        }
+        l += sum;
+        const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + (32 * d + n) * 128 + (((2 * k + half) ^ swizzle_v(n)) * 16)); };
+        const auto probs = [&](int k, v8h &p, v8h &p2) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float e = x[k >> 1][8 * (k & 1) + j];
+                p[j] = (_Float16)e;
+                if (F32OUT) p2[j] = (_Float16)(e - (float)p[j]);
+            }
+        };
+        if (!masked) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v8h p, p2;
+                probs(k, p, p2);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const v8h w = halves(v_piece(d, k));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p, o[d], 0, 0, 0);
+                    if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p2, o[d], 0, 0, 0);
+                }
+            }
+            return;
+        }
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v8h p, p2;
+            probs(k, p, p2);
+            const int there = bad >> k & 1 ? 0 : end - (mine + 16 * k);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const v8h w = halves(bounded(first_of(v_piece(d, k), there), any));       // as in attn_few
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p, o[d], 0, 0, 0);
+                if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p2, o[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);                         // one piece after the other: registers
+            }
+        }
+        if (__any(any)) {
+            uint32_t seen = 0;
+            int first = mine - lo;
+            asm("" : "+v"(first));                                         // the comparisons once more, rather than 32 of them kept
+#pragma unroll
+            for (int i = 0; i < 32; i++) seen |= (uint32_t)sees(i, first) << i;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma nounroll
+                for (int kind = 0; kind < 3; kind++) {
+                    v16f n_seen = {0};
+#pragma nounroll
+                    for (int k = 0; k < 4; k++)
+                        n_seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(of_kind(first_of(v_piece(d, k), bad >> k & 1 ? 0 : end - (mine + 16 * k)), kind), ones(seen >> (8 * k) & 0xFF), n_seen, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
+                }
+        }
+    };
+    if (from < stop) {
+        int4 pg = pages_of(from);
+        int bad = check(pg);
+        request(from, pg, 0);
+        int4 next = pages_of(min(from + 1, stop - 1));
+        for (int kt = from; kt < stop; kt++) {
+            const int buf = (kt - from) & 1, kb = begin + 64 * kt;
+            landed();                                                      // this tile is in LDS ...
+            __syncthreads();                                               // ... all of it, and nobody reads the other buffer any more
+            const int bad_now = bad;
+            if (kt + 1 < stop) {
+                bad = check(next);
+                request(kt + 1, next, buf ^ 1);
+                next = pages_of(min(kt + 2, stop - 1));
+            }
+            if (bad_now && a.err) {
+                int wanted = 0;                                            // groups with a position that some row sees (a page before the window may be gone)
+#pragma unroll
+                for (int g = 0; g < 4; g++) wanted |= (kb + 16 * g < end && kb + 16 * g + 16 > rt.lo_any()) << g;
+                if (bad_now & wanted) *a.err = 1;
+            }
+            if (idle) continue;
+            compute(kt, buf, bad_now, kb + 64 > hi_all || kb < lo_all || bad_now);
+        }
+    }
+    l = pair_reduce(l, [](float p, float q) { return p + q; });
+    if (idle || rt.r0 + wave * 32 + n >= rt.rows) return;
+    const int row = wave * 32 + n;
+    if (whole) {
+        uint8_t *dst = a.out + (int64_t)(sq.row0 + token) * a.o_t + (int64_t)hq * a.o_h;
+        const float f = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;     // 0: sees no key
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = 32 * d + 8 * i + 4 * half;
+                const float v0 = o[d][4 * i] * f, v1 = o[d][4 * i + 1] * f, v2 = o[d][4 * i + 2] * f, v3 = o[d][4 * i + 3] * f;
+                if (F32OUT) *(float4 *)(dst + at * 4) = make_float4(v0, v1, v2, v3);
+                else *(uint2 *)(dst + at * 2) = make_uint2(f2h(v0) | (uint32_t)f2h(v1) << 16, f2h(v2) | (uint32_t)f2h(v3) << 16);
+            }
+    } else {
+        float *part = a.chunk_part + ((int64_t)unit * a.chunk_pieces + piece) * CHUNK_ROWS * (D + 2);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(float4 *)(part + row * D + 32 * d + 8 * i + 4 * half) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+        if (half == 0) { part[CHUNK_ROWS * D + row] = m; part[CHUNK_ROWS * D + CHUNK_ROWS + row] = l; }
+    }
+}
+
+// ---- the rows whose keys several workgroups shared: R rows per workgroup, TILE of them to a tile ---------------------------------------
+template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void join_rows(const attn_args &a, const row_tile &rt, const pg_seq &sq, int head, int sub, int pieces, const float *part) {
     for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-        const int row = i / (D / 4), d = (i - row * (D / 4)) * 4;
-        if (r0 + row >= rows) continue;
+        const int row = sub * 16 + i / (D / 4), d = (i % (D / 4)) * 4;
+        if (row >= rt.n_row) continue;
         float mx = -INFINITY, sum = 0.0f;
-        for (int p = 0; p < pieces; p++) mx = fmaxf(mx, part[(int64_t)p * 16 * (D + 2) + 16 * D + row]);
+        for (int p = 0; p < pieces; p++) mx = fmaxf(mx, part[(int64_t)p * TILE * (D + 2) + TILE * D + row]);
         const float base = mx == -INFINITY ? 0.0f : mx;
         v4f v = v4f{0, 0, 0, 0};
         for (int p = 0; p < pieces; p++) {
-            const float *q = part + (int64_t)p * 16 * (D + 2);
-            const float w = exp2_(q[16 * D + row] - base);
-            sum += w * q[16 * D + 16 + row];
+            const float *q = part + (int64_t)p * TILE * (D + 2);
+            const float w = exp2_(q[TILE * D + row] - base);
+            sum += w * q[TILE * D + TILE + row];
             v += w * *(const v4f *)(q + row * D + d);
         }
-        const int t = (r0 + row) / a.group, hh = head * a.group + (r0 + row - t * a.group);
+        const int t = (rt.r0 + row) / a.group, hh = head * a.group + (rt.r0 + row - t * a.group);
         uint8_t *dst = a.out + (int64_t)(sq.row0 + t) * a.o_t + (int64_t)hh * a.o_h;
         const bool none = mx == -INFINITY && sum == 0.0f;
 #pragma unroll
@@ -266,27 +587,71 @@ __global__ __launch_bounds__(256) void attn_join_kernel(attn_args a) {
         else *(uint2 *)(dst + d * 2) = make_uint2(f2h(v[0]) | (uint32_t)f2h(v[1]) << 16, f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
     }
 }
+template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_kernel(attn_args a, int few_units) {
+    if ((int)blockIdx.x < few_units) {
+        const int unit = blockIdx.x, s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
+        const pg_seq sq = pg_sequence(a.b, s, nullptr);
+        if (!sq.ok) return;
+        const row_tile rt(a, sq, tile, 16);
+        if (rt.n_row <= 0 || rt.rows > a.few) return;
+        const int n_tile = max((rt.end() - (rt.lo_any() & ~31) + 31) >> 5, 0), pieces = (n_tile + a.few_split - 1) / a.few_split;
+        if (pieces > 1) join_rows<D, F32OUT, 16>(a, rt, sq, head, 0, pieces, a.few_part + (int64_t)unit * a.few_pieces * 16 * (D + 2));
+        return;
+    }
+    const int b = blockIdx.x - few_units, unit = b / (CHUNK_ROWS / 16), sub = b % (CHUNK_ROWS / 16), head = unit % a.G;
+    int tile, count;
+    const int s = find_tile(a, unit / a.G, tile, count);
+    if (s < 0) return;
+    const pg_seq sq = pg_sequence(a.b, s, nullptr);
+    const row_tile rt(a, sq, count - 1 - tile, CHUNK_ROWS);
+    const int n_tile = max((rt.end() - (rt.lo_any() & ~63) + 63) >> 6, 0), pieces = (n_tile + a.chunk_split - 1) / a.chunk_split;
+    if (pieces > 1) join_rows<D, F32OUT, CHUNK_ROWS>(a, rt, sq, head, sub, pieces, a.chunk_part + (int64_t)unit * a.chunk_pieces * CHUNK_ROWS * (D + 2));
+}
+
+template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
+    __shared__ few_shared<D> sh;
+    attn_few<D, F32OUT>(a, sh, blockIdx.x);
+}
+// Both kinds of sequences in one launch, the chunks first: they take longest, and the single tokens' reads of memory run beside their products
+template <int D, bool F32OUT> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_mixed_kernel(attn_args a) {
+    __shared__ union { few_shared<D> few; chunk_shared<D> chunk; } sh;
+    if ((int)blockIdx.x < a.chunk_blocks) attn_chunk<D, F32OUT>(a, sh.chunk, blockIdx.x);
+    else attn_few<D, F32OUT>(a, sh.few, blockIdx.x - a.chunk_blocks);
+}
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-struct attn_plan { int64_t tiles, units, split, n_split; size_t scratch; };
+#define FEW_ROWS 16
+struct attn_plan { int64_t few_tiles, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
+// `units` tiles by heads and `key_tiles` tiles of keys: key tiles per workgroup so that `want` workgroups get work, `least` of them at least
+static void attn_share(int64_t units, int64_t key_tiles, int64_t want, int64_t least, int64_t &split, int64_t &pieces) {
+    const int64_t n = (want + units - 1) / units;
+    split = (key_tiles + n - 1) / n;
+    if (split < least) split = least;
+    pieces = (key_tiles + split - 1) / split;
+}
 static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *b, attn_plan &p) {
-    SPY_CHECK_ARG(q && k_pages && q->ne[1] > 0 && q->ne[1] <= 65535);
+    SPY_CHECK_ARG(q && k_pages && q->ne[1] > 0 && q->ne[1] <= 65535 && q->ne[2] > 0 && q->ne[2] < (1 << 28));
     int rc = pg_check_batch(b);
     if (!rc) rc = pg_check_pages(k_pages, 1);
     if (rc) return rc;
     const int64_t G = k_pages->ne[2], H = q->ne[1], hd = k_pages->ne[0];
     SPY_CHECK_ARG(G <= 65535 && H % G == 0);
-    const int64_t group = H / G;
-    p.tiles = ((int64_t)b->max_new * group + 15) / 16;
-    p.units = (int64_t)b->n_seq * p.tiles * G;
-    SPY_CHECK_ARG(p.units < (1ll << 30));
+    const int64_t group = H / G, most = (int64_t)b->max_new * group, cu = spy_num_cu();
+    SPY_CHECK_ARG(most < (1ll << 30));
     // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups: as many as fill the card twice over, 256 keys at least
-    const int64_t key_tiles = ((int64_t)b->max_kv + 31) / 32 + 1, want = (2 * (int64_t)spy_num_cu() + p.units - 1) / p.units;
-    p.split = (key_tiles + want - 1) / want;
-    if (p.split < 8) p.split = 8;
-    p.n_split = (key_tiles + p.split - 1) / p.split;
-    if (p.n_split > 65535) { p.n_split = 65535; p.split = (key_tiles + 65534) / 65535; }
-    p.scratch = p.n_split > 1 ? (size_t)(p.units * p.n_split * 16 * (hd + 2) * 4) : 0;
+    p.few_tiles = ((most < FEW_ROWS ? most : FEW_ROWS) + 15) / 16;
+    p.few_units = (int64_t)b->n_seq * p.few_tiles * G;
+    attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 2 * cu, 8, p.few_split, p.few_pieces);
+    p.chunk_tiles = p.chunk_units = 0; p.chunk_split = p.chunk_pieces = 1;
+    if (most > FEW_ROWS) {
+        const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = q->ne[2] * group / CHUNK_ROWS + b->n_seq;
+        p.chunk_tiles = each * b->n_seq < all ? each * b->n_seq : all;
+        p.chunk_units = p.chunk_tiles * G;
+        attn_share(p.chunk_units, ((int64_t)b->max_kv + 63) / 64 + 1, 2 * cu, 8, p.chunk_split, p.chunk_pieces);
+    }
+    SPY_CHECK_ARG(p.few_units * p.few_pieces + p.chunk_units * p.chunk_pieces < (1ll << 30) && p.chunk_units * (CHUNK_ROWS / 16) < (1ll << 30));
+    p.few_bytes = p.few_pieces > 1 ? (size_t)(p.few_units * p.few_pieces * 16 * (hd + 2) * 4) : 0;
+    p.scratch = p.few_bytes + (p.chunk_pieces > 1 ? (size_t)(p.chunk_units * p.chunk_pieces * CHUNK_ROWS * (hd + 2) * 4) : 0);
     return 0;
 }
 
@@ -296,10 +661,12 @@ extern "C" size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, 
 }
 
 template <int D, bool F32OUT> static int attn_launch(const attn_args &a, const attn_plan &p, hipStream_t st) {
-    attn_few_kernel<D, F32OUT><<<dim3((unsigned)p.units, (unsigned)p.n_split), dim3(256), 0, st>>>(a);
-    int rc = SPY_LAUNCH_RC();
-    if (rc || p.n_split == 1) return rc;
-    attn_join_kernel<D, F32OUT><<<dim3((unsigned)p.units), dim3(256), 0, st>>>(a);
+    if (a.chunk_blocks) attn_mixed_kernel<D, F32OUT><<<dim3((unsigned)(a.chunk_blocks + a.few_blocks)), dim3(256), 0, st>>>(a);
+    else attn_few_kernel<D, F32OUT><<<dim3((unsigned)a.few_blocks), dim3(256), 0, st>>>(a);
+    const int rc = SPY_LAUNCH_RC();
+    if (rc || !p.scratch) return rc;
+    const int64_t few = p.few_pieces > 1 ? p.few_units : 0, chunk = p.chunk_pieces > 1 ? p.chunk_units * (CHUNK_ROWS / 16) : 0;
+    attn_join_kernel<D, F32OUT><<<dim3((unsigned)(few + chunk)), dim3(256), 0, st>>>(a, (int)few);
     return SPY_LAUNCH_RC();
 }
 
@@ -313,7 +680,7 @@ extern "C" int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, co
     if (q->type != SPY_HIP_F16 || (out->type != SPY_HIP_F32 && out->type != SPY_HIP_F16)) return SPY_HIP_EUNSUPPORTED;
     const int64_t hd = k_pages->ne[0], ps = k_pages->ne[1], G = k_pages->ne[2], n_row = q->ne[2], H = q->ne[1];
     SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3]);
-    SPY_CHECK_ARG(n_row > 0 && n_row < (1 << 28) && pg_rows_ok(q, hd, H, n_row) && pg_rows_ok(out, hd, H, n_row) && window >= 0 && scale - scale == 0.0f);
+    SPY_CHECK_ARG(pg_rows_ok(q, hd, H, n_row) && pg_rows_ok(out, hd, H, n_row) && window >= 0 && scale - scale == 0.0f && scale != 0.0f);
     if (p.scratch) {
         if (scratch_bytes < p.scratch) return SPY_HIP_ENOSPACE;
         SPY_CHECK_ARG(scratch && ((uintptr_t)scratch & 255) == 0);
@@ -326,7 +693,9 @@ extern "C" int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, co
     a.b.row_start = batch->row_start; a.b.kv_len = batch->kv_len; a.b.pages = batch->pages; a.b.page_stride = batch->page_stride;
     a.b.n_seq = batch->n_seq; a.b.n_row = (int)n_row; a.b.max_new = batch->max_new; a.b.max_kv = batch->max_kv; a.b.n_page = (int)k_pages->ne[3]; a.b.page_log2 = pg_log2(ps);
     a.G = (int)G; a.group = (int)(H / G); a.c = scale * 1.44269504088896341f; a.causal = causal != 0; a.window = window > (1 << 30) ? 0 : window;
-    a.tiles = (int)p.tiles; a.split = (int)p.split; a.n_split = (int)p.n_split; a.part = (float *)scratch; a.err = spy_hip_err_flag_ptr();
+    a.few = FEW_ROWS; a.few_tiles = (int)p.few_tiles; a.few_split = (int)p.few_split; a.few_pieces = (int)p.few_pieces; a.few_blocks = (int)(p.few_units * p.few_pieces);
+    a.chunk_tiles = (int)p.chunk_tiles; a.chunk_split = (int)p.chunk_split; a.chunk_pieces = (int)p.chunk_pieces; a.chunk_blocks = (int)(p.chunk_units * p.chunk_pieces);
+    a.few_part = (float *)scratch; a.chunk_part = (float *)((uint8_t *)scratch + p.few_bytes); a.err = spy_hip_err_flag_ptr();
     hipStream_t st = (hipStream_t)stream;
     const bool f32 = out->type == SPY_HIP_F32;
     if (hd == 64) return f32 ? attn_launch<64, true>(a, p, st) : attn_launch<64, false>(a, p, st);

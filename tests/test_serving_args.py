@@ -64,7 +64,7 @@ def test_append_does_not_support(kw):
 
 
 @pytest.mark.parametrize("kw", INVALID_BATCH + [dict(q=None), dict(out=None), dict(q=rows(3), out=rows(3)), dict(out=rows(4, n_row=9)), dict(out=rows(2)), dict(q=rows(4, hd=64)), dict(q=rows(4, at=0)),
-                                                dict(out=rows(4, at=4100)), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf"))])
+                                                dict(out=rows(4, at=4100)), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0)])
 def test_attention_refuses(kw):
     assert attend(**kw) == H.EINVAL
 
