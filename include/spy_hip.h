@@ -191,7 +191,7 @@ int spy_hip_argmax(void *stream, const float *logits, int64_t n, int32_t *out_in
  *     min_p   those with w >= min_p (0 or less: all; more than 1 counts as 1)
  *     top_p   the fewest whose w add up to top_p times the sum over the tokens that top_k leaves (1 or more: all)
  *   the token drawn is, in order of index, the first kept one at which the running sum of w exceeds uniform * (sum of the kept w).
- * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab < 2^19.  All five settings are device arrays with one value per
+ * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab at most 2^18.  All five settings are device arrays with one value per
  * row; NULL: temperature 1, no top_k, no min_p, no top_p.  uniform is required: numbers in [0, 1) (below 0 and NaN count as 0, 1 and above as the last number before 1).
  * temperature <= 0 (or NaN) takes the first of the largest logits.  -inf and NaN logits are never drawn; where a logit is +inf, all that are +inf have w = 1 and
  * the others 0.  A row without a logit above -inf gives token -1 and probability 0.

@@ -88,7 +88,7 @@ def sample(t=H.F32, n=1000, n_row=3, at=4096, nb=None, uniform=4096, tokens=4096
     return L.spy_hip_sample(None, B(l), B(p) if param else None, tokens, None, 4096, L.spy_hip_sample_scratch_size(B(l)))
 
 
-@pytest.mark.parametrize("kw", [dict(n=0), dict(n_row=0), dict(n=1 << 19), dict(at=0), dict(at=4097), dict(uniform=None), dict(uniform=4098), dict(tokens=None), dict(tokens=4099), dict(param=False),
+@pytest.mark.parametrize("kw", [dict(n=0), dict(n_row=0), dict(n=(1 << 18) + 1), dict(at=0), dict(at=4097), dict(uniform=None), dict(uniform=4098), dict(tokens=None), dict(tokens=4099), dict(param=False),
                                 dict(nb=[4, 4002]), dict(nb=[8, 8000]), dict(ne2=2)])
 def test_sample_refuses(kw):
     assert sample(**kw) == H.EINVAL
