@@ -27,6 +27,7 @@ struct sample_args {
     const uint8_t *logits;
     int64_t stride;
     int n, part, held;                 // vocabulary; a wave's part of a row (a multiple of 256), and how much of it lies in LDS
+    int range_log2;                    // a token's index by this many bits less is below SM_BINS
     const float *temperature, *top_p, *min_p, *uniform;
     const int32_t *top_k;
     int32_t *tokens;
@@ -48,72 +49,75 @@ static __device__ __forceinline__ float logit_of(u64 x) {
 // distance the same way.  The exponential is good to an ulp.
 struct weigher {
     float top, c, c_lo;
-    __device__ __forceinline__ float far(float l) const {                         // of a logit above -inf
+    __device__ __forceinline__ float far(float l) const {                         // -inf: as good as infinitely far
         const float d = fminf(top - l, 3.4e38f);
         return fmaf(d, c, d * c_lo);
     }
     static __device__ __forceinline__ u64 at(float y) {
         const float e = __builtin_amdgcn_exp2f(-y) * 4096.0f;                     // 2^12 and 2^32: 44 bits
-        const uint32_t h = (uint32_t)e;
-        return (u64)h << 32 | (uint32_t)((e - (float)h) * 4294967296.0f);
+        return (u64)(uint32_t)e << 32 | (uint32_t)(__builtin_amdgcn_fractf(e) * 4294967296.0f);
     }
     __device__ __forceinline__ u64 operator()(float l) const { return at(far(l)); }
 };
 
-struct sample_shared {
+struct __attribute__((aligned(16))) sample_shared {      // (the logits lie behind it, read 16 bytes at a time)
     u64 mass[SM_BINS];
     uint32_t count[SM_BINS];
     u64 x[SM_LIST], w[SM_LIST];
-    u64 wave_a[16], wave_min[16], wave_max[16];
-    uint32_t wave_b[16];
+    u64 wave_sum[16], part[16], least[16], most[16];
     float wave_f[16], wave_g[16];
-    u64 pick, pick_mass;
+    u64 pick;
     uint32_t pick_count, n_list;
     int bin;
 };
 
-static __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, SPY_WAVE);
+// Inclusive sums over lanes without LDS: shifts by 1, 2, 4, 8 inside the rows of 16 lanes, then the last lanes of rows 0 and 2, and of row 1, to the rows behind
+template <int CTRL, int ROWS> static __device__ __forceinline__ uint32_t moved(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS> static __device__ __forceinline__ u64 moved(u64 v) { return (u64)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v); }
+template <class T> static __device__ __forceinline__ T row_scan(T v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
     return v;
 }
-// Inclusive sums over the threads of (a, b)
-static __device__ __forceinline__ void block_scan(sample_shared &s, u64 &a, uint32_t &b) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 va = __shfl_up(a, o, SPY_WAVE);
-        const uint32_t vb = __shfl_up(b, o, SPY_WAVE);
-        if (lane >= o) { a += va; b += vb; }
-    }
-    __syncthreads();
-    if (lane == 63) { s.wave_a[wave] = a; s.wave_b[wave] = b; }
-    __syncthreads();
-    for (int w = 0; w < wave; w++) { a += s.wave_a[w]; b += s.wave_b[w]; }
+template <class T> static __device__ __forceinline__ T wave_scan(T v) {
+    v = row_scan(v);
+    v += moved<0x142, 0xA>(v);
+    v += moved<0x143, 0xC>(v);
+    return v;
 }
-// The bin (one per thread: a weights, b tokens) where the running sum -- by_mass -- or count first reaches what is wanted, and both before it.  SM_BINS: none does.
-static __device__ __forceinline__ int find_bin(sample_shared &s, u64 a, uint32_t b, bool by_mass, u64 want, uint32_t &count_before, u64 &mass_before, u64 *all = nullptr) {
+static __device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+static __device__ __forceinline__ u64 of_lane(u64 v, int lane) { return (u64)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane); }
+// Inclusive sum over the threads, and the sum of all.  Two calls have a barrier between them.
+template <class T> static __device__ __forceinline__ T block_scan(sample_shared &s, T v, T &all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_scan(v);
+    if (lane == 63) s.wave_sum[wave] = v;
+    __syncthreads();
+    const T sums = row_scan((T)s.wave_sum[lane & 15]);
+    all = of_lane(sums, 15);
+    return wave ? v + of_lane(sums, wave - 1) : v;
+}
+// The bin (one per thread, v: its weights or its tokens) where the running sum first reaches `want`, and the sum before it.  SM_BINS: none does.
+template <class T> static __device__ __forceinline__ int find_bin(sample_shared &s, T v, T want, T &before, T &all) {
     const int t = threadIdx.x;
-    const u64 a0 = a;
-    const uint32_t b0 = b;
     if (t == 0) s.bin = SM_BINS;
-    block_scan(s, a, b);
-    const bool here = by_mass ? a >= want && a - a0 < want : b >= want && b - b0 < want;
-    if (here) { s.bin = t; s.pick_mass = a - a0; s.pick_count = b - b0; }         // one thread: the sums do not descend
-    if (t == SM_THREADS - 1) s.pick = a;
+    const T upto = block_scan(s, v, all);
+    if (upto >= want && upto - v < want) { s.bin = t; s.pick = upto - v; }        // one thread: the sums do not descend
     __syncthreads();
     const int bin = s.bin;
-    count_before = s.pick_count; mass_before = s.pick_mass;
-    if (all) *all = s.pick;
+    before = (T)s.pick;
     __syncthreads();
     return bin;
 }
 
-// The row: wave w has the logits part * w .. , the first `held` of them in LDS.
+// The row: wave w has the logits part * w .. , a piece of `held` of them in LDS at a time -- all of them up to 32768, else the piece that it looked at last.
 struct sample_row {
     const float *g;
     f4 *lds;                           // this wave's
-    int n, begin, end, held;
+    int n, begin, part, held;          // part and held: multiples of 256
+    int here;                          // the piece in LDS
     bool infinite;                     // the largest logit is +inf: +inf counts as 0 and every other one as -inf
     __device__ __forceinline__ f4 clean(f4 v) const {                             // NaN: never drawn, as -inf
 #pragma unroll
@@ -124,106 +128,83 @@ struct sample_row {
         return v;
     }
     __device__ __forceinline__ f4 fetch(int i) const {                            // logits i .. i + 3, -inf behind the row
-        if (i + 4 <= n) return clean(*(const f4u *)(g + i));
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = i + e < n ? g[i + e] : -INFINITY;
         return clean(v);
     }
-    // f(four logits, index of the first) over the part's logits from `from` on, in memory: four requests at a time
-    template <class F> __device__ __forceinline__ void stream(int from, F f) const {
-        int i = from + 4 * ((int)threadIdx.x & 63);
-        for (const int full = end - 1024; i - 4 * ((int)threadIdx.x & 63) <= full; i += 1024) {
-            f4 v[4];
+    __device__ __forceinline__ int blocks(int piece) const { return min(held, part - piece * held) >> 8; }       // of 256 logits
+    // A piece to LDS, all its requests at once.  What reaches over the end of the row is requested from where the row's last four logits are, and put right afterwards.
+    __device__ __forceinline__ void load(int piece) {
+        const int lane = threadIdx.x & 63, from = begin + piece * held, number = blocks(piece);
+        f4 v[SM_HELD / 256];
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = *(const f4u *)(g + i + 256 * j);
+        for (int j = 0; j < SM_HELD / 256; j++) if (j < number && n >= 4) v[j] = *(const f4u *)(g + min(from + 4 * (lane + 64 * j), n - 4));
 #pragma unroll
-            for (int j = 0; j < 4; j++) f(clean(v[j]), i + 256 * j);
-        }
-        for (; i < end; i += 256) f(fetch(i), i);
+        for (int j = 0; j < SM_HELD / 256; j++) if (j < number && n >= 4) lds[lane + 64 * j] = clean(v[j]);
+        if (from + 256 * number > n)
+#pragma nounroll
+            for (int j = max(0, (n - from) >> 8); j < number; j++) lds[lane + 64 * j] = fetch(from + 4 * (lane + 64 * j));
+        here = piece;
     }
-    // f(logit, index) of the wave's part, four indices in a row per lane; -inf past the end of the row
-    template <class F> __device__ __forceinline__ void each(F f) const {
-        const int lane = threadIdx.x & 63, groups = held / 4;
-        f4 next = lds[lane];
-        for (int i = lane; i < groups; i += 64) {
-            const f4 v = next;
-            next = lds[i + 64 < groups ? i + 64 : lane];
-#pragma unroll
-            for (int e = 0; e < 4; e++) f(v[e], begin + 4 * i + e);
+    // f(four logits, index of the first) of the wave's part, by all lanes of the wave; -inf past the end of the row.  The piece in LDS first.
+    template <class F> __device__ __forceinline__ void groups(F f) {
+        const int lane = threadIdx.x & 63, last = (part - 1) / held, first = here;
+#pragma nounroll
+        for (int k = 0; k <= last; k++) {
+            const int piece = k == 0 ? first : k <= first ? k - 1 : k;
+            if (piece != here) load(piece);
+            const int number = blocks(piece), from = begin + piece * held + 4 * lane;
+            f4 next = lds[lane];
+#pragma nounroll
+            for (int j = 0; j < number; j++) {
+                const f4 v = next;
+                if (j + 1 < number) next = lds[lane + 64 * (j + 1)];
+                f(v, from + 256 * j);
+            }
         }
-        stream(begin + held, [&](f4 v, int i) {
+    }
+    // f(logit, index)
+    template <class F> __device__ __forceinline__ void each(F f) {
+        groups([&](f4 v, int i) {
 #pragma unroll
             for (int e = 0; e < 4; e++) f(v[e], i + e);
         });
     }
 };
 
-// Tokens for which `in` holds, into the list; returns their number, which may be more than the list has room for (it is incomplete then).
-template <class In> static __device__ __forceinline__ uint32_t collect(sample_shared &s, const sample_row &row, const weigher &weigh, In in) {
-    if (threadIdx.x == 0) s.n_list = 0;
-    __syncthreads();
-    row.each([&](float v, int i) {
-        const bool take = in(v, i);
-        const unsigned long long who = __ballot(take);
-        if (who) {
-            uint32_t base = 0;
-            if ((threadIdx.x & 63) == 0) base = atomicAdd(&s.n_list, (uint32_t)__popcll(who));
-            base = __builtin_amdgcn_readfirstlane(base) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            if (take && base < SM_LIST) { s.x[base] = rank_word(v, i); s.w[base] = weigh(v); }
-        }
-    });
-    __syncthreads();
-    const uint32_t m = s.n_list;
-    __syncthreads();
-    return m;
+// Called by every lane of a wave: the token to the list where `take` holds.  n_list counts them all, also those that the list has no room for.
+static __device__ __forceinline__ void append(sample_shared &s, bool take, float v, int i, const weigher &weigh) {
+    const unsigned long long who = __ballot(take);
+    if (!who) return;
+    uint32_t base = 0;
+    if ((threadIdx.x & 63) == 0) base = atomicAdd(&s.n_list, (uint32_t)__popcll(who));
+    base = __builtin_amdgcn_readfirstlane(base) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+    if (take && base < SM_LIST) { s.x[base] = rank_word(v, i); s.w[base] = weigh(v); }
 }
-// Least and greatest of the threads' x
-static __device__ __forceinline__ void block_range(sample_shared &s, u64 &least, u64 &most) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 a = __shfl_xor(least, o, SPY_WAVE), b = __shfl_xor(most, o, SPY_WAVE);
-        least = a < least ? a : least;
-        most = b > most ? b : most;
-    }
-    if (lane == 0) { s.wave_min[wave] = least; s.wave_max[wave] = most; }
-    __syncthreads();
-    for (int w = 0; w < 16; w++) { least = s.wave_min[w] < least ? s.wave_min[w] : least; most = s.wave_max[w] > most ? s.wave_max[w] : most; }
-    __syncthreads();
-}
-static __device__ __forceinline__ int bin_shift(u64 least, u64 most) { return max(0, 64 - __clzll((long long)(most - least)) - 10); }        // 1024 bins from least to most
-
-// The list by rank: s.x and s.w in order, s.mass[r] the weights up to rank r.  Tokens are dealt to bins of X between its ends, of which most hold one or none.
-static __device__ __forceinline__ void rank_list(sample_shared &s, uint32_t m) {
+// The list by rank: s.x and s.w in order, s.mass[r] the weights up to rank r.  bin_of: a bin for a logit of the list, ascending with the rank; most hold one or none.
+template <class Bin> static __device__ __forceinline__ void rank_list(sample_shared &s, uint32_t m, Bin bin_of) {
     const uint32_t t = threadIdx.x;
     const u64 x = t < m ? s.x[t] : 0, w = t < m ? s.w[t] : 0;
-    u64 least = t < m ? x : ~0ull, most = x;
+    const int bin = t < m ? bin_of(x) : 0;
     s.count[t] = 0;
-    block_range(s, least, most);
-    const int shift = bin_shift(least, most), bin = t < m ? (int)((x - least) >> shift) : 0;
-    uint32_t at = 0;
+    __syncthreads();
+    uint32_t at = 0, all;
     if (t < m) at = atomicAdd(&s.count[bin], 1u);
     __syncthreads();
-    u64 none = 0;
-    const uint32_t mine = s.count[t];
-    uint32_t sum = mine;
-    block_scan(s, none, sum);
-    __syncthreads();
-    s.count[t] = sum - mine;                                                      // first place of bin t
+    const uint32_t mine = s.count[t], upto = block_scan(s, mine, all);
+    s.count[t] = upto - mine;                                                     // first place of bin t
     __syncthreads();
     const uint32_t from = s.count[bin], to = bin + 1 < SM_BINS ? s.count[bin + 1] : m;
     if (t < m) s.x[from + at] = x;
     __syncthreads();
     uint32_t rank = from;
-    if (t < m) for (uint32_t i = from; i < to; i++) rank += s.x[i] < x;
+    if (t < m && to - from > 1) for (uint32_t i = from; i < to; i++) rank += s.x[i] < x;
     __syncthreads();
     if (t < m) { s.x[rank] = x; s.w[rank] = w; }
     __syncthreads();
-    u64 upto = t < m ? s.w[t] : 0;
-    uint32_t zero = 0;
-    block_scan(s, upto, zero);
-    s.mass[t] = upto;
+    u64 total;
+    s.mass[t] = block_scan(s, t < m ? s.w[t] : 0ull, total);
     __syncthreads();
 }
 // Rank in the ordered list at which the weights first add up to `want` (they do), by every thread
@@ -247,23 +228,65 @@ static __device__ __forceinline__ u64 draw_at(float u, u64 total) {             
     return __umul64hi(u64s, total) + 1;
 }
 
-// Rank word of the last token kept by a setting that keeps the first tokens up to a count, or up to a sum of weights (reached by those of `in`).
-// upto: the weights from `before` on, up to the found token's.
-template <class In>
-static __device__ __forceinline__ u64 find_last(sample_shared &s, const sample_row &row, const weigher &weigh, In in, bool by_mass, u64 want, u64 before, u64 &upto) {
-    const int t = threadIdx.x;
-    u64 lo = 0, hi = ~0ull;
-    uint32_t m;
-    while ((m = collect(s, row, weigh, [&](float v, int i) { if (!in(v)) return false; const u64 x = rank_word(v, i); return x >= lo && x <= hi; })) > SM_LIST) {
-        // finer bins between the least and the greatest rank word there are
+// The draw from a list of up to 128 tokens that has all that top_k leaves, by one wave: two tokens a lane, ranked by comparing each with all.
+static __device__ __forceinline__ void draw_from_few(const sample_args &a, sample_shared &s, int r, uint32_t m, int k, bool by_mass, float p, u64 last, float u) {
+    const uint32_t lane = threadIdx.x & 63, q = lane + 64;
+    u64 x0 = lane < m ? s.x[lane] : ~0ull, x1 = q < m ? s.x[q] : ~0ull, w0 = lane < m ? s.w[lane] : 0, w1 = q < m ? s.w[q] : 0;
+    uint32_t r0 = 0, r1 = 0;
+    for (uint32_t j = 0; j < m; j++) { const u64 x = s.x[j]; r0 += x < x0; r1 += x < x1; }
+    // in rank order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    if (lane < m) { s.x[r0] = x0; s.w[r0] = w0; }
+    if (q < m) { s.x[r1] = x1; s.w[r1] = w1; }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    x0 = lane < m ? s.x[lane] : ~0ull; x1 = q < m ? s.x[q] : ~0ull; w0 = lane < m ? s.w[lane] : 0; w1 = q < m ? s.w[q] : 0;
+    const u64 upto0 = wave_scan(w0), upto1 = of_lane(upto0, 63) + wave_scan(w1);
+    const auto upto = [&](uint32_t rank) { return rank < 64 ? of_lane(upto0, rank) : of_lane(upto1, rank - 64); };
+    const auto number = [&](bool in0, bool in1) { return (uint32_t)__popcll(__ballot(in0)) + (uint32_t)__popcll(__ballot(in1)); };
+    uint32_t keep = min((uint32_t)k, m);
+    if (by_mass) {
+        const u64 want = share_of(p, upto(keep - 1));
+        keep = min(keep, number(upto0 < want, upto1 < want) + 1);
+    }
+    keep = min(keep, number(lane < m && x0 <= last, q < m && x1 <= last));
+    const u64 total = upto(keep - 1), want = draw_at(u, total);
+    // in order of index: the first with a running sum that reaches `want`
+    u64 sum0 = 0, sum1 = 0;
+    for (uint32_t j = 0; j < keep; j++) {
+        const uint32_t index = (uint32_t)s.x[j];
+        const u64 w = s.w[j];
+        sum0 += index <= (uint32_t)x0 ? w : 0;
+        sum1 += index <= (uint32_t)x1 ? w : 0;
+    }
+    if (lane < keep && sum0 >= want && sum0 - w0 < want) { a.tokens[r] = (int)(uint32_t)x0; if (a.probs) a.probs[r] = (float)((double)w0 / (double)total); }
+    if (q < keep && sum1 >= want && sum1 - w1 < want) { a.tokens[r] = (int)(uint32_t)x1; if (a.probs) a.probs[r] = (float)((double)w1 / (double)total); }
+}
+
+// More tokens than the list has room for in a bin of the distances (`in`): those of them whose rank words are in lo .. hi, a narrower range at every turn, until the
+// list has room.  Finds where a running count or sum reaches `want`, which it leaves as what is wanted of the list; before: the weights before the list, added up.
+template <class In> static __device__ __forceinline__ uint32_t narrow(sample_shared &s, sample_row &row, const weigher &weigh, In in, bool by_mass, u64 &want, u64 &before, u64 &lo, int &fine) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    u64 hi = ~0ull;
+    lo = 0;
+    for (;;) {
         u64 least = ~0ull, most = 0;
         row.each([&](float v, int i) {
             const u64 x = rank_word(v, i);
             if (in(v) && x >= lo && x <= hi) { least = x < least ? x : least; most = x > most ? x : most; }
         });
         s.mass[t] = 0; s.count[t] = 0;
-        block_range(s, least, most);
-        const int shift = bin_shift(least, most);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const u64 a = __shfl_xor(least, o, SPY_WAVE), b = __shfl_xor(most, o, SPY_WAVE);
+            least = a < least ? a : least;
+            most = b > most ? b : most;
+        }
+        if (lane == 0) { s.least[wave] = least; s.most[wave] = most; }
+        __syncthreads();
+        for (int w = 0; w < 16; w++) { least = s.least[w] < least ? s.least[w] : least; most = s.most[w] > most ? s.most[w] : most; }
+        const int shift = max(0, 64 - __clzll((long long)(most - least)) - 10);
         row.each([&](float v, int i) {
             const u64 x = rank_word(v, i);
             if (in(v) && x >= least && x <= most) {
@@ -273,29 +296,33 @@ static __device__ __forceinline__ u64 find_last(sample_shared &s, const sample_r
             }
         });
         __syncthreads();
-        uint32_t cb;
-        u64 mb;
-        const int bin = find_bin(s, s.mass[t], s.count[t], by_mass, want, cb, mb);
-        want -= by_mass ? mb : cb;
-        before += mb;
+        u64 sum, all;
+        const int bin = find_bin(s, by_mass ? s.mass[t] : (u64)s.count[t], want, sum, all);
+        const u64 upto = block_scan(s, s.mass[t], all);
+        if (t == bin) s.pick = upto - s.mass[t];
+        __syncthreads();
+        before += s.pick;
+        want -= sum;
+        const uint32_t m = s.count[bin];
+        __syncthreads();
         lo = least + ((u64)bin << shift);
         hi = lo + ((1ull << shift) - 1);
+        if (m > SM_LIST) continue;
+        fine = max(0, shift - 10);
+        row.each([&](float v, int i) { const u64 x = rank_word(v, i); append(s, in(v) && x >= lo && x <= hi, v, i, weigh); });
+        __syncthreads();
+        if (t == 0) s.n_list = 0;
+        return m;
     }
-    rank_list(s, m);
-    const uint32_t r = by_mass ? rank_of_mass(s, m, want) : (uint32_t)want - 1;
-    const u64 x = s.x[r];
-    upto = before + s.mass[r];
-    __syncthreads();
-    return x;
 }
 
 __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     sample_shared &s = *(sample_shared *)smem;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = blockIdx.x;
     sample_row row;
     row.g = (const float *)(a.logits + r * a.stride);
-    row.n = a.n; row.begin = wave * a.part; row.end = min(row.begin + a.part, a.n); row.held = a.held;
+    row.n = a.n; row.begin = wave * a.part; row.part = a.part; row.held = a.held;
     f4 *const held = (f4 *)(smem + sizeof(sample_shared));
     row.lds = held + wave * (a.held / 4);
     const float temp = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f, u = a.uniform[r];
@@ -304,26 +331,12 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     row.infinite = false;
 
     float own = -INFINITY;                                                        // this thread's maximum
-    const auto take = [&](f4 v, int i) {                                          // i: group of four of the part
-        row.lds[i] = v;
-        own = fmaxf(own, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-    };
-    if (row.begin + a.held <= a.n) {
-        int i = lane;
-        for (; i - lane + 512 <= a.held / 4; i += 512) {                          // eight requests at a time
-            f4 v[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = *(const f4u *)(row.g + row.begin + 4 * (i + 64 * j));
-#pragma unroll
-            for (int j = 0; j < 8; j++) take(row.clean(v[j]), i + 64 * j);
-        }
-        for (; i < a.held / 4; i += 64) take(row.fetch(row.begin + 4 * i), i);
-    } else
-        for (int i = lane; i < a.held / 4; i += 64) take(row.fetch(row.begin + 4 * i), i);
-    row.stream(row.begin + a.held, [&](f4 v, int) { own = fmaxf(own, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))); });
+    row.load(0);
+    row.groups([&](f4 v, int) { own = fmaxf(own, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))); });
     float top = wave_max(own), low = -wave_max(own > -INFINITY ? -own : -INFINITY);
     if (lane == 0) { s.wave_f[wave] = top; s.wave_g[wave] = low; }
     s.count[t] = 0; s.mass[t] = 0;
+    if (t == 0) s.n_list = 0;
     __syncthreads();
     for (int w = 0; w < 16; w++) { top = fmaxf(top, s.wave_f[w]); low = fminf(low, s.wave_g[w]); }
     if (top == -INFINITY) {
@@ -332,17 +345,17 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     }
     if (top == INFINITY) {
         row.infinite = true;
-        for (int i = lane; i < a.held / 4; i += 64) row.lds[i] = row.clean(row.lds[i]);
+        row.load(row.here);
         own = own == INFINITY ? 0.0f : -INFINITY;
         top = low = 0.0f;
     }
     if (!(temp > 0.0f)) {
         if (t == 0) s.bin = 0x7FFFFFFF;
         __syncthreads();
-        if (own == top) {
+        if (__any(own == top)) {
             int first = 0x7FFFFFFF;
             row.each([&](float v, int i) { if (v == top) first = min(first, i); });
-            atomicMin(&s.bin, first);
+            if (own == top) atomicMin(&s.bin, first);
         }
         __syncthreads();
         if (t == 0) { a.tokens[r] = s.bin; if (a.probs) a.probs[r] = 1.0f; }
@@ -361,25 +374,40 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
         if ((double)f < limit) f = nextafterf(f, INFINITY);
         last = (u64)order_word(fminf(f, top)) << 32 | 0xFFFFFFFFu;
     }
-    uint32_t cb;
-    u64 mb;
     if (by_rank && k <= SM_FAST) {
         // a bin of the threads' maxima, between the least and the greatest, by which k of them are counted
         const float scale = top > low ? (SM_BINS - 1) / (top - low) : 0.0f;
         const auto near = [&](float v) { return (int)fminf((top - v) * scale, (float)SM_BINS); };
         if (own > -INFINITY) atomicAdd(&s.count[min(near(own), SM_BINS - 1)], 1u);
         __syncthreads();
-        const int bin = find_bin(s, 0, s.count[t], false, (u64)k, cb, mb);       // SM_BINS: fewer threads than k have a logit, all tokens make the list
-        const uint32_t m = collect(s, row, weigh, [&](float v, int) { return v > -INFINITY && near(v) <= bin; });
+        uint32_t some, number;
+        const int bin = find_bin(s, s.count[t], (uint32_t)k, some, number);
+        // the least of those k or more maxima.  Fewer threads than k have a logit above -inf: all those tokens
+        float limit = own > -INFINITY && near(own) <= bin ? own : INFINITY;
+        limit = bin == SM_BINS ? -3.4028235e38f : -wave_max(-limit);
+        if (lane == 0) s.wave_g[wave] = limit;
+        __syncthreads();
+        for (int w = 0; w < 16; w++) limit = fminf(limit, s.wave_g[w]);
+        row.groups([&](f4 v, int i) {
+            if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= limit)) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++) append(s, v[e] >= limit, v[e], i + e, weigh);
+        });
+        __syncthreads();
+        const uint32_t m = s.n_list;
+        if (m <= 128) {
+            if (wave == 0) draw_from_few(a, s, r, m, k, by_mass, p, last, u);
+            return;
+        }
+        __syncthreads();
+        if (t == 0) s.n_list = 0;
         if (m <= SM_LIST) {
-            rank_list(s, m);
+            const float fine = scale * (float)SM_BINS / (float)(bin + 1);
+            rank_list(s, m, [&](u64 x) { return (int)fminf((top - logit_of(x)) * fine, (float)(SM_BINS - 1)); });
             uint32_t keep = min((uint32_t)k, m);
             if (by_mass) keep = min(keep, rank_of_mass(s, m, share_of(p, s.mass[keep - 1])) + 1);
-            if (t == 0) s.pick_count = 0;
-            __syncthreads();
             // those that min_p leaves: the first ones too
-            const unsigned long long who = __ballot((uint32_t)t < keep && s.x[t] <= last);
-            if (lane == 0 && who) atomicAdd(&s.pick_count, (uint32_t)__popcll(who));
+            if ((uint32_t)t < keep && s.x[t] <= last && ((uint32_t)t + 1 == keep || s.x[t + 1] > last)) s.pick_count = t + 1;
             __syncthreads();
             keep = s.pick_count;
             const u64 total = s.mass[keep - 1], want = draw_at(u, total);
@@ -387,81 +415,160 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
             const u64 x = mine ? s.x[t] : 0, w = mine ? s.w[t] : 0;
             const uint32_t index = (uint32_t)x;
             // in order of index: weights by range of the index, then inside one of the ranges
-            const int range = (int)((u64)index * SM_BINS / (uint32_t)a.n);
+            const int range = (int)(index >> a.range_log2);
             __syncthreads();
             s.mass[t] = 0;
-            if (t == 0) s.n_list = 0;
             __syncthreads();
             if (mine) atomicAdd(&s.mass[range], w);
             __syncthreads();
-            const int in = find_bin(s, s.mass[t], 0, true, want, cb, mb);
+            u64 before, all;
+            const int in = find_bin(s, s.mass[t], want, before, all);
             if (mine && range == in) { const uint32_t at = atomicAdd(&s.n_list, 1u); s.x[at] = index; s.w[at] = w; }
             __syncthreads();
             if (mine && range == in) {
-                u64 upto = mb + w;
+                u64 upto = before + w;
                 for (uint32_t i = 0; i < s.n_list; i++) if (s.x[i] < index) upto += s.w[i];
                 if (upto >= want && upto - w < want) { a.tokens[r] = (int)index; if (a.probs) a.probs[r] = (float)((double)w / (double)total); }
             }
             return;
         }
+        __syncthreads();
         s.count[t] = 0;
         __syncthreads();
     }
+    bool summed = false;                                                          // the kept weights of this wave's part are in s.part
+    const bool flat = weigh.c < 1e-30f;                                           // a temperature by which -inf is not far enough away by itself
     if (by_rank || by_mass) {
-        const auto bin_at = [&](float y) { return (int)fminf(y * 32.0f, (float)(SM_BINS - 1)); };
+        const float reach = (float)(SM_BINS - 1) / 32.0f;                         // distances from here on have one bin together
+        u64 tail = 0;
+        uint32_t n_tail = 0;
+        const bool look = by_rank || flat;                                        // (else -inf adds 0, and nothing is counted)
         row.each([&](float v, int) {
-            if (!(v > -INFINITY)) return;
+            const bool there = (!look) | (v > -INFINITY);
             const float y = weigh.far(v);
-            const int b = bin_at(y);
-            if (by_rank) atomicAdd(&s.count[b], 1u);
-            atomicAdd(&s.mass[b], weigh.at(y));
+            const u64 w = weigh.at(y);
+            if ((y < reach) & there) {
+                const int b = (int)(y * 32.0f);
+                if (by_rank) atomicAdd(&s.count[b], 1u);
+                atomicAdd(&s.mass[b], w);
+            } else if (there) { tail += w; n_tail++; }
         });
+        n_tail = of_lane(wave_scan(n_tail), 63);                                  // (one addition per wave: the same place for all)
+        tail = of_lane(wave_scan(tail), 63);
+        if (lane == 0 && n_tail) { atomicAdd(&s.count[SM_BINS - 1], n_tail); atomicAdd(&s.mass[SM_BINS - 1], tail); }
         __syncthreads();
-        const u64 mass = s.mass[t];
-        const uint32_t count = s.count[t];
+        const u64 mass = s.mass[t], count = s.count[t];
         u64 upto;
-        int bin = find_bin(s, mass, count, false, (u64)k, cb, mb, &upto);
-        if (by_rank && bin < SM_BINS) {                                           // (not: k or fewer tokens have a logit above -inf)
-            const u64 x = find_last(s, row, weigh, [&](float v) { return v > -INFINITY && bin_at(weigh.far(v)) == bin; }, false, (u64)k - cb, mb, upto);
+        const u64 mass_upto = block_scan(s, mass, upto);
+        __syncthreads();
+#pragma nounroll
+        for (int which = by_rank ? 0 : 1; which < (by_mass ? 2 : 1); which++) {   // 0: top_k, 1: top_p
+            u64 want = which ? share_of(p, upto) : (u64)k, before, all;
+            const int bin = find_bin(s, which ? mass : count, want, before, all);
+            if (bin == SM_BINS) continue;                                         // k or fewer tokens have a logit above -inf
+            want -= before;
+            if (t == bin) s.pick = mass_upto - mass;
+            __syncthreads();
+            before = s.pick;
+            // the bin's tokens, and beside them for top_p, which is the last to cut, the weights of the parts in the bins before it, as far as the others leave them
+            const float near = bin * (1.0f / 32.0f), upper = bin == SM_BINS - 1 ? NAN : (bin + 1) * (1.0f / 32.0f);
+            const auto in = [&](float v) { const float y = weigh.far(v); return y >= near && !(y >= upper) && v > -INFINITY; };
+            const float last_l = last == ~0ull ? -INFINITY : logit_of(last);
+            const int last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
+            u64 sum = 0;
+            row.groups([&](f4 v, int i) {
+                float y[4];
+                bool there[4], any = false;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    y[e] = weigh.far(v[e]);
+                    if (flat) y[e] = v[e] > -INFINITY ? y[e] : INFINITY;
+                    there[e] = (y[e] >= near) & !(y[e] >= upper) & (v[e] > -INFINITY);
+                    any |= there[e];
+                }
+                if (__any(any))
+#pragma unroll
+                    for (int e = 0; e < 4; e++) append(s, there[e], v[e], i + e, weigh);
+                if (which) {
+                    bool some = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool before_it = (y[e] < near) & ((v[e] > last_l) | ((v[e] == last_l) & (i + e <= last_i)));
+                        y[e] = before_it ? y[e] : INFINITY;
+                        some |= before_it;
+                    }
+                    if (__any(some))
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum += weigh.at(y[e]);
+                }
+            });
+            sum = of_lane(wave_scan(sum), 63);
+            if (lane == 0) s.part[wave] = sum;
+            __syncthreads();
+            uint32_t m = s.n_list;
+            __syncthreads();
+            if (t == 0) s.n_list = 0;
+            const bool listed = m <= SM_LIST;
+            u64 lo = 0;
+            int fine = 0;
+            if (!listed) { __syncthreads(); m = narrow(s, row, weigh, in, which == 1, want, before, lo, fine); }
+            rank_list(s, m, [&](u64 x) {
+                return listed ? (int)fminf((weigh.far(logit_of(x)) * 32.0f - (float)bin) * (float)SM_BINS, (float)(SM_BINS - 1)) : (int)((x - lo) >> fine);
+            });
+            const uint32_t rank = which ? rank_of_mass(s, m, want) : (uint32_t)want - 1;
+            const u64 x = s.x[rank];
+            upto = before + s.mass[rank];
             last = x < last ? x : last;
-        }
-        if (by_mass) {
-            const u64 want = share_of(p, upto);
-            bin = find_bin(s, mass, count, true, want, cb, mb);
-            u64 unused;
-            const u64 x = find_last(s, row, weigh, [&](float v) { return v > -INFINITY && bin_at(weigh.far(v)) == bin; }, true, want - mb, mb, unused);
-            last = x < last ? x : last;
+            if (which && listed) {
+                if ((uint32_t)t < m && s.x[t] <= last) atomicAdd(&s.part[(uint32_t)s.x[t] / (uint32_t)a.part], s.w[t]);
+                summed = true;
+            }
+            __syncthreads();
         }
     }
     // The kept weights of each wave's part of the row, then inside the part that the random number falls into, by threads
-    const auto weight = [&](float v, int i) -> u64 { return v > -INFINITY && rank_word(v, i) <= last ? weigh(v) : 0; };
-    u64 sum = 0;
-    row.each([&](float v, int i) { sum += weight(v, i); });
-    sum = wave_sum_u64(sum);
-    if (lane == 0) s.wave_min[wave] = sum;
+    const bool all_kept = last == ~0ull;
+    const float last_l = all_kept ? -INFINITY : logit_of(last);
+    const int last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
+    const auto kept = [&](float v, int i) { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); };
+    const auto weight = [&](float v, int i) { return weigh.at(kept(v, i) ? weigh.far(v) : INFINITY); };
+    if (!summed) {
+        u64 sum = 0;
+        if (all_kept && !flat) row.each([&](float v, int) { sum += weigh(v); });  // (-inf adds 0)
+        else
+            row.groups([&](f4 v, int i) {
+                bool in[4], some = false;
+#pragma unroll
+                for (int e = 0; e < 4; e++) { in[e] = kept(v[e], i + e); some |= in[e]; }
+                if (!__any(some)) return;
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += weigh.at(in[e] ? weigh.far(v[e]) : INFINITY);
+            });
+        sum = of_lane(wave_scan(sum), 63);
+        if (lane == 0) s.part[wave] = sum;
+    }
     __syncthreads();
-    u64 total = 0;
-    for (int w = 0; w < 16; w++) total += s.wave_min[w];
-    u64 want = draw_at(u, total);
-    int part = 0;
-    while (part < 15 && want > s.wave_min[part]) want -= s.wave_min[part++];
+    const u64 sums = row_scan(s.part[lane & 15]), total = of_lane(sums, 15), want_all = draw_at(u, total);
+    const int part = __ffsll(__ballot(sums >= want_all)) - 1;                      // the first of the row's 16 lanes
+    const u64 want = want_all - (part ? of_lane(sums, part - 1) : 0);
     const int each = (a.part / 4 + SM_THREADS - 1) / SM_THREADS;                  // groups of four per thread
     const auto group = [&](int i) {                                               // of the part
-        return 4 * i < a.held ? held[part * (a.held / 4) + i] : 4 * i < a.part && part * a.part + 4 * i < a.n ? row.fetch(part * a.part + 4 * i) : f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        return a.held == a.part && 4 * i < a.held ? held[part * (a.held / 4) + i] : 4 * i < a.part ? row.fetch(part * a.part + 4 * i) : f4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     };
-    u64 here = 0;
+    u64 here = 0, whole;
+#pragma nounroll
     for (int j = 0; j < each; j++) {
         const f4 v = group(t * each + j);
 #pragma unroll
         for (int e = 0; e < 4; e++) here += weight(v[e], part * a.part + 4 * (t * each + j) + e);
     }
-    u64 run = here;
-    uint32_t zero = 0;
-    block_scan(s, run, zero);
+    const u64 run = block_scan(s, here, whole);
     if (run >= want && run - here < want) {
         u64 upto = run - here;
+#pragma nounroll
         for (int j = 0; j < each; j++) {
             const f4 v = group(t * each + j);
+#pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = part * a.part + 4 * (t * each + j) + e;
                 const u64 w = weight(v[e], i);
@@ -488,6 +595,8 @@ extern "C" int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const 
     sample_args a;
     a.logits = (const uint8_t *)logits->data; a.stride = logits->nb[1]; a.n = (int)n;
     a.part = (int)((n + 4095) / 4096 * 256); a.held = a.part < SM_HELD ? a.part : SM_HELD;
+    a.range_log2 = 0;
+    while ((n - 1) >> a.range_log2 >= SM_BINS) a.range_log2++;
     a.temperature = param->temperature; a.top_p = param->top_p; a.min_p = param->min_p; a.uniform = param->uniform; a.top_k = param->top_k;
     a.tokens = tokens; a.probs = probs;
     const size_t lds = sizeof(sample_shared) + (size_t)16 * a.held * 4;
