@@ -21,6 +21,8 @@ static __device__ __forceinline__ pg_seq pg_checked(const pg_batch &b, int row0,
     q.ok = sound && q.n_new > 0;
     return q;
 }
+// An entry of an array that no kernel of the call writes, at an index that is the same for the whole wave: read through the scalar cache
+static __device__ __forceinline__ int32_t pg_entry(const int32_t *p, int64_t i) { return *(const __attribute__((address_space(4))) int32_t *)(p + i); }
 static __device__ __forceinline__ pg_seq pg_sequence(const pg_batch &b, int s, int *err) {
     return pg_checked(b, b.row_start[s], b.row_start[s + 1], b.kv_len[s], err);
 }

@@ -113,8 +113,8 @@ static __device__ __forceinline__ float kind_value(int kind) { return kind == 2 
 
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
-// Bound by the bytes of K and V.  The four waves take every fourth tile of 32 keys, straight from memory into the registers of the matrix instruction: nothing is
-// shared between waves before the end.
+// Bound by the bytes of K and V.  The four waves take tiles of 32 keys in turn, straight from memory into the registers of the matrix instruction: nothing is shared
+// between waves before the end.
 template <int D> struct few_shared {
     static constexpr int HALF = D < 128 ? D : 128;
     float m[4][16], l[4][16];
@@ -122,7 +122,7 @@ template <int D> struct few_shared {
 };
 template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(const attn_args &a, few_shared<D> &sh, int block) {
     constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D>::HALF;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, quarter = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quarter = lane >> 4;
     const int units = a.b.n_seq * a.few_tiles * a.G, piece = block / units, unit = block - piece * units;
     const int s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
     const pg_seq sq = pg_sequence(a.b, s, a.err);
@@ -142,29 +142,51 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
 #pragma unroll
     for (int k = 0; k < KS; k++) fq[k] = halves(*(const uint4 *)(qrow + (32 * k + 8 * quarter) * 2));
     const int32_t *table = a.b.pages + (int64_t)s * a.b.page_stride;
-    const int pmask = (1 << a.b.page_log2) - 1, last = (sq.kv - 1) >> a.b.page_log2;
+    const int plog = a.b.page_log2, pmask = (1 << plog) - 1, last = (sq.kv - 1) >> plog;
+
+    // Instruction row i of score tile t is key 8 (i / 4) + 4 t + i % 4: a lane's scores are then of keys 8 quarter + 4 t + 0 .. 3, as the product wants them.
+    const uint8_t *kbase = a.kp + (int64_t)head * a.kp_h + (int64_t)(n & 3) * a.kp_p + quarter * 16, *vbase = a.vp + (int64_t)head * a.vp_h + (int64_t)n * a.vp_d;
+    struct page_pair { int first, second; };                               // of the tile's two groups of 16 keys
+    const auto pages_of = [&](int kt) {
+        const int kb = begin + 32 * min(kt, stop - 1);
+        return page_pair{pg_entry(table, min(kb >> plog, last)), pg_entry(table, min((kb + 16) >> plog, last))};
+    };
+    const auto missing = [&](int page) { return (uint32_t)page >= (uint32_t)a.b.n_page; };
+    const auto place = [&](page_pair g, int q, int64_t step) {             // keys 8 q ..: their page
+        const int page = q & 2 ? g.second : g.first;
+        return (int64_t)(missing(page) ? 0 : page) * step;
+    };
+    uint4 fk[2][KS], fv[DT];
+    const auto load_k = [&](int kt, page_pair g) {
+        const uint8_t *kr = kbase + place(g, n >> 2, a.kp_g) + (int64_t)((begin + 32 * kt + 8 * (n >> 2)) & pmask) * a.kp_p;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) fk[t][k] = *(const uint4 *)(kr + 4 * t * a.kp_p + k * 64);
+    };
+    const auto v_row = [&](int kt, page_pair g) { return vbase + place(g, quarter, a.vp_g) + (int64_t)((begin + 32 * kt + 8 * quarter) & pmask) * 2; };
+    const auto load_v = [&](const uint8_t *vr) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) fv[d] = *(const uint4 *)(vr + 16 * d * a.vp_d);
+    };
 
     float m = -INFINITY, l = 0.0f;
     v4f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
-    for (int kt = piece * a.few_split + wave; kt < stop; kt += 4) {
-        const int kb = begin + 32 * kt;
-        // instruction row i of score tile t is key 8 (i / 4) + 4 t + i % 4: a lane's scores are then of keys 8 quarter + 4 t + 0 .. 3
-        const int kk = kb + 8 * (n >> 2) + (n & 3), vk = kb + 8 * quarter;
-        int kpage = table[min(kk >> a.b.page_log2, last)], vpage = table[min(vk >> a.b.page_log2, last)];
-        const bool kbad = kpage < 0 || kpage >= a.b.n_page, vbad = vpage < 0 || vpage >= a.b.n_page;
-        if (kbad) kpage = 0;
-        if (vbad) vpage = 0;
-        const uint8_t *kr = a.kp + kpage * a.kp_g + head * a.kp_h + (kk & pmask) * a.kp_p + quarter * 16;
-        const uint8_t *vr = a.vp + vpage * a.vp_g + head * a.vp_h + (vk & pmask) * 2 + n * a.vp_d;
-        uint4 fk[2][KS], fv[DT];
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int k = 0; k < KS; k++) fk[t][k] = *(const uint4 *)(kr + t * 4 * a.kp_p + k * 64);
-#pragma unroll
-        for (int d = 0; d < DT; d++) fv[d] = *(const uint4 *)(vr + 16 * d * a.vp_d);
+    // K of the next tile is requested when this one's scores are done with the registers, V^T when the product is: memory always has a tile of each wave to fetch
+    const int first = piece * a.few_split + wave;
+    page_pair pg = {0, 0}, pg1 = {0, 0};
+    if (first < stop) {
+        pg = pages_of(first);
+        pg1 = pages_of(first + 4);
+        load_k(first, pg);
+        load_v(v_row(first, pg));
+    }
+    for (int kt = first; kt < stop; kt += 4) {
+        const page_pair pg2 = pages_of(kt + 8);
+        const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
+        const bool vbad = missing(quarter & 2 ? pg.second : pg.first);
         v4f x[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -172,7 +194,8 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
 #pragma unroll
             for (int k = 0; k < KS; k++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fk[t][k]), fq[k], x[t], 0, 0, 0);
         }
-        float e[8];
+        if (kt + 4 < stop) load_k(kt + 4, pg1);
+        float e[8];                                                        // of this lane's query and keys vk ..
 #pragma unroll
         for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
         const bool masked = __any(kb + 32 > hi_all || kb < lo_all || vbad);
@@ -188,17 +211,22 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
             for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), any);
             fix = __any(any);
         }
-        float top = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+        float top = e[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) top = fmaxf(top, e[j]);
         top = fmaxf(m, quad_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
         const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_(m - base);
         m = top;
         float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) { e[j] = exp2_(e[j] - base); sum += e[j]; }
-        l = l * shrink + sum;
         v8h p, p2;
 #pragma unroll
-        for (int j = 0; j < 8; j++) { p[j] = (_Float16)e[j]; if (F32OUT) p2[j] = (_Float16)(e[j] - (float)p[j]); }
+        for (int j = 0; j < 8; j++) {
+            e[j] = exp2_(e[j] - base);
+            sum += e[j];
+            p[j] = (_Float16)e[j];
+            if (F32OUT) p2[j] = (_Float16)(e[j] - (float)p[j]);
+        }
+        l = l * shrink + sum;
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             o[d] *= shrink;
@@ -212,7 +240,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
             const v8h see = ones(seen);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const uint4 w = first_of(*(const uint4 *)(vr + 16 * d * a.vp_d), there);
+                const uint4 w = first_of(*(const uint4 *)(v_row(kt, pg) + 16 * d * a.vp_d), there);
 #pragma nounroll
                 for (int kind = 0; kind < 3; kind++) {
                     const v4f n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), see, v4f{0, 0, 0, 0}, 0, 0, 0);
@@ -221,6 +249,8 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
                 }
             }
         }
+        if (kt + 4 < stop) load_v(v_row(kt + 4, pg1));
+        pg = pg1; pg1 = pg2;
     }
     l = quad_reduce(l, [](float p, float q) { return p + q; });
     if (quarter == 0) { sh.m[wave][n] = m; sh.l[wave][n] = l; }
@@ -563,28 +593,80 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     }
 }
 
-// ---- the rows whose keys several workgroups shared: R rows per workgroup, TILE of them to a tile ---------------------------------------
+// ---- the rows whose keys several workgroups shared: 16 rows per workgroup ---------------------------------------------------------------
+// Latency: a wave has the (m, l) of four rows, a lane one workgroup's; then eight pieces of o are requested at a time.
 template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void join_rows(const attn_args &a, const row_tile &rt, const pg_seq &sq, int head, int sub, int pieces, const float *part) {
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-        const int row = sub * 16 + i / (D / 4), d = (i % (D / 4)) * 4;
-        if (row >= rt.n_row) continue;
-        float mx = -INFINITY, sum = 0.0f;
-        for (int p = 0; p < pieces; p++) mx = fmaxf(mx, part[(int64_t)p * TILE * (D + 2) + TILE * D + row]);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        v4f v = v4f{0, 0, 0, 0};
-        for (int p = 0; p < pieces; p++) {
-            const float *q = part + (int64_t)p * TILE * (D + 2);
-            const float w = exp2_(q[TILE * D + row] - base);
-            sum += w * q[TILE * D + TILE + row];
-            v += w * *(const v4f *)(q + row * D + d);
-        }
-        const int t = (rt.r0 + row) / a.group, hh = head * a.group + (rt.r0 + row - t * a.group);
-        uint8_t *dst = a.out + (int64_t)(sq.row0 + t) * a.o_t + (int64_t)hh * a.o_h;
-        const bool none = mx == -INFINITY && sum == 0.0f;
+    __shared__ float s_w[16][64], s_sum[16];
+    constexpr int64_t STEP = TILE * (D + 2);
+    constexpr int ITEMS = 16 * (D / 4) / 256;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = min(16, rt.n_row - 16 * sub);
+    if (rows <= 0) return;
+    v4f v[ITEMS], x[ITEMS][8];
+    const auto request = [&](int p) {                                      // the first eight of o from piece p on, for every item of the thread
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = none ? 0.0f : v[k] / sum;
-        if (F32OUT) *(v4f *)(dst + d * 4) = v;
-        else *(uint2 *)(dst + d * 2) = make_uint2(f2h(v[0]) | (uint32_t)f2h(v[1]) << 16, f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+        for (int k = 0; k < ITEMS; k++) {
+            const int i = threadIdx.x + 256 * k, row = i / (D / 4), d = (i % (D / 4)) * 4;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[k][j] = *(const v4f *)(part + min(p + j, pieces - 1) * STEP + (16 * sub + row) * D + d);
+        }
+    };
+    request(0);
+    float top[4], sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = 4 * wave + i;
+        top[i] = -INFINITY; sum[i] = 0.0f;
+        if (row >= rows) continue;
+        for (int p = lane; p < pieces; p += 64) top[i] = fmaxf(top[i], part[p * STEP + TILE * D + 16 * sub + row]);
+        top[i] = wave_max(top[i]);
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) v[k] = v4f{0, 0, 0, 0};
+    for (int base = 0; base < pieces; base += 64) {
+        const int n = min(64, pieces - base);
+        if (base) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 4 * wave + i;
+            if (row >= rows) continue;
+            float w = 0.0f;
+            if (lane < n) {
+                const float *q = part + (base + lane) * STEP + TILE * D + 16 * sub + row;
+                w = exp2_(q[0] - (top[i] == -INFINITY ? 0.0f : top[i]));
+                sum[i] += w * q[TILE];
+            }
+            s_w[row][lane] = w;
+        }
+        __syncthreads();
+        for (int p = 0; p < n; p += 8) {
+            if (base + p) request(base + p);
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++) {
+                const int row = (threadIdx.x + 256 * k) / (D / 4);
+                if (row >= rows) continue;
+#pragma unroll
+                for (int j = 0; j < 8; j++) if (p + j < n) v[k] += s_w[row][p + j] * x[k][j];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float all = wave_sum(sum[i]);
+        if (lane == 0) s_sum[4 * wave + i] = top[i] == -INFINITY && all == 0.0f ? 0.0f : all;      // 0: sees no key
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        const int i = threadIdx.x + 256 * k, row = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (row >= rows) continue;
+        const int r = rt.r0 + 16 * sub + row, t = r / a.group, hh = head * a.group + (r - t * a.group);
+        uint8_t *dst = a.out + (int64_t)(sq.row0 + t) * a.o_t + (int64_t)hh * a.o_h;
+        const float all = s_sum[row];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[k][j] = all == 0.0f ? 0.0f : v[k][j] / all;
+        if (F32OUT) *(v4f *)(dst + d * 4) = v[k];
+        else *(uint2 *)(dst + d * 2) = make_uint2(f2h(v[k][0]) | (uint32_t)f2h(v[k][1]) << 16, f2h(v[k][2]) | (uint32_t)f2h(v[k][3]) << 16);
     }
 }
 template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_kernel(attn_args a, int few_units) {
@@ -608,7 +690,7 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_k
     if (pieces > 1) join_rows<D, F32OUT, CHUNK_ROWS>(a, rt, sq, head, sub, pieces, a.chunk_part + (int64_t)unit * a.chunk_pieces * CHUNK_ROWS * (D + 2));
 }
 
-template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_few_kernel(attn_args a) {
+template <int D, bool F32OUT> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(attn_args a) {
     __shared__ few_shared<D> sh;
     attn_few<D, F32OUT>(a, sh, blockIdx.x);
 }
@@ -625,7 +707,7 @@ struct attn_plan { int64_t few_tiles, few_units, few_split, few_pieces, chunk_ti
 // `units` tiles by heads and `key_tiles` tiles of keys: key tiles per workgroup so that `want` workgroups get work, `least` of them at least
 static void attn_share(int64_t units, int64_t key_tiles, int64_t want, int64_t least, int64_t &split, int64_t &pieces) {
     const int64_t n = (want + units - 1) / units;
-    split = (key_tiles + n - 1) / n;
+    split = n == 1 ? key_tiles : ((key_tiles + n - 1) / n + 2) / 4 * 4;    // four waves' worth
     if (split < least) split = least;
     pieces = (key_tiles + split - 1) / split;
 }
@@ -638,10 +720,11 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
     SPY_CHECK_ARG(G <= 65535 && H % G == 0);
     const int64_t group = H / G, most = (int64_t)b->max_new * group, cu = spy_num_cu();
     SPY_CHECK_ARG(most < (1ll << 30));
-    // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups: as many as fill the card twice over, 256 keys at least
+    // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups.  Few rows: 256 keys at least (one request of 4096 keys,
+    // 32 heads: 20 us, 23.5 with 128 keys), else for six workgroups per compute unit (8 requests of up to 30000: 142 us, 150 with two, 151 with three).
     p.few_tiles = ((most < FEW_ROWS ? most : FEW_ROWS) + 15) / 16;
     p.few_units = (int64_t)b->n_seq * p.few_tiles * G;
-    attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 2 * cu, 8, p.few_split, p.few_pieces);
+    attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 6 * cu, 8, p.few_split, p.few_pieces);
     p.chunk_tiles = p.chunk_units = 0; p.chunk_split = p.chunk_pieces = 1;
     if (most > FEW_ROWS) {
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = q->ne[2] * group / CHUNK_ROWS + b->n_seq;
