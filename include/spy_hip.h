@@ -209,7 +209,7 @@ int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sam
 
 /* ---- a batch of sequences over a cache in pages: no counterpart in the reference, whose caches hold one sequence
  *      (attention.cpp:180-265).  K pages are {hd, page_size, n_kv_head, n_page} and V^T pages {page_size, hd, n_kv_head, n_page}, F16, nb[0] = 2, the other
- *      strides any multiples of 16 bytes (nb[1] at most 2^20), data 16-byte aligned: within a page the layouts of the caches above (rows of K, rows of V^T).  page_size is a power of
+ *      strides any multiples of 16 bytes (nb[1] at most 2^20, nb[3] below 2^32), data 16-byte aligned: within a page the layouts of the caches above (rows of K, rows of V^T).  page_size is a power of
  *      two from 16 to 1024, hd 64, 128 or 256, n_head a multiple of n_kv_head (query head h reads K/V head h / (n_head / n_kv_head)). ----------------- */
 typedef struct spy_hip_paged_batch {
     int32_t n_seq;               /* sequences */

@@ -43,7 +43,7 @@ static inline int pg_check_batch(const spy_hip_paged_batch *b) {
 static inline int pg_check_pages(const spy_hip_tensor *t, int page_dim) {
     SPY_CHECK_ARG(t->data && ((uintptr_t)t->data & 15) == 0 && t->ne[2] > 0 && t->ne[3] > 0 && t->ne[3] < (1ll << 31) && t->nb[0] == 2);
     for (int i = 1; i < 4; i++) SPY_CHECK_ARG(t->nb[i] > 0 && t->nb[i] % 16 == 0);
-    SPY_CHECK_ARG(t->nb[1] <= (1 << 20));                                  // offsets inside a page are 32-bit numbers
+    SPY_CHECK_ARG(t->nb[1] <= (1 << 20) && t->nb[3] < (1ll << 32));         // offsets inside a page are 32-bit numbers, and so is a page's size
     const int64_t ps = t->ne[page_dim], hd = t->ne[1 - page_dim];
     if (t->type != SPY_HIP_F16 || (hd != 64 && hd != 128 && hd != 256) || ps < 16 || ps > 1024 || (ps & (ps - 1))) return SPY_HIP_EUNSUPPORTED;
     return 0;

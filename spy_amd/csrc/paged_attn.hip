@@ -113,15 +113,15 @@ static __device__ __forceinline__ float kind_value(int kind) { return kind == 2 
 
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
-// Bound by the bytes of K and V.  The four waves take tiles of 32 keys in turn, straight from memory into the registers of the matrix instruction: nothing is shared
+// Bound by the bytes of K and V.  The waves take tiles of 32 keys in turn, straight from memory into the registers of the matrix instruction: nothing is shared
 // between waves before the end.
-template <int D> struct few_shared {
+template <int D, int WAVES> struct few_shared {
     static constexpr int HALF = D < 128 ? D : 128;
-    float m[4][16], l[4][16];
-    __attribute__((aligned(16))) float o[4][16][HALF + 4];
+    float m[WAVES][16], l[WAVES][16];
+    __attribute__((aligned(16))) float o[WAVES][16][HALF + 4];
 };
-template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(const attn_args &a, few_shared<D> &sh, int block) {
-    constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D>::HALF;
+template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void attn_few(const attn_args &a, few_shared<D, WAVES> &sh, int block) {
+    constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D, WAVES>::HALF;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quarter = lane >> 4;
     const int units = a.b.n_seq * a.few_tiles * a.G, piece = block / units, unit = block - piece * units;
     const int s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
@@ -179,12 +179,12 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
     page_pair pg = {0, 0}, pg1 = {0, 0};
     if (first < stop) {
         pg = pages_of(first);
-        pg1 = pages_of(first + 4);
+        pg1 = pages_of(first + WAVES);
         load_k(first, pg);
         load_v(v_row(first, pg));
     }
-    for (int kt = first; kt < stop; kt += 4) {
-        const page_pair pg2 = pages_of(kt + 8);
+    for (int kt = first; kt < stop; kt += WAVES) {
+        const page_pair pg2 = pages_of(kt + 2 * WAVES);
         const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
         const bool vbad = missing(quarter & 2 ? pg.second : pg.first);
         v4f x[2];
@@ -194,7 +194,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
 #pragma unroll
             for (int k = 0; k < KS; k++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fk[t][k]), fq[k], x[t], 0, 0, 0);
         }
-        if (kt + 4 < stop) load_k(kt + 4, pg1);
+        if (kt + WAVES < stop) load_k(kt + WAVES, pg1);
         float e[8];                                                        // of this lane's query and keys vk ..
 #pragma unroll
         for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
@@ -249,7 +249,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
                 }
             }
         }
-        if (kt + 4 < stop) load_v(v_row(kt + 4, pg1));
+        if (kt + WAVES < stop) load_v(v_row(kt + WAVES, pg1));
         pg = pg1; pg1 = pg2;
     }
     l = quad_reduce(l, [](float p, float q) { return p + q; });
@@ -257,7 +257,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, sh.m[w][n]);
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, sh.m[w][n]);
     const float shrink = exp2_(m - (top == -INFINITY ? 0.0f : top));
     float *part = a.few_part + ((int64_t)unit * a.few_pieces + piece) * 16 * (D + 2);
 #pragma unroll
@@ -269,15 +269,15 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
             *(v4f *)&sh.o[wave][n][16 * d + 4 * quarter] = v;
         }
         __syncthreads();
-        for (int i = tid; i < 16 * (HALF / 4); i += 256) {
+        for (int i = tid; i < 16 * (HALF / 4); i += 64 * WAVES) {
             const int row = i / (HALF / 4), d = (i - row * (HALF / 4)) * 4;
             v4f v = v4f{0, 0, 0, 0};
             float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) { v += *(const v4f *)&sh.o[w][row][d]; mx = fmaxf(mx, sh.m[w][row]); }
+            for (int w = 0; w < WAVES; w++) { v += *(const v4f *)&sh.o[w][row][d]; mx = fmaxf(mx, sh.m[w][row]); }
             const float base = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-            for (int w = 0; w < 4; w++) sum += sh.l[w][row] * exp2_(sh.m[w][row] - base);
+            for (int w = 0; w < WAVES; w++) sum += sh.l[w][row] * exp2_(sh.m[w][row] - base);
             if (r0 + row >= rows) continue;
             const int dd = h * HALF + d;
             if (whole) {
@@ -298,11 +298,12 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_few(co
 
 // ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
 // Bound by the matrix cores and, beside them, by the vector instructions of the softmax: 64 keys by 32 rows take a wave 32 matrix instructions of 32 cycles, and
-// (D = 128) 32 exponentials of 16 cycles, 32 fmas and 32 additions of 4, 16 + 16 for maximum and conversion.  Two waves per SIMD, so that one's softmax runs beside the
-// other's products.  Each of the four waves has 32 rows; the 64 keys' K and V^T lie in LDS, requested straight from memory one tile ahead into the other of two
-// buffers.  An LDS row is a row of the matrix instruction's operand (K: instruction row i of 32 is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that
-// a lane's scores are those of 8 keys that follow each other, as the product wants its probabilities); its 16-byte pieces are stored at their index xor a number
-// of the row, so that the lanes of a read meet different banks.
+// (D = 128) 32 exponentials of 16 cycles, 32 fmas and 32 additions of 4, 16 + 16 for maximum and conversion.  Four waves have 32 rows each; a second group of four
+// has the same rows and every other tile of keys, so that a SIMD always has a second wave whose products run beside the softmax of the first, to the end of a long row
+// of keys, and adds its (m, l, o) at the end.  (256-wide heads: one group, whose waves have all registers to themselves.)  The 64 keys' K and V^T of a group lie in LDS,
+// requested straight from memory one tile ahead into the other of two buffers.  An LDS row is a row of the matrix instruction's operand (K: instruction row i of 32 is key
+// 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a lane's scores are those of 8 keys that follow each other, as the product wants its
+// probabilities); its 16-byte pieces are stored at their index xor a number of the row, so that the lanes of a read meet different banks.
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 #pragma clang diagnostic push
@@ -321,6 +322,26 @@ static __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
     return (const uint8_t *)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
 }
 static __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+// Arguments are loaded sixteen registers at a time; where they live through the loop over the keys, the compiler runs out of scalar registers, keeps whole groups of
+// sixteen in lanes of a vector register and moves all of one back for each value it needs: 158 of 378 vector instructions per tile.  So the loop's values are scalars
+// of their own, and what is wanted after it is loaded again then (from the kernel's arguments, of which this struct is the first).
+typedef const __attribute__((address_space(4))) attn_args *args_ptr;
+static __device__ __forceinline__ args_ptr args_again() {
+    args_ptr p = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+static __device__ __forceinline__ uint32_t alone(uint32_t v) {
+    uint32_t r;
+    asm volatile("s_mov_b32 %0, %1" : "=s"(r) : "s"(uniform(v)));
+    return r;
+}
+static __device__ __forceinline__ int alone(int v) { return (int)alone((uint32_t)v); }
+template <class T> static __device__ __forceinline__ T *alone(T *p) {
+    const uint8_t *r;
+    asm volatile("s_mov_b64 %0, %1" : "=s"(r) : "s"(uniform((const uint8_t *)p)));
+    return (T *)r;
+}
 static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <int D> static __device__ __forceinline__ int swizzle_k(int row) { return D == 64 ? (row >> 1 & 3) | (((row ^ row >> 3) & 1) << 2) : row & 15; }
@@ -357,12 +378,15 @@ static __device__ __forceinline__ int find_tile(const attn_args &a, int left, in
     return -1;
 }
 
-template <int D> struct chunk_shared { __attribute__((aligned(1024))) uint8_t k[2][64 * D * 2], v[2][64 * D * 2]; };
+static constexpr __host__ __device__ int chunk_groups(int D) { return D == 256 ? 1 : 2; }
+template <int D> struct chunk_group { __attribute__((aligned(1024))) uint8_t k[2][64 * D * 2], v[2][64 * D * 2]; };
+template <int D> struct chunk_shared { chunk_group<D> group[chunk_groups(D)]; int unbounded[chunk_groups(D)][3]; };
 
-template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(const attn_args &a, chunk_shared<D> &sh, int block) {
+template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(const attn_args &a, chunk_shared<D> &shared, int block) {
     constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
-    constexpr int KC = D / 8, KR = 64 / KC;                                // 16-byte pieces of a K row, K rows per request
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, half = lane >> 5;
+    constexpr int KC = D / 8, KR = 64 / KC, GROUPS = chunk_groups(D);      // 16-byte pieces of a K row, K rows per request
+    const int tid = threadIdx.x, lane = tid & 63, wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3, group = wave8 >> 2, n = lane & 31, half = lane >> 5;
+    chunk_group<D> &sh = shared.group[group];
     // heads fastest: a head's tiles run on one XCD where the number of heads is a multiple of 8, and share its L2
     const int per = a.chunk_tiles * a.G, piece = block / per, unit = block - piece * per, head = unit % a.G;
     int tile, count;
@@ -371,13 +395,14 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     tile = count - 1 - tile;                                               // late tiles, which see most keys, first
     const pg_seq sq = pg_sequence(a.b, s, nullptr);
     const row_tile rt(a, sq, tile, CHUNK_ROWS);
-    const int begin = rt.lo_any() & ~63, end = rt.end(), n_tile = max((end - begin + 63) >> 6, 0);
-    const int from = piece * a.chunk_split, stop = min(from + a.chunk_split, n_tile);
+    const int lo_any = alone(rt.lo_any()), begin = lo_any & ~63, end = alone(rt.end()), n_tile = max((end - begin + 63) >> 6, 0);
+    const int from = alone(piece * a.chunk_split), stop = alone(min(from + a.chunk_split, n_tile));
     if (piece > 0 && from >= n_tile) return;
-    const bool whole = n_tile <= a.chunk_split;
+    const bool whole = alone((int)(n_tile <= a.chunk_split));
     const int r = min(rt.r0 + wave * 32 + n, rt.rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
-    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all();
-    const bool idle = wave * 32 >= rt.n_row;                               // waves without rows fetch, and compute nothing
+    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = alone(rt.hi_all()), lo_all = alone(rt.lo_all());
+    const int n_row = alone(rt.n_row), row0 = alone(sq.row0);
+    const bool idle = wave * 32 >= n_row;                                  // waves without rows fetch, and compute nothing
 
     const float c = fabsf(a.c);
     v8h fq[KS];
@@ -391,71 +416,88 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
             fq[k] = halves(w);
         }
     }
-    const int32_t *table = a.b.pages + (int64_t)s * a.b.page_stride;
-    const int plog = a.b.page_log2, pmask = (1 << plog) - 1, last = (sq.kv - 1) >> plog;
-    const uint32_t lds_k = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.k[0], lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.v[0];
+    const int32_t *table = alone(a.b.pages + (int64_t)s * a.b.page_stride);
+    const int plog = alone(a.b.page_log2), pmask = alone((1 << plog) - 1), last = alone((sq.kv - 1) >> plog), n_page = alone(a.b.n_page);
+    const uint32_t lds_k = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.k[0] + wave * 1024),
+                   lds_v = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.v[0] + wave * 1024);
 
-    // K request i of a wave: LDS rows KR (4 i + wave) .., which are keys of one group of 16.  V request: V^T rows 8 (4 i + wave) .., lane's piece: keys 8 vc .. of the tile
+    // K request i of a wave: LDS rows KR (4 i + wave) .., which are keys of one group of 16.  V request: V^T rows 8 (4 i + wave) .., lane's piece: keys 8 vc .. of the tile.
+    // Offsets inside a page are 32-bit numbers.
+    const uint32_t kp_p = alone((uint32_t)a.kp_p), vp_d = alone((uint32_t)a.vp_d), kp_g = alone((uint32_t)a.kp_g), vp_g = alone((uint32_t)a.vp_g);
     uint32_t koff[NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) {
         const int row = KR * (4 * i + wave) + lane / KC;
-        koff[i] = (uint32_t)((8 * (row >> 2 & 1) + 4 * (row >> 3 & 1) + (row & 3)) * (int)a.kp_p + (((lane % KC) ^ swizzle_k<D>(row)) * 16));
+        koff[i] = (8 * (row >> 2 & 1) + 4 * (row >> 3 & 1) + (row & 3)) * kp_p + (((lane % KC) ^ swizzle_k<D>(row)) * 16);
     }
     const int vrow = 8 * wave + (lane >> 3), vc = (lane & 7) ^ swizzle_v(vrow);
-    const uint8_t *kbase = a.kp + head * a.kp_h, *vbase = a.vp + head * a.vp_h;
+    const uint32_t voff = vrow * vp_d + vc * 16;
+    const uint8_t *kbase = alone(a.kp + head * a.kp_h), *vbase = alone(a.vp + head * a.vp_h);
+    int *const err = alone(a.err);
     // pages of the tile's four groups of 16 keys (all the same one, or two, where pages are larger); bit g of `bad`: group g's is not there
-    auto pages_of = [&](int kt) {
-        const int kb = begin + 64 * kt;
-        return make_int4(table[min(kb >> plog, last)], table[min((kb + 16) >> plog, last)], table[min((kb + 32) >> plog, last)], table[min((kb + 48) >> plog, last)]);
+    struct group_pages { int a, b, c, d; };
+    const bool large = plog >= 6;
+    const auto pages_of = [&](int kt) {
+        const int kb = begin + 64 * min(kt, stop - 1);
+        const auto at = [&](int i) { return pg_entry(table, min((kb + 16 * i) >> plog, last)); };
+        if (large) { const int p = at(0); return group_pages{p, p, p, p}; }
+        return group_pages{at(0), at(1), at(2), at(3)};
     };
-    auto check = [&](int4 &pg) {
-        int id[4] = {pg.x, pg.y, pg.z, pg.w};
-        int bad = 0;
+    const auto check = [&](group_pages &g) {
+        const auto one = [&](int &id, int bit) { const bool gone = (uint32_t)id >= (uint32_t)n_page; id = gone ? 0 : id; return gone ? bit : 0; };
+        return one(g.a, 1) | one(g.b, 2) | one(g.c, 4) | one(g.d, 8);
+    };
+    const auto request = [&](int kt, group_pages g, uint32_t buf) {        // buf: bytes of the buffer behind the first
+        const int kb = begin + 64 * kt;
+        if (large) {
+            const uint32_t at = kb & pmask;
+            const uint8_t *k = uniform(kbase + (uint64_t)(uint32_t)g.a * kp_g + at * kp_p), *v = uniform(vbase + (uint64_t)(uint32_t)g.a * vp_g + at * 2);
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            id[g] = __builtin_amdgcn_readfirstlane(id[g]);
-            if (id[g] < 0 || id[g] >= a.b.n_page) { id[g] = 0; bad |= 1 << g; }
+            for (int i = 0; i < NI; i++) to_lds(uniform(k + (D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1)) * 16 * kp_p), koff[i], uniform(lds_k + buf + i * 4096));
+#pragma unroll
+            for (int i = 0; i < NI; i++) to_lds(uniform(v + i * 32 * vp_d), voff, uniform(lds_v + buf + i * 4096));
+            return;
         }
-        pg = make_int4(id[0], id[1], id[2], id[3]);
-        return bad;
-    };
-    auto request = [&](int kt, int4 pg, int buf) {
-        const int kb = begin + 64 * kt;
-        const int id[4] = {pg.x, pg.y, pg.z, pg.w};
 #pragma unroll
         for (int i = 0; i < NI; i++) {
-            const int g = D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1);
-            const int page = D == 64 ? (wave >> 1 ? id[(2 * i + 1) & 3] : id[(2 * i) & 3]) : id[g & 3];
-            to_lds(uniform(kbase + page * a.kp_g + ((kb + 16 * g) & pmask) * a.kp_p), koff[i], uniform(lds_k + buf * (64 * D * 2) + (4 * i + wave) * 1024));
+            const int q = D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1);
+            const uint32_t page = q & 2 ? (q & 1 ? g.d : g.c) : (q & 1 ? g.b : g.a);
+            to_lds(uniform(kbase + (uint64_t)page * kp_g + ((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds_k + buf + i * 4096));
         }
-        if (plog >= 6) {
-            const uint8_t *b = vbase + id[0] * a.vp_g + (kb & pmask) * 2;
+        const uint32_t mine = vc & 4 ? (vc & 2 ? g.d : g.c) : (vc & 2 ? g.b : g.a);
+        const uint8_t *v = vbase + (uint64_t)mine * vp_g + ((kb + 8 * vc) & pmask) * 2 + vrow * vp_d;
 #pragma unroll
-            for (int i = 0; i < NI; i++) to_lds(uniform(b + (int64_t)i * 32 * a.vp_d), (uint32_t)(vrow * (int)a.vp_d + vc * 16), uniform(lds_v + buf * (64 * D * 2) + (4 * i + wave) * 1024));
-        } else {
-            const int mine = vc & 4 ? (vc & 2 ? id[3] : id[2]) : (vc & 2 ? id[1] : id[0]);
-            const uint8_t *b = vbase + mine * a.vp_g + ((kb + 8 * vc) & pmask) * 2 + vrow * a.vp_d;
-#pragma unroll
-            for (int i = 0; i < NI; i++) to_lds(b + (int64_t)i * 32 * a.vp_d, uniform(lds_v + buf * (64 * D * 2) + (4 * i + wave) * 1024));
-        }
+        for (int i = 0; i < NI; i++) to_lds(v + i * 32 * vp_d, uniform(lds_v + buf + i * 4096));
     };
 
     float m = -INFINITY, l = 0.0f;
     v16f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v16f{0};
-    auto compute = [&](int kt, int buf, int bad, bool masked) {
+    int *const sh_unbounded = shared.unbounded[group];                     // of the tiles in turn: three, so that one is cleared while no wave sets or reads it
+    const auto compute = [&](int kt, int buf, int bad, bool masked, int turn) {
         const int kb = begin + 64 * kt;
-        v16f x[2];
+        // LDS answers after some 130 cycles, four times what an instruction that waits for it takes: operands are asked for in order, well before their use, and the
+        // barriers between keep the compiler from moving the requests back to where they are used
+        const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + (32 * d + n) * 128 + (((2 * k + half) ^ swizzle_v(n)) * 16)); };
+        v16f x[2] = {{0}, {0}};
+        uint4 w[2][DT];
+        {
+            constexpr int AHEAD = KS < 8 ? KS : 8;
+            v8h fk[AHEAD];
+            const auto k_piece = [&](int i) { return *(const v8h *)(sh.k[buf] + (32 * (i / KS) + n) * (2 * D) + (((2 * (i % KS) + half) ^ swizzle_k<D>(n)) * 16)); };
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            x[t] = v16f{0};
+            for (int i = 0; i < AHEAD; i++) fk[i] = k_piece(i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const v8h fk = *(const v8h *)(sh.k[buf] + (32 * t + n) * (2 * D) + (((2 * k + half) ^ swizzle_k<D>(n)) * 16));
-                x[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, fq[k], x[t], 0, 0, 0);
+            for (int i = 0; i < 2 * KS; i++) {
+                x[i / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk[i % AHEAD], fq[i % KS], x[i / KS], 0, 0, 0);
+                if (i + AHEAD < 2 * KS) fk[i % AHEAD] = k_piece(i + AHEAD);
+                else if (i + AHEAD < 2 * KS + 2 * DT) w[(i + AHEAD - 2 * KS) / DT][(i + AHEAD - 2 * KS) % DT] = v_piece((i + AHEAD - 2 * KS) % DT, (i + AHEAD - 2 * KS) / DT);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int i = AHEAD; i < 2 * DT; i++) w[i / DT][i % DT] = v_piece(i % DT, i / DT);
         }
         // register 8 s + j of tile t: key 32 t + 16 s + 8 half + j.  This lane's query sees register i's where lies(i, first) holds, first: the register 0's from lo on
         const int mine = kb + 8 * half;
@@ -486,7 +528,6 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
             sum += e;
         }
         l += sum;
-        const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + (32 * d + n) * 128 + (((2 * k + half) ^ swizzle_v(n)) * 16)); };
         const auto probs = [&](int k, v8h &p, v8h &p2) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -495,35 +536,19 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 if (F32OUT) p2[j] = (_Float16)(e - (float)p[j]);
             }
         };
-        if (!masked) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v8h p, p2;
-                probs(k, p, p2);
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const v8h w = halves(v_piece(d, k));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p, o[d], 0, 0, 0);
-                    if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p2, o[d], 0, 0, 0);
-                }
-            }
-            return;
-        }
-        bool any = false;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             v8h p, p2;
             probs(k, p, p2);
-            const int there = bad >> k & 1 ? 0 : end - (mine + 16 * k);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const v8h w = halves(bounded(first_of(v_piece(d, k), there), any));       // as in attn_few
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p, o[d], 0, 0, 0);
-                if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p2, o[d], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);                         // one piece after the other: registers
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p, o[d], 0, 0, 0);
+                if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p2, o[d], 0, 0, 0);
+                if (k < 2) w[k & 1][d] = v_piece(d, k + 2);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (__any(any)) {
+        if (masked && sh_unbounded[turn]) {                                // the infinities and NaN that bound_v took out, from memory
             uint32_t seen = 0;
             int first = mine - lo;
             asm("" : "+v"(first));                                         // the comparisons once more, rather than 32 of them kept
@@ -535,43 +560,84 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 for (int kind = 0; kind < 3; kind++) {
                     v16f n_seen = {0};
 #pragma nounroll
-                    for (int k = 0; k < 4; k++)
-                        n_seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(of_kind(first_of(v_piece(d, k), bad >> k & 1 ? 0 : end - (mine + 16 * k)), kind), ones(seen >> (8 * k) & 0xFF), n_seen, 0, 0, 0);
+                    for (int k = 0; k < 4; k++) {
+                        const int at = mine + 16 * k, page = table[min(at >> plog, last)], there = bad >> k & 1 ? 0 : end - at;
+                        const uint4 v = *(const uint4 *)(vbase + (uint64_t)((uint32_t)page >= (uint32_t)n_page ? 0 : page) * vp_g + (uint32_t)(32 * d + n) * vp_d + (at & pmask) * 2);
+                        n_seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(of_kind(first_of(v, there), kind), ones(seen >> (8 * k) & 0xFF), n_seen, 0, 0, 0);
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
                 }
         }
     };
-    if (from < stop) {
-        int4 pg = pages_of(from);
-        int bad = check(pg);
-        request(from, pg, 0);
-        int4 next = pages_of(min(from + 1, stop - 1));
-        for (int kt = from; kt < stop; kt++) {
-            const int buf = (kt - from) & 1, kb = begin + 64 * kt;
-            landed();                                                      // this tile is in LDS ...
-            __syncthreads();                                               // ... all of it, and nobody reads the other buffer any more
-            const int bad_now = bad;
-            if (kt + 1 < stop) {
-                bad = check(next);
-                request(kt + 1, next, buf ^ 1);
-                next = pages_of(min(kt + 2, stop - 1));
-            }
-            if (bad_now && a.err) {
+    // The pieces of V^T that this wave requested: as in attn_few, positions behind the cache's last one hold anything and are taken as 0, and infinities and NaN, which some
+    // rows may see and others not, as well
+    const auto bound_v = [&](int kt, int buf, int bad, int turn) {
+        const int there = bad >> (vc >> 1) & 1 ? 0 : end - (begin + 64 * kt + 8 * vc);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            uint4 *const v = (uint4 *)(sh.v[buf] + (4 * i + wave) * 1024 + lane * 16);
+            *v = bounded(first_of(*v, there), any);
+        }
+        if (any) sh_unbounded[turn] = 1;
+    };
+    const int steps = (max(stop - from, 0) + GROUPS - 1) / GROUPS;
+    if (steps) {
+        int kt = from + group, bad = 0;
+        group_pages pg = pages_of(kt), next = pages_of(kt + GROUPS);
+        bad = check(pg);
+        if (kt < stop) request(kt, pg, 0);
+        if (tid < 3 * GROUPS) shared.unbounded[0][tid] = 0;
+        __syncthreads();
+        for (int i = 0, turn = 0; i < steps; i++, kt += GROUPS, turn = turn == 2 ? 0 : turn + 1) {
+            const int buf = i & 1, kb = begin + 64 * kt, bad_now = bad;
+            const bool masked = kt < stop && (kb + 64 > hi_all || kb < lo_all || bad_now);
+            landed();                                                      // what this wave requested of this tile is in LDS ...
+            if (masked) bound_v(kt, buf, bad_now, turn);
+            __syncthreads();                                               // ... and all of it, and nobody reads the other buffer any more
+            if (lane == 0) sh_unbounded[turn == 0 ? 2 : turn - 1] = 0;     // the last tile's
+            bad = check(next);
+            if (kt + GROUPS < stop) request(kt + GROUPS, next, (buf ^ 1) * (64 * D * 2));
+            next = pages_of(kt + 2 * GROUPS);
+            if (kt >= stop) continue;
+            if (bad_now && err) {
                 int wanted = 0;                                            // groups with a position that some row sees (a page before the window may be gone)
 #pragma unroll
-                for (int g = 0; g < 4; g++) wanted |= (kb + 16 * g < end && kb + 16 * g + 16 > rt.lo_any()) << g;
-                if (bad_now & wanted) *a.err = 1;
+                for (int g = 0; g < 4; g++) wanted |= (kb + 16 * g < end && kb + 16 * g + 16 > lo_any) << g;
+                if (bad_now & wanted) *err = 1;
             }
-            if (idle) continue;
-            compute(kt, buf, bad_now, kb + 64 > hi_all || kb < lo_all || bad_now);
+            if (!idle) compute(kt, buf, bad_now, masked, turn);
         }
     }
+    if constexpr (GROUPS == 2) {                                           // the second group's share
+        static_assert(sizeof(chunk_shared<D>) >= 4 * (16 * DT + 2) * 256);
+        float *const share = (float *)&shared + wave * (16 * DT + 2) * 64 + lane;
+        __syncthreads();
+        if (group) {
+            share[0] = m;
+            share[64] = l;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) share[(16 * d + i + 2) * 64] = o[d][i];
+        }
+        __syncthreads();
+        if (group) return;
+        const float m2 = share[0], top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top, f = exp2_(m - base), f2 = exp2_(m2 - base);
+        m = top;
+        l = l * f + share[64] * f2;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f + share[(16 * d + i + 2) * 64] * f2;
+    }
     l = pair_reduce(l, [](float p, float q) { return p + q; });
-    if (idle || rt.r0 + wave * 32 + n >= rt.rows) return;
     const int row = wave * 32 + n;
+    if (row >= n_row) return;
+    const args_ptr late = args_again();
     if (whole) {
-        uint8_t *dst = a.out + (int64_t)(sq.row0 + token) * a.o_t + (int64_t)hq * a.o_h;
+        uint8_t *dst = late->out + (int64_t)(row0 + token) * late->o_t + (int64_t)hq * late->o_h;
         const float f = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;     // 0: sees no key
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -583,7 +649,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 else *(uint2 *)(dst + at * 2) = make_uint2(f2h(v0) | (uint32_t)f2h(v1) << 16, f2h(v2) | (uint32_t)f2h(v3) << 16);
             }
     } else {
-        float *part = a.chunk_part + ((int64_t)unit * a.chunk_pieces + piece) * CHUNK_ROWS * (D + 2);
+        float *part = late->chunk_part + ((int64_t)unit * late->chunk_pieces + piece) * CHUNK_ROWS * (D + 2);
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -691,19 +757,19 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_k
 }
 
 template <int D, bool F32OUT> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(attn_args a) {
-    __shared__ few_shared<D> sh;
-    attn_few<D, F32OUT>(a, sh, blockIdx.x);
+    __shared__ few_shared<D, 4> sh;
+    attn_few<D, F32OUT, 4>(a, sh, blockIdx.x);
 }
 // Both kinds of sequences in one launch, the chunks first: they take longest, and the single tokens' reads of memory run beside their products
-template <int D, bool F32OUT> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_mixed_kernel(attn_args a) {
-    __shared__ union { few_shared<D> few; chunk_shared<D> chunk; } sh;
+template <int D, bool F32OUT> __global__ __launch_bounds__(256 * chunk_groups(D)) void attn_mixed_kernel(attn_args a) {
+    __shared__ union { few_shared<D, 4 * chunk_groups(D)> few; chunk_shared<D> chunk; } sh;
     if ((int)blockIdx.x < a.chunk_blocks) attn_chunk<D, F32OUT>(a, sh.chunk, blockIdx.x);
-    else attn_few<D, F32OUT>(a, sh.few, blockIdx.x - a.chunk_blocks);
+    else attn_few<D, F32OUT, 4 * chunk_groups(D)>(a, sh.few, blockIdx.x - a.chunk_blocks);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 #define FEW_ROWS 16
-struct attn_plan { int64_t few_tiles, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
+struct attn_plan { int64_t few, few_tiles, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
 // `units` tiles by heads and `key_tiles` tiles of keys: key tiles per workgroup so that `want` workgroups get work, `least` of them at least
 static void attn_share(int64_t units, int64_t key_tiles, int64_t want, int64_t least, int64_t &split, int64_t &pieces) {
     const int64_t n = (want + units - 1) / units;
@@ -722,11 +788,13 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
     SPY_CHECK_ARG(most < (1ll << 30));
     // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups.  Few rows: 256 keys at least (one request of 4096 keys,
     // 32 heads: 20 us, 23.5 with 128 keys), else for six workgroups per compute unit (8 requests of up to 30000: 142 us, 150 with two, 151 with three).
-    p.few_tiles = ((most < FEW_ROWS ? most : FEW_ROWS) + 15) / 16;
-    p.few_units = (int64_t)b->n_seq * p.few_tiles * G;
-    attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 6 * cu, 8, p.few_split, p.few_pieces);
+    p.few = most > FEW_ROWS && b->n_seq == 1 ? 0 : FEW_ROWS;              // a single sequence that may bring many rows goes one way whatever it brings: no empty launches
+    p.few_tiles = (FEW_ROWS + 15) / 16;
+    p.few_units = p.few ? (int64_t)b->n_seq * p.few_tiles * G : 0;
+    p.few_split = 1; p.few_pieces = 0;
+    if (p.few) attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 6 * cu, 8, p.few_split, p.few_pieces);
     p.chunk_tiles = p.chunk_units = 0; p.chunk_split = p.chunk_pieces = 1;
-    if (most > FEW_ROWS) {
+    if (most > p.few) {
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = q->ne[2] * group / CHUNK_ROWS + b->n_seq;
         p.chunk_tiles = each * b->n_seq < all ? each * b->n_seq : all;
         p.chunk_units = p.chunk_tiles * G;
@@ -744,7 +812,7 @@ extern "C" size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, 
 }
 
 template <int D, bool F32OUT> static int attn_launch(const attn_args &a, const attn_plan &p, hipStream_t st) {
-    if (a.chunk_blocks) attn_mixed_kernel<D, F32OUT><<<dim3((unsigned)(a.chunk_blocks + a.few_blocks)), dim3(256), 0, st>>>(a);
+    if (a.chunk_blocks) attn_mixed_kernel<D, F32OUT><<<dim3((unsigned)(a.chunk_blocks + a.few_blocks)), dim3(256 * chunk_groups(D)), 0, st>>>(a);
     else attn_few_kernel<D, F32OUT><<<dim3((unsigned)a.few_blocks), dim3(256), 0, st>>>(a);
     const int rc = SPY_LAUNCH_RC();
     if (rc || !p.scratch) return rc;
@@ -776,7 +844,7 @@ extern "C" int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, co
     a.b.row_start = batch->row_start; a.b.kv_len = batch->kv_len; a.b.pages = batch->pages; a.b.page_stride = batch->page_stride;
     a.b.n_seq = batch->n_seq; a.b.n_row = (int)n_row; a.b.max_new = batch->max_new; a.b.max_kv = batch->max_kv; a.b.n_page = (int)k_pages->ne[3]; a.b.page_log2 = pg_log2(ps);
     a.G = (int)G; a.group = (int)(H / G); a.c = scale * 1.44269504088896341f; a.causal = causal != 0; a.window = window > (1 << 30) ? 0 : window;
-    a.few = FEW_ROWS; a.few_tiles = (int)p.few_tiles; a.few_split = (int)p.few_split; a.few_pieces = (int)p.few_pieces; a.few_blocks = (int)(p.few_units * p.few_pieces);
+    a.few = (int)p.few; a.few_tiles = (int)p.few_tiles; a.few_split = (int)p.few_split; a.few_pieces = (int)p.few_pieces; a.few_blocks = (int)(p.few_units * p.few_pieces);
     a.chunk_tiles = (int)p.chunk_tiles; a.chunk_split = (int)p.chunk_split; a.chunk_pieces = (int)p.chunk_pieces; a.chunk_blocks = (int)(p.chunk_units * p.chunk_pieces);
     a.few_part = (float *)scratch; a.chunk_part = (float *)((uint8_t *)scratch + p.few_bytes); a.err = spy_hip_err_flag_ptr();
     hipStream_t st = (hipStream_t)stream;
