@@ -297,10 +297,14 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
 }
 
 // ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
-// Bound by the matrix cores and, beside them, by the vector instructions of the softmax: 64 keys by 32 rows take a wave 32 matrix instructions of 32 cycles, and
-// (D = 128) 32 exponentials of 16 cycles, 32 fmas and 32 additions of 4, 16 + 16 for maximum and conversion.  Four waves have 32 rows each; a second group of four
-// has the same rows and every other tile of keys, so that a SIMD always has a second wave whose products run beside the softmax of the first, to the end of a long row
-// of keys, and adds its (m, l, o) at the end.  (256-wide heads: one group, whose waves have all registers to themselves.)  The 64 keys' K and V^T of a group lie in LDS,
+// Bound by the matrix cores and the vector instructions of the softmax together: 64 keys by 32 rows take a wave (D = 128) 32 matrix instructions of 33 cycles, and some 215
+// vector instructions of 4.7, 32 of them exponentials of 11; two waves of a SIMD need 4600 of the 5200 cycles that a step takes.  Measured (128 wide, 32 heads): a prompt of
+// 2048 tokens 57 us, 603 TFLOP/s of what its rows see; 512 tokens on 7680 91 us, 734 TFLOP/s; 16 us of the former are spent outside the loop, by two workgroups one after the
+// other.  Tried and not kept: the next tile's scores computed beside this one's exponentials in one instruction stream (58 and 91 us), a barrier for each group by
+// itself (59 and 98).
+// Four waves have 32 rows each; a second group of four has the same rows and every other tile of keys, so that a SIMD always has a second wave, to the end of a long row
+// of keys, and the groups exchange halves of (m, l, o) at the end (one group of 256 rows would leave the short rows of a prompt's triangle without a second wave).
+// (256-wide heads: one group, whose waves have all registers to themselves.)  The 64 keys' K and V^T of a group lie in LDS,
 // requested straight from memory one tile ahead into the other of two buffers.  An LDS row is a row of the matrix instruction's operand (K: instruction row i of 32 is key
 // 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a lane's scores are those of 8 keys that follow each other, as the product wants its
 // probabilities); its 16-byte pieces are stored at their index xor a number of the row, so that the lanes of a read meet different banks.
@@ -310,11 +314,12 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 #pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from memory to LDS, in lane order from byte `lds` (uniform) on; base uniform, or an address per lane.  Written as instructions so that the compiler does
 // not wait for them at the next LDS read; landed() does.
-static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+// `there` 0: not requested.  (The branch is written out as well: as one of the compiler's it would part the instructions on either side into blocks of their own.)
+static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds, uint32_t there) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, %2\n.Lno%=:" :: "s"(lds), "v"(off), "s"(base), "s"(there) : "memory", "m0", "scc");
 }
-static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(addr) : "memory", "m0");
+static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds, uint32_t there) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, off\n.Lno%=:" :: "s"(lds), "v"(addr), "s"(there) : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 static __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
@@ -354,12 +359,13 @@ template <class Op> static __device__ __forceinline__ float pair_reduce(float v,
 }
 
 // Tile `left` of the sequences of many rows, one after the other: its sequence and its number there.  64 sequences per round; every lane the same.
-static __device__ __forceinline__ int find_tile(const attn_args &a, int left, int &tile, int &count) {
+static __device__ __forceinline__ int find_tile(const attn_args &a, int left, int &tile, int &count, pg_seq &sq) {
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.b.n_seq; base += 64) {
         int n = 0;
+        pg_seq q = {0, 0, 0, false};
         if (base + lane < a.b.n_seq) {
-            const pg_seq q = pg_sequence(a.b, base + lane, a.err);
+            q = pg_sequence(a.b, base + lane, a.err);
             const int rows = q.ok ? q.n_new * a.group : 0;
             n = rows > a.few ? (rows + CHUNK_ROWS - 1) / CHUNK_ROWS : 0;
         }
@@ -368,12 +374,13 @@ static __device__ __forceinline__ int find_tile(const attn_args &a, int left, in
         for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(sum, o, SPY_WAVE); if (lane >= o) sum += v; }
         const unsigned long long past = __ballot(sum > left);
         if (past) {
-            const int at = __ffsll(past) - 1;
-            tile = __builtin_amdgcn_readfirstlane(left - __shfl(sum - n, at, SPY_WAVE));
-            count = __builtin_amdgcn_readfirstlane(__shfl(n, at, SPY_WAVE));
-            return __builtin_amdgcn_readfirstlane(base + at);
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+            tile = left - __builtin_amdgcn_readlane(sum - n, at);
+            count = __builtin_amdgcn_readlane(n, at);
+            sq = {__builtin_amdgcn_readlane(q.row0, at), __builtin_amdgcn_readlane(q.n_new, at), __builtin_amdgcn_readlane(q.kv, at), true};
+            return base + at;
         }
-        left -= __shfl(sum, 63, SPY_WAVE);
+        left -= __builtin_amdgcn_readlane(sum, 63);
     }
     return -1;
 }
@@ -390,10 +397,10 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     // heads fastest: a head's tiles run on one XCD where the number of heads is a multiple of 8, and share its L2
     const int per = a.chunk_tiles * a.G, piece = block / per, unit = block - piece * per, head = unit % a.G;
     int tile, count;
-    const int s = find_tile(a, unit / a.G, tile, count);
+    pg_seq sq;
+    const int s = find_tile(a, unit / a.G, tile, count, sq);
     if (s < 0) return;
     tile = count - 1 - tile;                                               // late tiles, which see most keys, first
-    const pg_seq sq = pg_sequence(a.b, s, nullptr);
     const row_tile rt(a, sq, tile, CHUNK_ROWS);
     const int lo_any = alone(rt.lo_any()), begin = lo_any & ~63, end = alone(rt.end()), n_tile = max((end - begin + 63) >> 6, 0);
     const int from = alone(piece * a.chunk_split), stop = alone(min(from + a.chunk_split, n_tile));
@@ -404,18 +411,6 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     const int n_row = alone(rt.n_row), row0 = alone(sq.row0);
     const bool idle = wave * 32 >= n_row;                                  // waves without rows fetch, and compute nothing
 
-    const float c = fabsf(a.c);
-    v8h fq[KS];
-    {
-        const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
-        const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u;               // a negative scale: -q, so that the largest product is the largest score
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            uint4 w = *(const uint4 *)(qrow + (16 * k + 8 * half) * 2);
-            w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-            fq[k] = halves(w);
-        }
-    }
     const int32_t *table = alone(a.b.pages + (int64_t)s * a.b.page_stride);
     const int plog = alone(a.b.page_log2), pmask = alone((1 << plog) - 1), last = alone((sq.kv - 1) >> plog), n_page = alone(a.b.n_page);
     const uint32_t lds_k = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.k[0] + wave * 1024),
@@ -431,61 +426,74 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
         koff[i] = (8 * (row >> 2 & 1) + 4 * (row >> 3 & 1) + (row & 3)) * kp_p + (((lane % KC) ^ swizzle_k<D>(row)) * 16);
     }
     const int vrow = 8 * wave + (lane >> 3), vc = (lane & 7) ^ swizzle_v(vrow);
-    const uint32_t voff = vrow * vp_d + vc * 16;
     const uint8_t *kbase = alone(a.kp + head * a.kp_h), *vbase = alone(a.vp + head * a.vp_h);
     int *const err = alone(a.err);
-    // pages of the tile's four groups of 16 keys (all the same one, or two, where pages are larger); bit g of `bad`: group g's is not there
-    struct group_pages { int a, b, c, d; };
-    const bool large = plog >= 6;
-    const auto pages_of = [&](int kt) {
-        const int kb = begin + 64 * min(kt, stop - 1);
-        const auto at = [&](int i) { return pg_entry(table, min((kb + 16 * i) >> plog, last)); };
-        if (large) { const int p = at(0); return group_pages{p, p, p, p}; }
-        return group_pages{at(0), at(1), at(2), at(3)};
+    // Pages of the tiles' groups of 16 keys: 64 groups, which are 16 tiles, in the lanes of a register, and bit g of `gone`: group g's is not there
+    const auto entries_of = [&](int tile) __attribute__((always_inline)) { return ((const __attribute__((address_space(1))) int32_t *)table)[min((begin + 64 * (from + (tile & ~15)) + 16 * lane) >> plog, last)]; };
+    uint64_t gone = 0;
+    int entries = 0;
+    const auto take_entries = [&](int fetched) __attribute__((always_inline)) {
+        const bool absent = (uint32_t)fetched >= (uint32_t)n_page;
+        gone = __ballot(absent);
+        entries = absent ? 0 : fetched;
     };
-    const auto check = [&](group_pages &g) {
-        const auto one = [&](int &id, int bit) { const bool gone = (uint32_t)id >= (uint32_t)n_page; id = gone ? 0 : id; return gone ? bit : 0; };
-        return one(g.a, 1) | one(g.b, 2) | one(g.c, 4) | one(g.d, 8);
-    };
-    const auto request = [&](int kt, group_pages g, uint32_t buf) {        // buf: bytes of the buffer behind the first
-        const int kb = begin + 64 * kt;
-        if (large) {
-            const uint32_t at = kb & pmask;
-            const uint8_t *k = uniform(kbase + (uint64_t)(uint32_t)g.a * kp_g + at * kp_p), *v = uniform(vbase + (uint64_t)(uint32_t)g.a * vp_g + at * 2);
+    const int first_pages = entries_of(0);                                 // asked for before the queries, which are waited for later
+    const float c = fabsf(a.c);
+    v8h fq[KS];
+    {
+        const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
+        const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u;               // a negative scale: -q, so that the largest product is the largest score
 #pragma unroll
-            for (int i = 0; i < NI; i++) to_lds(uniform(k + (D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1)) * 16 * kp_p), koff[i], uniform(lds_k + buf + i * 4096));
-#pragma unroll
-            for (int i = 0; i < NI; i++) to_lds(uniform(v + i * 32 * vp_d), voff, uniform(lds_v + buf + i * 4096));
-            return;
+        for (int k = 0; k < KS; k++) {
+            uint4 w = *(const uint4 *)(qrow + (16 * k + 8 * half) * 2);
+            w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+            fq[k] = halves(w);
         }
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int q = D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1);
-            const uint32_t page = q & 2 ? (q & 1 ? g.d : g.c) : (q & 1 ? g.b : g.a);
-            to_lds(uniform(kbase + (uint64_t)page * kp_g + ((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds_k + buf + i * 4096));
-        }
-        const uint32_t mine = vc & 4 ? (vc & 2 ? g.d : g.c) : (vc & 2 ? g.b : g.a);
-        const uint8_t *v = vbase + (uint64_t)mine * vp_g + ((kb + 8 * vc) & pmask) * 2 + vrow * vp_d;
-#pragma unroll
-        for (int i = 0; i < NI; i++) to_lds(v + i * 32 * vp_d, uniform(lds_v + buf + i * 4096));
+    }
+    typedef int group_pages __attribute__((ext_vector_type(4)));           // (a struct's members, chosen from by the lane, would be put into memory)
+    const auto pages_of = [&](int tile) __attribute__((always_inline)) {
+        const int g = 4 * tile & 63;
+        return group_pages{__builtin_amdgcn_readlane(entries, g), __builtin_amdgcn_readlane(entries, g + 1), __builtin_amdgcn_readlane(entries, g + 2), __builtin_amdgcn_readlane(entries, g + 3)};
     };
+    const auto gone_of = [&](int tile) __attribute__((always_inline)) { return (int)(gone >> (4 * tile & 63)) & 15; };
+    // Request i of NI; buf: bytes of the buffer behind the first
+    const auto ask_k = [&](int kb, group_pages g, uint32_t buf, uint32_t there, int i) __attribute__((always_inline)) {
+        const int q = D == 128 ? i : D == 256 ? i >> 1 : 2 * i + (wave >> 1);
+        const uint32_t page = q & 2 ? (q & 1 ? g.w : g.z) : (q & 1 ? g.y : g.x);
+        to_lds(uniform(kbase + (uint64_t)page * kp_g + ((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds_k + buf + i * 4096), there);
+    };
+    const auto v_source = [&](int kb, group_pages g) __attribute__((always_inline)) {
+        const uint32_t mine = vc & 4 ? (vc & 2 ? g.w : g.z) : (vc & 2 ? g.y : g.x);
+        return vbase + (uint64_t)mine * vp_g + (((kb + 8 * vc) & pmask) * 2 + vrow * vp_d);
+    };
+    const auto there_is = [&](int kt) {                                    // a tile kt
+        uint32_t yes;
+        // written out: the compiler drops the builtin, and then keeps the number in a vector register.  The register that it reads may not be written by the instruction before.
+        asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1" : "=s"(yes) : "v"((kt - stop) >> 31));
+        return yes;
+    };
+    const auto ask_v = [&](const uint8_t *source, uint32_t buf, uint32_t there, int i) __attribute__((always_inline)) { to_lds(source + i * 32 * vp_d, uniform(lds_v + buf + i * 4096), there); };
 
     float m = -INFINITY, l = 0.0f;
     v16f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v16f{0};
+    constexpr uint32_t BUF = 64 * D * 2;                                   // bytes of one buffer
     int *const sh_unbounded = shared.unbounded[group];                     // of the tiles in turn: three, so that one is cleared while no wave sets or reads it
-    const auto compute = [&](int kt, int buf, int bad, bool masked, int turn) {
+    uint32_t k_at = n * (2 * D) + (half ^ swizzle_k<D>(n)) * 16, v_at = n * 128 + (half ^ swizzle_v(n)) * 16;     // this lane's pieces in LDS
+    const auto compute = [&](int kt, int buf, int bad, bool masked, int turn, group_pages next) {
         const int kb = begin + 64 * kt;
+        const uint32_t more = there_is(kt + GROUPS);
         // LDS answers after some 130 cycles, four times what an instruction that waits for it takes: operands are asked for in order, well before their use, and the
         // barriers between keep the compiler from moving the requests back to where they are used
-        const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + (32 * d + n) * 128 + (((2 * k + half) ^ swizzle_v(n)) * 16)); };
+        asm volatile("" : "+v"(k_at), "+v"(v_at));                         // (addresses once more for every tile: the compiler would keep all of them, in registers that it has not)
+        const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + d * 4096 + (v_at ^ k * 32)); };
         v16f x[2] = {{0}, {0}};
         uint4 w[2][DT];
         {
             constexpr int AHEAD = KS < 8 ? KS : 8;
             v8h fk[AHEAD];
-            const auto k_piece = [&](int i) { return *(const v8h *)(sh.k[buf] + (32 * (i / KS) + n) * (2 * D) + (((2 * (i % KS) + half) ^ swizzle_k<D>(n)) * 16)); };
+            const auto k_piece = [&](int i) { return *(const v8h *)(sh.k[buf] + (i / KS) * 64 * D + (k_at ^ (i % KS) * 32)); };
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) fk[i] = k_piece(i);
             __builtin_amdgcn_sched_barrier(0);
@@ -494,6 +502,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 x[i / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk[i % AHEAD], fq[i % KS], x[i / KS], 0, 0, 0);
                 if (i + AHEAD < 2 * KS) fk[i % AHEAD] = k_piece(i + AHEAD);
                 else if (i + AHEAD < 2 * KS + 2 * DT) w[(i + AHEAD - 2 * KS) / DT][(i + AHEAD - 2 * KS) % DT] = v_piece((i + AHEAD - 2 * KS) % DT, (i + AHEAD - 2 * KS) / DT);
+                if (i % 4 == 0) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, more, i / 4);        // the next tile's, one at a time: all at once, they take 1000 cycles to issue
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -525,9 +534,10 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
         for (int i = 0; i < 32; i++) {
             const float e = exp2_(fmaf(x[i >> 4][i & 15], c, -base));
             x[i >> 4][i & 15] = e;
-            sum += e;
+            if (F32OUT) sum += e;
         }
         l += sum;
+        const uint8_t *const v_from = v_source(kb + 64 * GROUPS, next);
         const auto probs = [&](int k, v8h &p, v8h &p2) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -540,11 +550,18 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
         for (int k = 0; k < 4; k++) {
             v8h p, p2;
             probs(k, p, p2);
+            if (!F32OUT) {                                                 // the sum of what the product takes, two at a time
+                typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+                const v2h one = {1, 1};
+#pragma unroll
+                for (int j = 0; j < 4; j++) l = __builtin_amdgcn_fdot2((v2h){p[2 * j], p[2 * j + 1]}, one, l, false);
+            }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p, o[d], 0, 0, 0);
                 if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p2, o[d], 0, 0, 0);
                 if (k < 2) w[k & 1][d] = v_piece(d, k + 2);
+                if (d % 4 == 0) ask_v(v_from, (buf ^ 1) * BUF, more, (k * DT + d) / 4);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -584,53 +601,77 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     };
     const int steps = (max(stop - from, 0) + GROUPS - 1) / GROUPS;
     if (steps) {
-        int kt = from + group, bad = 0;
-        group_pages pg = pages_of(kt), next = pages_of(kt + GROUPS);
-        bad = check(pg);
-        if (kt < stop) request(kt, pg, 0);
+        int kt = from + group, i = 0, turn = 0, fetched = 0;               // (tiles are numbered from `from` on where their pages are looked up)
+        take_entries(first_pages);
+        int bad = gone_of(group);
+        {
+            const group_pages now = pages_of(group);
+            const uint8_t *const v_from = v_source(begin + 64 * kt, now);
+#pragma unroll
+            for (int j = 0; j < NI; j++) ask_k(begin + 64 * kt, now, 0, there_is(kt), j);
+#pragma unroll
+            for (int j = 0; j < NI; j++) ask_v(v_from, 0, there_is(kt), j);
+        }
         if (tid < 3 * GROUPS) shared.unbounded[0][tid] = 0;
         __syncthreads();
-        for (int i = 0, turn = 0; i < steps; i++, kt += GROUPS, turn = turn == 2 ? 0 : turn + 1) {
-            const int buf = i & 1, kb = begin + 64 * kt, bad_now = bad;
-            const bool masked = kt < stop && (kb + 64 > hi_all || kb < lo_all || bad_now);
+        const auto step = [&](auto idle_) __attribute__((always_inline)) { // one tile; true: it was the last
+            const int buf = i & 1, kb = begin + 64 * kt;
+            const bool masked = kt < stop && (kb + 64 > hi_all || kb < lo_all || bad);
             landed();                                                      // what this wave requested of this tile is in LDS ...
-            if (masked) bound_v(kt, buf, bad_now, turn);
+            if (masked) bound_v(kt, buf, bad, turn);
             __syncthreads();                                               // ... and all of it, and nobody reads the other buffer any more
             if (lane == 0) sh_unbounded[turn == 0 ? 2 : turn - 1] = 0;     // the last tile's
-            bad = check(next);
-            if (kt + GROUPS < stop) request(kt + GROUPS, next, (buf ^ 1) * (64 * D * 2));
-            next = pages_of(kt + 2 * GROUPS);
-            if (kt >= stop) continue;
-            if (bad_now && err) {
+            const int ahead = kt - from + GROUPS;
+            if ((ahead & 15) == group) take_entries(fetched);
+            if ((ahead + GROUPS & 15) == group) fetched = entries_of(ahead + GROUPS);
+            const group_pages next = pages_of(ahead);
+            if (kt < stop && bad && err) {
                 int wanted = 0;                                            // groups with a position that some row sees (a page before the window may be gone)
 #pragma unroll
                 for (int g = 0; g < 4; g++) wanted |= (kb + 16 * g < end && kb + 16 * g + 16 > lo_any) << g;
-                if (bad_now & wanted) *err = 1;
+                if (bad & wanted) *err = 1;
             }
-            if (!idle) compute(kt, buf, bad_now, masked, turn);
-        }
+            if constexpr (idle_) {
+                const uint8_t *const v_from = v_source(kb + 64 * GROUPS, next);
+#pragma unroll
+                for (int j = 0; j < NI; j++) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
+#pragma unroll
+                for (int j = 0; j < NI; j++) ask_v(v_from, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
+            } else if (kt < stop) compute(kt, buf, bad, masked, turn, next);
+            bad = gone_of(ahead);
+            kt += GROUPS;
+            turn = turn == 2 ? 0 : turn + 1;
+            return ++i == steps;
+        };
+        // (a loop of their own for waves without rows: a branch around the products in one loop for both costs registers)
+        if (idle) while (!step(std::true_type{})) {}
+        else while (!step(std::false_type{})) {}
     }
-    if constexpr (GROUPS == 2) {                                           // the second group's share
-        static_assert(sizeof(chunk_shared<D>) >= 4 * (16 * DT + 2) * 256);
-        float *const share = (float *)&shared + wave * (16 * DT + 2) * 64 + lane;
+    constexpr int HAVE = DT / GROUPS;                                      // output tiles that this wave has in the end, from `d0` on
+    const int d0 = group * HAVE;
+    if constexpr (GROUPS == 2) {                                           // each group takes one half of the output from the other
+        static_assert(sizeof(chunk_shared<D>) >= 8 * (16 * HAVE + 2) * 256);
+        const auto share = [&](int g) { return (float *)&shared + (4 * g + wave) * (16 * HAVE + 2) * 64 + lane; };
+        float *const give = share(group);
+        const float *const take = share(1 - group);
         __syncthreads();
-        if (group) {
-            share[0] = m;
-            share[64] = l;
+        give[0] = m;
+        give[64] = l;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+        for (int d = 0; d < HAVE; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) share[(16 * d + i + 2) * 64] = o[d][i];
-        }
+            for (int i = 0; i < 16; i++) {
+                give[(16 * d + i + 2) * 64] = group ? o[d][i] : o[HAVE + d][i];
+                o[d][i] = group ? o[HAVE + d][i] : o[d][i];
+            }
         __syncthreads();
-        if (group) return;
-        const float m2 = share[0], top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top, f = exp2_(m - base), f2 = exp2_(m2 - base);
+        const float m2 = take[0], top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top, f = exp2_(m - base), f2 = exp2_(m2 - base);
         m = top;
-        l = l * f + share[64] * f2;
+        l = l * f + take[64] * f2;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < HAVE; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f + share[(16 * d + i + 2) * 64] * f2;
+            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f + take[(16 * d + i + 2) * 64] * f2;
     }
     l = pair_reduce(l, [](float p, float q) { return p + q; });
     const int row = wave * 32 + n;
@@ -640,10 +681,10 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
         uint8_t *dst = late->out + (int64_t)(row0 + token) * late->o_t + (int64_t)hq * late->o_h;
         const float f = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;     // 0: sees no key
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < HAVE; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int at = 32 * d + 8 * i + 4 * half;
+                const int at = 32 * (d0 + d) + 8 * i + 4 * half;
                 const float v0 = o[d][4 * i] * f, v1 = o[d][4 * i + 1] * f, v2 = o[d][4 * i + 2] * f, v3 = o[d][4 * i + 3] * f;
                 if (F32OUT) *(float4 *)(dst + at * 4) = make_float4(v0, v1, v2, v3);
                 else *(uint2 *)(dst + at * 2) = make_uint2(f2h(v0) | (uint32_t)f2h(v1) << 16, f2h(v2) | (uint32_t)f2h(v3) << 16);
@@ -651,11 +692,11 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     } else {
         float *part = late->chunk_part + ((int64_t)unit * late->chunk_pieces + piece) * CHUNK_ROWS * (D + 2);
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < HAVE; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                *(float4 *)(part + row * D + 32 * d + 8 * i + 4 * half) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-        if (half == 0) { part[CHUNK_ROWS * D + row] = m; part[CHUNK_ROWS * D + CHUNK_ROWS + row] = l; }
+                *(float4 *)(part + row * D + 32 * (d0 + d) + 8 * i + 4 * half) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+        if (half == 0 && group == 0) { part[CHUNK_ROWS * D + row] = m; part[CHUNK_ROWS * D + CHUNK_ROWS + row] = l; }
     }
 }
 
@@ -748,9 +789,9 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_k
     }
     const int b = blockIdx.x - few_units, unit = b / (CHUNK_ROWS / 16), sub = b % (CHUNK_ROWS / 16), head = unit % a.G;
     int tile, count;
-    const int s = find_tile(a, unit / a.G, tile, count);
+    pg_seq sq;
+    const int s = find_tile(a, unit / a.G, tile, count, sq);
     if (s < 0) return;
-    const pg_seq sq = pg_sequence(a.b, s, nullptr);
     const row_tile rt(a, sq, count - 1 - tile, CHUNK_ROWS);
     const int n_tile = max((rt.end() - (rt.lo_any() & ~63) + 63) >> 6, 0), pieces = (n_tile + a.chunk_split - 1) / a.chunk_split;
     if (pieces > 1) join_rows<D, F32OUT, CHUNK_ROWS>(a, rt, sq, head, sub, pieces, a.chunk_part + (int64_t)unit * a.chunk_pieces * CHUNK_ROWS * (D + 2));
@@ -798,7 +839,8 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = q->ne[2] * group / CHUNK_ROWS + b->n_seq;
         p.chunk_tiles = each * b->n_seq < all ? each * b->n_seq : all;
         p.chunk_units = p.chunk_tiles * G;
-        attn_share(p.chunk_units, ((int64_t)b->max_kv + 63) / 64 + 1, 2 * cu, 8, p.chunk_split, p.chunk_pieces);
+        // one workgroup per compute unit fits (512 tokens on 7680: 92 us, 101 with two per unit, 118 with three for four units), 512 keys at least
+        attn_share(p.chunk_units, ((int64_t)b->max_kv + 63) / 64 + 1, cu, 8, p.chunk_split, p.chunk_pieces);
     }
     SPY_CHECK_ARG(p.few_units * p.few_pieces + p.chunk_units * p.chunk_pieces < (1ll << 30) && p.chunk_units * (CHUNK_ROWS / 16) < (1ll << 30));
     p.few_bytes = p.few_pieces > 1 ? (size_t)(p.few_units * p.few_pieces * 16 * (hd + 2) * 4) : 0;
