@@ -269,3 +269,36 @@ def test_attention_of_strided_rows(hip):
     got = out.download(np.float32).reshape(p.rows, 6, 64)
     assert (got[:, 0] == 77).all() and (got[:, 5] == 77).all()
     P.check_attention(p, wide[:, 2:6], got[:, 1:5], True)
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("new", [1, 2, 64])
+def test_many_keys_of_little_weight(hip, new, f32):
+    """One key weighs e^10.4 times as much as each of the others, whose probabilities are subnormal fp16 numbers, and all of which together have a tenth of its weight."""
+    rng = np.random.default_rng(new)
+    p = P.Paged(rng, [(new, 4000)], 2, 2, 64, 64)
+    p.k_rows[0][:] = 0
+    p.k_rows[0][5, :, 0] = 10.4
+    p.v_rows[0][:] = 1
+    p.v_rows[0][5] = 0
+    p.store()
+    p.upload()
+    q = np.zeros((p.rows, 2, 64), np.float16)
+    q[:, :, 0] = 1
+    got = P.run_attention(p, q, f32, scale=1.0)
+    P.check_attention(p, q, got, f32, scale=1.0)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_that_share_pages(hip, new):
+    """The first pages of one sequence in the table of another, as for prompts that begin alike."""
+    rng = np.random.default_rng(13)
+    p = P.Paged(rng, [(new, 200), (new, 150)], 4, 2, 128, 32)
+    p.table[1, :3] = p.table[0, :3]
+    p.k_rows[1][:96], p.v_rows[1][:96] = p.k_rows[0][:96], p.v_rows[0][:96]
+    p.store()
+    p.upload()
+    q = rng.standard_normal((p.rows, 4, 128)).astype(np.float16)
+    got = P.run_attention(p, q, True)
+    assert P.flag() == 0
+    P.check_attention(p, q, got, True)
