@@ -49,6 +49,9 @@ APPENDS = [
     ([(200, 1111)], 5, 1, 128, 128, 0, 16),
     ([(1, 7)] * 70 + [(2, 9)], 2, 1, 64, 16, 2, 64),             # more sequences than lanes
     ([(9, 40), (0, 3)] * 40, 1, 1, 64, 1024, -1, 64),
+    ([(8, 8), (1, 9), (0, 0), (130, 177)], 4, 4, 256, 16, 2, 256),
+    ([(1, 700)] * 120 + [(8, 13)], 3, 1, 64, 32, 0, 48),
+    ([(7, 70)] * 19, 4, 2, 128, 16, 2, 128),
 ]
 
 
@@ -85,7 +88,7 @@ def test_append_at_far_positions(hip):
         _check_append(p, q, k, v, qo, (p.k_pool, p.v_pool), 0, 128, 10000.0, 1.0, 1.0)
 
 
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 40, 45])
 def test_append_without_a_place_raises_the_flag_and_stores_nothing(hip, new):
     """Pages that are not there, positions before the first: the other sequences' tokens are stored."""
     rng = np.random.default_rng(3)
