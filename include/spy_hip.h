@@ -209,8 +209,12 @@ int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sam
 
 /* ---- a batch of sequences over a cache in pages: no counterpart in the reference, whose caches hold one sequence
  *      (attention.cpp:180-265).  K pages are {hd, page_size, n_kv_head, n_page} and V^T pages {page_size, hd, n_kv_head, n_page}, F16, nb[0] = 2, the other
- *      strides any multiples of 16 bytes (nb[1] at most 2^20, nb[3] below 2^32), data 16-byte aligned: within a page the layouts of the caches above (rows of K, rows of V^T).  page_size is a power of
- *      two from 16 to 1024, hd 64, 128 or 256, n_head a multiple of n_kv_head (query head h reads K/V head h / (n_head / n_kv_head)). ----------------- */
+ *      strides any multiples of 16 bytes (nb[1] at most 2^20, nb[3] below 2^32), data 16-byte aligned: within a page the layouts of the caches above
+ *      (rows of K, rows of V^T).  page_size is a power of two from 16 to 1024, hd 64, 128 or 256, n_head a multiple of n_kv_head (query head h reads K/V head
+ *      h / (n_head / n_kv_head)).  Sequences may share pages that neither call appends to.
+ *      The device arrays are read when the call runs, so that a recorded call can be replayed with other lengths, rows and pages in them.  A sequence that does
+ *      not fit -- more new tokens than max_new, more cached ones than max_kv or than page_stride pages hold, rows outside the tensors -- raises the error flag of
+ *      spy_hip_take_error and takes no part: its rows are left alone. ----------------- */
 typedef struct spy_hip_paged_batch {
     int32_t n_seq;               /* sequences */
     int32_t max_new, max_kv;     /* no sequence has more new / cached tokens than these (the launches are sized by them) */
@@ -233,7 +237,7 @@ int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const spy_hip_te
                          const spy_hip_rope_param *rope, const spy_hip_tensor *q_out, const spy_hip_tensor *k_pages, const spy_hip_tensor *v_pages);
 /* Attention of the batch's new tokens over the pages (which hold them already): MatMul(K, q) -> Softmax(mask, scale) -> MatMul(V^T, P) per sequence and head
  * (attention.cpp:25-302).  q {hd, n_head, n_row} F16, out the same shape F32 or F16, strides and alignment as above.  A token sees the positions below
- * kv_len of its sequence; causal != 0: none behind its own; window > 0: of those the last `window` up to its own position only.  A token that sees no
+ * kv_len of its sequence; causal != 0: none behind its own; window > 0: none at or before its own less `window`.  A token that sees no
  * position gets zeros; what lies in the pages at positions it does not see, infinities and NaN too, does not reach its output.  Pages outside 0 .. n_page - 1 hold nothing
  * and raise the error flag.  scale: finite, not 0.  Scores, sums and the product are fp32; probabilities enter the product as fp16 (a relative error of 2^-11 each) for
  * F16 outputs and as two fp16 terms (2^-22) for F32 outputs.  scratch: device memory of spy_hip_paged_attention_scratch_size bytes, 256-byte aligned, this call's
