@@ -413,7 +413,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
     const bool idle = wave * 32 >= n_row;                                  // waves without rows fetch, and compute nothing
 
     const int32_t *table = alone(a.b.pages + (int64_t)s * a.b.page_stride);
-    const int plog = alone(a.b.page_log2), pmask = alone((1 << plog) - 1), last = alone((sq.kv - 1) >> plog), n_page = alone(a.b.n_page);
+    const int plog = alone(a.b.page_log2), pmask = alone((1 << plog) - 1), last = alone(max(sq.kv - 1, 0) >> plog), n_page = alone(a.b.n_page);
     const uint32_t lds_k = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.k[0] + wave * 1024),
                    lds_v = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.v[0] + wave * 1024);
 

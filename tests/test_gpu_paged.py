@@ -292,6 +292,20 @@ def test_many_keys_of_little_weight(hip, new, f32):
     P.check_attention(p, q, got, f32, scale=1.0)
 
 
+@pytest.mark.parametrize("causal", [1, 0])
+def test_fewer_cached_tokens_than_new_ones(hip, causal):
+    """Tokens at negative positions, an empty cache: rows that see nothing get zeros."""
+    rng = np.random.default_rng(17)
+    p = P.Paged(rng, [(70, 0), (1, 0), (70, 3), (20, 5), (3, 1), (2, 40)], 2, 1, 128, 16)
+    p.store()
+    p.upload()
+    q = rng.standard_normal((p.rows, 2, 128)).astype(np.float16)
+    got = P.run_attention(p, q, True, causal)
+    assert P.flag() == 0
+    P.check_attention(p, q, got, True, causal)
+    assert (got[:71] == 0).all()
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_sequences_that_share_pages(hip, new):
     """The first pages of one sequence in the table of another, as for prompts that begin alike."""
