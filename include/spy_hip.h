@@ -239,7 +239,7 @@ int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const spy_hip_te
  * (attention.cpp:25-302).  q {hd, n_head, n_row} F16, out the same shape F32 or F16, strides and alignment as above.  A token sees the positions below
  * kv_len of its sequence; causal != 0: none behind its own; window > 0: none at or before its own less `window`.  A token that sees no
  * position gets zeros; what lies in the pages at positions it does not see, infinities and NaN too, does not reach its output.  Pages outside 0 .. n_page - 1 hold nothing
- * and raise the error flag.  scale: finite, not 0.  Scores, sums and the product are fp32; probabilities enter the product as fp16 (a relative error of 2^-11 each) for
+ * and raise the error flag.  scale: 1e-37 to 1e24 in magnitude.  out must not overlap q.  Scores, sums and the product are fp32; probabilities enter the product as fp16 (a relative error of 2^-11 each) for
  * F16 outputs and as two fp16 terms (2^-22) for F32 outputs.  scratch: device memory of spy_hip_paged_attention_scratch_size bytes, 256-byte aligned, this call's
  * alone until the stream has passed it (a captured call: until its graph is done with); its contents need not be set. */
 size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch);

@@ -50,9 +50,9 @@ static __device__ __forceinline__ float logit_of(u64 x) {
 // e^((l - max) / T) = 2^-y as a multiple of 2^-44, y = (max - l) log2(e) / T.  log2(e) / T in two floats: a rounded one alone would shift all weights of the same
 // distance the same way.  The exponential is good to an ulp.
 struct weigher {
-    float top, c, c_lo;
+    float top, c, c_lo, cap;           // cap: distances from here on count as this one, y as 1e20 at most: products beyond a float would have either sign
     __device__ __forceinline__ float far(float l) const {                         // -inf: as good as infinitely far
-        const float d = fminf(top - l, 3.4e38f);
+        const float d = fminf(top - l, cap);
         return fmaf(d, c, d * c_lo);
     }
     static __device__ __forceinline__ u64 at(float y) {
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     row.n = a.n; row.begin = wave * a.part; row.part = a.part; row.held = a.held;
     f4 *const held = (f4 *)(smem + sizeof(sample_shared));
     row.lds = held + wave * (a.held / 4);
-    const float temp = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f, u = a.uniform[r];
+    const float temp = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p && a.min_p[r] > 0.0f ? fminf(a.min_p[r], 1.0f) : 0.0f, u = a.uniform[r];
     const int k = a.top_k ? a.top_k[r] : 0;
 
     row.infinite = false;
@@ -367,6 +367,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     const double c = 1.4426950408889634074 / (double)temp;
     weigh.top = top; weigh.c = (float)c; weigh.c_lo = (float)(c - (double)weigh.c);
     if (!(weigh.c <= 3.4e38f)) { weigh.c = 3.4e38f; weigh.c_lo = 0.0f; }          // a temperature next to 0
+    weigh.cap = weigh.c > 1e-18f ? 1e20f / weigh.c : 3.4e38f;
     const bool by_rank = k > 0 && k < a.n, by_mass = p < 1.0f;
     u64 last = ~0ull;                                                             // rank word of the last token kept
     if (mp > 0.0f && temp < INFINITY) {
@@ -379,8 +380,8 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     if (by_rank && k <= SM_FAST) {
         // a bin of the threads' maxima, between the least and the greatest, by which k of them are counted
         const float scale = top > low ? (SM_BINS - 1) / (top - low) : 0.0f;
-        const auto near = [&](float v) { return (int)fminf((top - v) * scale, (float)SM_BINS); };
-        if (own > -INFINITY) atomicAdd(&s.count[min(near(own), SM_BINS - 1)], 1u);
+        const auto near = [&](float v) { return (int)fminf((top - v) * scale, (float)(SM_BINS - 1)); };
+        if (own > -INFINITY) atomicAdd(&s.count[near(own)], 1u);
         __syncthreads();
         uint32_t some, number;
         const int bin = find_bin(s, s.count[t], (uint32_t)k, some, number);

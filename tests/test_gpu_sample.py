@@ -138,6 +138,30 @@ def test_masked_tokens_infinities_and_nan(hip, n):
     assert got[2] == -1 and got[3] == -1 and prob[2] == 0 and prob[3] == 0 and got[8] == n - 1 and got[6] in (3, 9, 60) and got[7] in (3, 9)
 
 
+@pytest.mark.parametrize("n", [1000, 40000])
+def test_temperatures_next_to_zero_and_far_masks(hip, n):
+    """Masks of -inf and of the type's lowest value beside temperatures by which their distance is past the largest float: only what is as large as the maximum weighs."""
+    rng = np.random.default_rng(n)
+    temps = np.array([1e-3, 1e-6, 9e-8, 7e-8, 3e-8, 1e-8, 1e-12, 1e-20, 1e-30, 1e-37, 1e-40], np.float32)
+    logits = np.repeat(logits_of(rng, 1, n), len(temps), axis=0)
+    logits[:, rng.permutation(n)[:n // 3]] = -np.inf
+    logits[:, rng.permutation(n)[:n // 3]] = np.finfo(np.float32).min
+    logits[:, rng.permutation(n)[:3]] = logits[0].max()
+    for a in (dict(top_p=0.9), dict(top_k=n // 2 + 600, top_p=0.9), dict(top_k=50), dict(min_p=0.1, top_p=0.5), dict()):
+        check(hip, logits, temperature=temps, uniform=rng.random(len(temps)).astype(np.float32), **a)
+
+
+def test_logits_further_apart_than_a_float(hip):
+    """A largest and a least logit whose difference is infinite, every temperature, the flat one too."""
+    rng = np.random.default_rng(2)
+    logits = rng.standard_normal((4, 1500)).astype(np.float32)
+    logits[:, :700] = -3e38
+    logits[:, rng.permutation(1500)[:3]] = 3e38
+    temps = np.array([1.0, 1e30, np.inf, 1e-9], np.float32)
+    for a in (dict(top_k=40), dict(top_k=1400), dict(top_p=0.7), dict()):
+        check(hip, logits, temperature=temps, uniform=np.array([0.1, 0.9, 0.999, 0.4], np.float32), **a)
+
+
 def test_random_numbers_at_and_past_their_ends(hip):
     rng = np.random.default_rng(2)
     l = np.repeat(logits_of(rng, 1, 777), 8, axis=0)

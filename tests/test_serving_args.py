@@ -34,7 +34,7 @@ def append(**kw):
 
 
 def attend(scale=0.1, window=0, scratch=4096, room=None, **kw):
-    a = {"q": rows(4), "kp": pages("k"), "vp": pages("v"), "out": rows(4), "b": batch(), **kw}
+    a = {"q": rows(4), "kp": pages("k"), "vp": pages("v"), "out": rows(4, at=8192), "b": batch(), **kw}
     ref = lambda x: None if x is None else B(x)                                                   # noqa: E731
     L = H.load()
     if room is None:
@@ -64,7 +64,8 @@ def test_append_does_not_support(kw):
 
 
 @pytest.mark.parametrize("kw", INVALID_BATCH + [dict(q=None), dict(out=None), dict(q=rows(3), out=rows(3)), dict(out=rows(4, n_row=9)), dict(out=rows(2)), dict(q=rows(4, hd=64)), dict(q=rows(4, at=0)),
-                                                dict(out=rows(4, at=4100)), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0)])
+                                                dict(out=rows(4, at=4100)), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=0.0), dict(scale=1e-38), dict(scale=-1e25),
+                                                dict(out=rows(4))])
 def test_attention_refuses(kw):
     assert attend(**kw) == H.EINVAL
 
