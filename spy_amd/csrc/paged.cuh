@@ -1,7 +1,7 @@
 // What the kernels over a cache in pages share: where a batch's sequences, rows and pages are.
 #pragma once
 
-#include "common.cuh"
+#include "scan.cuh"
 
 struct pg_batch {
     const int32_t *row_start, *kv_len, *pages;

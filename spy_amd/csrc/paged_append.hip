@@ -160,9 +160,7 @@ template <bool F16IN> static __device__ __forceinline__ void append_v_tile(const
             f = max(q.kv - q.n_new, 0) >> 6;
             n = q.ok && q.kv > 0 ? ((q.kv - 1) >> 6) - f + 1 : 0;
         }
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(sum, o, SPY_WAVE); if (lane >= o) sum += v; }
+        const int sum = (int)wave_scan((uint32_t)n);
         const unsigned long long past = __ballot(sum > left);
         if (past) {
             const int at = __ffsll(past) - 1;

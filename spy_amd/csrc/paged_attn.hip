@@ -370,9 +370,7 @@ static __device__ __forceinline__ int find_tile(const attn_args &a, int left, in
             const int rows = q.ok ? q.n_new * a.group : 0;
             n = rows > a.few ? (rows + CHUNK_ROWS - 1) / CHUNK_ROWS : 0;
         }
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(sum, o, SPY_WAVE); if (lane >= o) sum += v; }
+        const int sum = (int)wave_scan((uint32_t)n);
         const unsigned long long past = __ballot(sum > left);
         if (past) {
             const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);

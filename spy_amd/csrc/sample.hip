@@ -11,7 +11,7 @@
 // One workgroup per row, which keeps 32768 logits in LDS at a time.  Measured: one row of 32000 with all settings 9 us, 64 rows 24 us: latency, some forty barriers with a
 // few dependent LDS accesses between them; 256 rows of 100003 with top_p alone 81 us: vector instructions, since a weight of every logit is worked out for the sums by
 // distance and once more for the sums by part (the memory's share, 103 MB at a copy's rate, is 22 us).
-#include "common.cuh"
+#include "scan.cuh"
 
 #define SM_THREADS 1024
 #define SM_BINS 1024           // one per thread
@@ -73,22 +73,6 @@ struct __attribute__((aligned(16))) sample_shared {      // (the logits lie behi
     int bin;
 };
 
-// Inclusive sums over lanes without LDS: shifts by 1, 2, 4, 8 inside the rows of 16 lanes, then the last lanes of rows 0 and 2, and of row 1, to the rows behind
-template <int CTRL, int ROWS> static __device__ __forceinline__ uint32_t moved(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
-template <int CTRL, int ROWS> static __device__ __forceinline__ u64 moved(u64 v) { return (u64)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v); }
-template <class T> static __device__ __forceinline__ T row_scan(T v) {
-    v += moved<0x111, 0xF>(v);
-    v += moved<0x112, 0xF>(v);
-    v += moved<0x114, 0xF>(v);
-    v += moved<0x118, 0xF>(v);
-    return v;
-}
-template <class T> static __device__ __forceinline__ T wave_scan(T v) {
-    v = row_scan(v);
-    v += moved<0x142, 0xA>(v);
-    v += moved<0x143, 0xC>(v);
-    return v;
-}
 static __device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 static __device__ __forceinline__ u64 of_lane(u64 v, int lane) { return (u64)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane); }
 // Inclusive sum over the threads, and the sum of all.  Two calls have a barrier between them.

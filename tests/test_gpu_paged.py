@@ -128,6 +128,9 @@ ATTENDS = [
     ([(40, 100), (200, 500)], 4, 1, 64, 32, 0, 37),
     ([(1, 20)] * 70, 2, 2, 64, 16, 1, 0),
     ([(300, 300)], 5, 5, 128, 1024, 1, 0),
+    ([(17, 1500)] * 60 + [(18, 2100), (40, 1040), (17, 1024), (19, 1025)], 4, 4, 64, 16, 1, 0),      # so many that no sequence's keys are shared out: long runs of tiles
+    ([(17, 2200)] * 32, 8, 8, 128, 128, 1, 2050),
+    ([(17, 1090)] * 64, 4, 4, 256, 32, 0, 0),
 ]
 
 
@@ -290,6 +293,20 @@ def test_many_keys_of_little_weight(hip, new, f32):
     q[:, :, 0] = 1
     got = P.run_attention(p, q, f32, scale=1.0)
     P.check_attention(p, q, got, f32, scale=1.0)
+
+
+def test_missing_pages_far_into_a_long_run_of_tiles(hip):
+    rng = np.random.default_rng(19)
+    p = P.Paged(rng, [(17, 2200)] * 64, 4, 4, 64, 16)
+    p.store()
+    hidden = {(s, int(i)) for s in (0, 3, 63) for i in rng.integers(0, 136, 5)} | {(1, 64), (1, 127), (2, 63), (2, 128)}
+    for s, i in hidden:
+        p.table[s, i] = [-1, p.n_page][i % 2]
+    p.upload()
+    q = rng.standard_normal((p.rows, 4, 64)).astype(np.float16)
+    got = P.run_attention(p, q, True)
+    assert P.flag() != 0
+    P.check_attention(p, q, got, True, hidden=hidden)
 
 
 @pytest.mark.parametrize("causal", [1, 0])
