@@ -300,9 +300,9 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
 // ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
 // Bound by the matrix cores and the vector instructions of the softmax together: 64 keys by 32 rows take a wave (D = 128) 32 matrix instructions of 33 cycles, and some 215
 // vector instructions of 4.7, 32 of them exponentials of 11; two waves of a SIMD need 4600 of the 5200 cycles that a step takes.  Measured (128 wide, 32 heads): a prompt of
-// 2048 tokens 57 us, 603 TFLOP/s of what its rows see; 512 tokens on 7680 91 us, 734 TFLOP/s; 16 us of the former are spent outside the loop, by two workgroups one after the
-// other.  Tried and not kept: the next tile's scores computed beside this one's exponentials in one instruction stream (58 and 91 us), a barrier for each group by
-// itself (59 and 98).
+// 2048 tokens 55 us, 628 TFLOP/s of what its rows see; 512 tokens on 7680 88 us, 754 TFLOP/s; 13 us of the former are spent outside the loop, by two workgroups one after the
+// other.  Tried and not kept (where this had 57 and 91 us): the next tile's scores computed beside this one's exponentials in one instruction stream (58 and 91), a barrier for
+// each group by itself (59 and 98), the groups half a step apart, wave priorities (no difference).
 // Four waves have 32 rows each; a second group of four has the same rows and every other tile of keys, so that a SIMD always has a second wave, to the end of a long row
 // of keys, and the groups exchange halves of (m, l, o) at the end (one group of 256 rows would leave the short rows of a prompt's triangle without a second wave).
 // (256-wide heads: one group, whose waves have all registers to themselves.)  The 64 keys' K and V^T of a group lie in LDS,
@@ -700,7 +700,8 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
 }
 
 // ---- the rows whose keys several workgroups shared: 16 rows per workgroup ---------------------------------------------------------------
-// Latency: a wave has the (m, l) of four rows, a lane one workgroup's; then eight pieces of o are requested at a time.
+// Latency, and what the first launch wrote: a wave has the (m, l) of four rows, a lane one workgroup's; eight pieces of o are requested at a time, the first before (m, l) are
+// there.  Measured: one request of 4096 keys (17 pieces) 4.5 us, 512 tokens on 7680 (two pieces, 17 MB) 8.
 template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void join_rows(const attn_args &a, const row_tile &rt, const pg_seq &sq, int head, int sub, int pieces, const float *part) {
     __shared__ float s_w[16][64], s_sum[16];
     constexpr int64_t STEP = TILE * (D + 2);
@@ -717,16 +718,22 @@ template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void j
             for (int j = 0; j < 8; j++) x[k][j] = *(const v4f *)(part + min(p + j, pieces - 1) * STEP + (16 * sub + row) * D + d);
         }
     };
+    float m0[4], l0[4], top[4], sum[4];                                    // m and l of the first 64 pieces, all asked for before the first is waited for
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float *q = part + min(lane, pieces - 1) * STEP + TILE * D + 16 * sub + min(4 * wave + i, rows - 1);
+        m0[i] = q[0]; l0[i] = q[TILE];
+    }
     request(0);
-    float top[4], sum[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int row = 4 * wave + i;
-        top[i] = -INFINITY; sum[i] = 0.0f;
-        if (row >= rows) continue;
-        for (int p = lane; p < pieces; p += 64) top[i] = fmaxf(top[i], part[p * STEP + TILE * D + 16 * sub + row]);
-        top[i] = wave_max(top[i]);
+        sum[i] = 0.0f;
+        top[i] = m0[i];                                                    // (a lane past the pieces has the last one's)
+        for (int p = 64 + lane; p < pieces; p += 64) top[i] = fmaxf(top[i], part[p * STEP + TILE * D + 16 * sub + min(row, rows - 1)]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) top[i] = wave_max(top[i]);
 #pragma unroll
     for (int k = 0; k < ITEMS; k++) v[k] = v4f{0, 0, 0, 0};
     for (int base = 0; base < pieces; base += 64) {
@@ -739,8 +746,8 @@ template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void j
             float w = 0.0f;
             if (lane < n) {
                 const float *q = part + (base + lane) * STEP + TILE * D + 16 * sub + row;
-                w = exp2_(q[0] - (top[i] == -INFINITY ? 0.0f : top[i]));
-                sum[i] += w * q[TILE];
+                w = exp2_((base ? q[0] : m0[i]) - (top[i] == -INFINITY ? 0.0f : top[i]));
+                sum[i] += w * (base ? q[TILE] : l0[i]);
             }
             s_w[row][lane] = w;
         }
