@@ -315,9 +315,10 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 #pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from memory to LDS, in lane order from byte `lds` (uniform) on; base uniform, or an address per lane.  Written as instructions so that the compiler does
 // not wait for them at the next LDS read; landed() does.
+// A base that a vector instruction has written may be read five instructions later: the compiler does not look into these.
 // `there` 0: not requested.  (The branch is written out as well: as one of the compiler's it would part the instructions on either side into blocks of their own.)
 static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds, uint32_t there) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, %2\n.Lno%=:" :: "s"(lds), "v"(off), "s"(base), "s"(there) : "memory", "m0", "scc");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\ts_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, %2\n.Lno%=:" :: "s"(lds), "v"(off), "s"(base), "s"(there) : "memory", "m0", "scc");
 }
 static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds, uint32_t there) {
     asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, off\n.Lno%=:" :: "s"(lds), "v"(addr), "s"(there) : "memory", "m0", "scc");
