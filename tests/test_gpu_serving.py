@@ -199,3 +199,55 @@ def test_calls_on_two_streams_at_once(hip):
             assert np.array_equal(s["out"].download(np.uint32)[:rows], o[:rows]) and np.array_equal(s["tokens"].download(np.int32), t), again
     for s in sides:
         H.check(L.spy_hip_stream_destroy(s["st"]))
+
+
+@pytest.mark.parametrize("seqs", [[(1, 3000), (1, 77), (1, 1500)], [(70, 2900), (1, 2000), (3, 3)], [(200, 2200)]])
+def test_a_recorded_call_follows_the_lengths(hip, seqs):
+    """Keys shared out and joined, recorded once, replayed with other lengths and pages in the device arrays, other calls on the same stream in between: the bits of an eager call."""
+    from spy_amd import _lib as H
+    L = H.load()
+    rng = np.random.default_rng(31)
+    p = P.Paged(rng, seqs, 4, 2, 128, 16)
+    p.store()
+    p.upload()
+    q = (rng.standard_normal((p.rows, 4, 128)) * 1.5).astype(np.float16)
+    dq = H.DeviceBuffer.from_numpy(q.view(np.uint16))
+    outs = [H.DeviceBuffer.from_numpy(np.full(q.shape, 77, np.float32)) for _ in range(2)]
+    tq, to = H.tensor(dq, H.F16, [128, 4, p.rows]), [H.tensor(o, H.F32, [128, 4, p.rows]) for o in outs]
+    need = L.spy_hip_paged_attention_scratch_size(B(tq), B(p.t_k), B(p.batch))
+    assert need > 0
+    scratch = [H.DeviceBuffer(need) for _ in range(2)]
+    st, graph = C.c_void_p(), C.c_void_p()
+    H.check(L.spy_hip_stream_create(B(st)))
+    call = lambda i, s: H.check(L.spy_hip_paged_attention(s, B(tq), B(p.t_k), B(p.t_v), B(to[i]), B(p.batch), 0.09, 1, 0, scratch[i].ptr, need))     # noqa: E731
+    H.check(L.spy_hip_capture_begin(st))
+    call(0, st)
+    H.check(L.spy_hip_capture_end(st, B(graph)))
+    full, starts = p.kv.copy(), p.row_start.copy()
+    for n in range(4):
+        p.kv = np.maximum(full - np.array([0, 500, 37, 1400])[n], p.n_new)            # shorter caches: the same tokens, fewer of them
+        if n == 2:                                                                    # the first sequence has ended
+            p.row_start = np.concatenate([[0], starts[1:] - starts[1]]).astype(np.int32)
+        else:
+            p.row_start = starts
+        p.n_new = np.diff(p.row_start)
+        p.d_kv.upload(p.kv.astype(np.int32))
+        p.d_start.upload(p.row_start)
+        for i in range(2):
+            outs[i].upload(np.full(q.shape, 77, np.float32))
+            scratch[i].fill(0xFF)
+        H.sync()
+        H.check(L.spy_hip_graph_launch(graph, st))
+        H.sync(st)
+        got = outs[0].download(np.float32).reshape(q.shape)
+        call(1, st)
+        H.sync(st)
+        assert np.array_equal(got.view(np.uint32), outs[1].download(np.uint32).reshape(q.shape)), n
+        k_rows, v_rows = p.k_rows, p.v_rows
+        p.k_rows, p.v_rows = [k[:x] for k, x in zip(k_rows, p.kv)], [v[:x] for v, x in zip(v_rows, p.kv)]
+        P.check_attention(p, q, got, True, scale=0.09)
+        p.k_rows, p.v_rows = k_rows, v_rows
+        p.n_new = np.diff(starts)
+    assert P.flag() == 0
+    H.check(L.spy_hip_graph_destroy(graph))
+    H.check(L.spy_hip_stream_destroy(st))
