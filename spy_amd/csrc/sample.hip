@@ -283,7 +283,8 @@ template <class In> static __device__ __forceinline__ uint32_t narrow(sample_sha
         });
         __syncthreads();
         u64 sum, all;
-        const int bin = find_bin(s, by_mass ? s.mass[t] : (u64)s.count[t], want, sum, all);
+        // (the last bin where none reaches it, which only logits that are written meanwhile can bring about: the range gets narrower all the same)
+        const int bin = min(find_bin(s, by_mass ? s.mass[t] : (u64)s.count[t], want, sum, all), SM_BINS - 1);
         const u64 upto = block_scan(s, s.mass[t], all);
         if (t == bin) s.pick = upto - s.mass[t];
         __syncthreads();
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     }
     __syncthreads();
     const u64 sums = row_scan(s.part[lane & 15]), total = of_lane(sums, 15), want_all = draw_at(u, total);
-    const int part = __ffsll(__ballot(sums >= want_all)) - 1;                      // the first of the row's 16 lanes
+    const int part = max(__ffsll(__ballot(sums >= want_all)) - 1, 0);              // the first of the row's 16 lanes
     const u64 want = want_all - (part ? of_lane(sums, part - 1) : 0);
     const int each = (a.part / 4 + SM_THREADS - 1) / SM_THREADS;                  // groups of four per thread
     const auto group = [&](int i) {                                               // of the part
