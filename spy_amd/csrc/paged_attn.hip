@@ -87,8 +87,9 @@ static __device__ __forceinline__ uint4 bounded(uint4 w, bool &any) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 // Where V holds infinities or NaN at positions that some rows of a tile see and others do not, a probability of 0 would not keep them out of the others' outputs (0 times
-// either is NaN).  There the product takes 0 in their place, and which of +inf, -inf and NaN a row sees in which dimension is counted by the same instruction
-// over indicators: w's elements that are of kind 0, 1, 2 as 1, the others as 0.
+// either is NaN), so the product takes 0 in their place there; and where all rows see them, what it makes of them depends on how a probability was rounded.  So where any
+// were taken out, or an output is not finite, which of +inf, -inf and NaN a row sees in which dimension is counted after all, in one more walk over V, by the matrix
+// instruction over indicators: w's elements that are of kind 0, 1, 2 as 1, the others as 0.
 static __device__ __forceinline__ v8h of_kind(uint4 w, int kind) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
     uint32_t r[4];
@@ -113,6 +114,9 @@ static __device__ __forceinline__ v8h ones(uint32_t bits) {
     return halves(make_uint4(r[0], r[1], r[2], r[3]));
 }
 static __device__ __forceinline__ float kind_value(int kind) { return kind == 2 ? NAN : kind ? -INFINITY : INFINITY; }
+static __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// A factor from one m to another that leaves infinities infinite: what is not above 2^-126 of a larger part adds nothing to it, as with 0
+static __device__ __forceinline__ float above_0(float f) { return fmaxf(f, 0x1p-126f); }
 
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
@@ -178,6 +182,7 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
     v4f o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
+    bool unbounded = false;
     // K of the next tile is requested when this one's scores are done with the registers, V^T when the product is: memory always has a tile of each wave to fetch
     const int first = piece * a.few_split + wave;
     page_pair pg = {0, 0}, pg1 = {0, 0};
@@ -204,16 +209,13 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
         for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
         const bool masked = __any(kb + 32 > hi_all || kb < lo_all || vbad);
         const int there = vbad ? 0 : end - vk;                             // positions of this lane's eight that the cache has, for this tile's rows
-        bool fix = false;
         if (masked) {
 #pragma unroll
             for (int j = 0; j < 8; j++) e[j] = vk + j >= lo && vk + j < hi && !vbad ? e[j] : -INFINITY;
             if (vbad && vk < end && vk + 8 > rt.lo_any() && a.err) *a.err = 1;     // (a page before the window may be gone)
             // what lies behind the cache's last position is taken as 0, and so are infinities and NaN, which some rows may see and others not
-            bool any = false;
 #pragma unroll
-            for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), any);
-            fix = __any(any);
+            for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), unbounded);
         }
         float top = e[0];
 #pragma unroll
@@ -238,24 +240,36 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fv[d]), p, o[d], 0, 0, 0);
             if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fv[d]), p2, o[d], 0, 0, 0);
         }
-        if (fix) {
-            uint32_t seen = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
-            const v8h see = ones(seen);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const uint4 w = first_of(*(const uint4 *)(v_row(kt, pg) + 16 * d * a.vp_d), there);
-#pragma nounroll
-                for (int kind = 0; kind < 3; kind++) {
-                    const v4f n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), see, v4f{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
-                }
-            }
-        }
         if (kt + WAVES < stop) load_v(v_row(kt + WAVES, pg1));
         pg = pg1; pg1 = pg2;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) unbounded |= !finite(o[d][i]);
+    if (__any(unbounded)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[d][i] = finite(o[d][i]) ? o[d][i] : 0.0f;       // (of a row with a score of NaN or +inf: l is NaN)
+#pragma nounroll
+            for (int kind = 0; kind < 3; kind++) {
+                v4f n_seen = {0, 0, 0, 0};
+#pragma nounroll
+                for (int kt = first; kt < stop; kt += WAVES) {
+                    const page_pair g = pages_of(kt);
+                    const int vk = begin + 32 * kt + 8 * quarter;
+                    const bool vbad = missing(quarter & 2 ? g.second : g.first);
+                    const uint4 w = first_of(*(const uint4 *)(v_row(kt, g) + 16 * d * a.vp_d), vbad ? 0 : end - vk);
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
+                    n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), ones(seen), n_seen, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
+            }
+        }
     }
     l = quad_reduce(l, [](float p, float q) { return p + q; });
     if (quarter == 0) { sh.m[wave][n] = m; sh.l[wave][n] = l; }
@@ -263,7 +277,7 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) top = fmaxf(top, sh.m[w][n]);
-    const float shrink = exp2_(m - (top == -INFINITY ? 0.0f : top));
+    const float shrink = above_0(exp2_(m - (top == -INFINITY ? 0.0f : top)));
     float *part = a.few_part + ((int64_t)unit * a.few_pieces + piece) * 16 * (D + 2);
 #pragma unroll
     for (int h = 0; h < D / HALF; h++) {
@@ -391,7 +405,7 @@ static __device__ __forceinline__ int find_tile(const attn_args &a, int left, in
 
 static constexpr __host__ __device__ int chunk_groups(int D) { return D == 256 ? 1 : 2; }
 template <int D> struct chunk_group { __attribute__((aligned(1024))) uint8_t k[2][64 * D * 2], v[2][64 * D * 2]; };
-template <int D> struct chunk_shared { chunk_group<D> group[chunk_groups(D)]; int unbounded[chunk_groups(D)][3]; };
+template <int D> struct chunk_shared { chunk_group<D> group[chunk_groups(D)]; int unbounded; };
 
 template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(const attn_args &a, chunk_shared<D> &shared, int block) {
     constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
@@ -484,9 +498,8 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = v16f{0};
     constexpr uint32_t BUF = 64 * D * 2;                                   // bytes of one buffer
-    int *const sh_unbounded = shared.unbounded[group];                     // of the tiles in turn: three, so that one is cleared while no wave sets or reads it
     uint32_t k_at = n * (2 * D) + (half ^ swizzle_k<D>(n)) * 16, v_at = n * 128 + (half ^ swizzle_v(n)) * 16;     // this lane's pieces in LDS
-    const auto compute = [&](int kt, int buf, int bad, bool masked, int turn, group_pages next) {
+    const auto compute = [&](int kt, int buf, int bad, bool masked, group_pages next) {
         const int kb = begin + 64 * kt;
         const uint32_t more = there_is(kt + GROUPS);
         // LDS answers after some 130 cycles, four times what an instruction that waits for it takes: operands are asked for in order, well before their use, and the
@@ -578,31 +591,10 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (masked && sh_unbounded[turn]) {                                // the infinities and NaN that bound_v took out, from memory
-            uint32_t seen = 0;
-            int first = mine - lo;
-            asm("" : "+v"(first));                                         // the comparisons once more, rather than 32 of them kept
-#pragma unroll
-            for (int i = 0; i < 32; i++) seen |= (uint32_t)sees(i, first) << i;
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma nounroll
-                for (int kind = 0; kind < 3; kind++) {
-                    v16f n_seen = {0};
-#pragma nounroll
-                    for (int k = 0; k < 4; k++) {
-                        const int at = mine + 16 * k, page = table[min(at >> plog, last)], there = bad >> k & 1 ? 0 : end - at;
-                        const uint4 v = *(const uint4 *)(vbase + (uint64_t)((uint32_t)page >= (uint32_t)n_page ? 0 : page) * vp_g + (uint32_t)(32 * d + n) * vp_d + (at & pmask) * 2);
-                        n_seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(of_kind(first_of(v, there), kind), ones(seen >> (8 * k) & 0xFF), n_seen, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
-                }
-        }
     };
     // The pieces of V^T that this wave requested: as in attn_few, positions behind the cache's last one hold anything and are taken as 0, and infinities and NaN, which some
     // rows may see and others not, as well
-    const auto bound_v = [&](int kt, int buf, int bad, int turn) {
+    const auto bound_v = [&](int kt, int buf, int bad) {
         const int there = bad >> (vc >> 1) & 1 ? 0 : end - (begin + 64 * kt + 8 * vc);
         bool any = false;
 #pragma unroll
@@ -610,11 +602,11 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
             uint4 *const v = (uint4 *)(sh.v[buf] + (4 * i + wave) * 1024 + lane * 16);
             *v = bounded(first_of(*v, there), any);
         }
-        if (any) sh_unbounded[turn] = 1;
+        if (any) shared.unbounded = 1;
     };
     const int steps = (max(stop - from, 0) + GROUPS - 1) / GROUPS;
     if (steps) {
-        int kt = from + group, i = 0, turn = 0, fetched = 0;               // (tiles are numbered from `from` on where their pages are looked up)
+        int kt = from + group, i = 0, fetched = 0;               // (tiles are numbered from `from` on where their pages are looked up)
         take_entries(first_pages);
         int bad = gone_of(group);
         {
@@ -625,15 +617,14 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
 #pragma unroll
             for (int j = 0; j < NI; j++) ask_v(v_from, 0, there_is(kt), j);
         }
-        if (tid < 3 * GROUPS) shared.unbounded[0][tid] = 0;
+        if (tid == 0) shared.unbounded = 0;
         __syncthreads();
         const auto step = [&](auto idle_) __attribute__((always_inline)) { // one tile; true: it was the last
             const int buf = i & 1, kb = begin + 64 * kt;
             const bool masked = kt < stop && (kb + 64 > hi_all || kb < lo_all || bad);
             landed();                                                      // what this wave requested of this tile is in LDS ...
-            if (masked) bound_v(kt, buf, bad, turn);
+            if (masked) bound_v(kt, buf, bad);
             __syncthreads();                                               // ... and all of it, and nobody reads the other buffer any more
-            if (lane == 0) sh_unbounded[turn == 0 ? 2 : turn - 1] = 0;     // the last tile's
             const int ahead = kt - from + GROUPS;
             if ((ahead & 15) == group) take_entries(fetched);
             if ((ahead + GROUPS & 15) == group) fetched = entries_of(ahead + GROUPS);
@@ -650,15 +641,42 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 for (int j = 0; j < NI; j++) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
 #pragma unroll
                 for (int j = 0; j < NI; j++) ask_v(v_from, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
-            } else if (kt < stop) compute(kt, buf, bad, masked, turn, next);
+            } else if (kt < stop) compute(kt, buf, bad, masked, next);
             bad = gone_of(ahead);
             kt += GROUPS;
-            turn = turn == 2 ? 0 : turn + 1;
             return ++i == steps;
         };
         // (a loop of their own for waves without rows: a branch around the products in one loop for both costs registers)
         if (idle) while (!step(std::true_type{})) {}
         else while (!step(std::false_type{})) {}
+        __syncthreads();
+        bool unbounded = shared.unbounded;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) unbounded |= !finite(o[d][j]);
+        if (__any(unbounded)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[d][j] = finite(o[d][j]) ? o[d][j] : 0.0f;
+#pragma nounroll
+                for (int kind = 0; kind < 3; kind++) {
+                    v16f n_seen = {0};
+#pragma nounroll
+                    for (int at = begin + 64 * (from + group) + 8 * half, k = 0; at < begin + 64 * stop; at += ++k & 3 ? 16 : 64 * GROUPS - 48) {   // (the tiles of this wave, 16 keys at a time)
+                        const int page = table[min(at >> plog, last)], there = (uint32_t)page >= (uint32_t)n_page ? 0 : end - at;
+                        const uint4 w = *(const uint4 *)(vbase + (uint64_t)(there == 0 ? 0 : page) * vp_g + (uint32_t)(32 * d + n) * vp_d + (at & pmask) * 2);
+                        uint32_t seen = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) seen |= (uint32_t)(at + j >= lo && at + j < hi && there > 0) << j;
+                        n_seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(of_kind(first_of(w, there), kind), ones(seen), n_seen, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) if (n_seen[j] != 0.0f) o[d][j] += kind_value(kind);
+                }
+            }
+        }
     }
     constexpr int HAVE = DT / GROUPS;                                      // output tiles that this wave has in the end, from `d0` on
     const int d0 = group * HAVE;
@@ -678,7 +696,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 o[d][i] = group ? o[HAVE + d][i] : o[d][i];
             }
         __syncthreads();
-        const float m2 = take[0], top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top, f = exp2_(m - base), f2 = exp2_(m2 - base);
+        const float m2 = take[0], top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top, f = above_0(exp2_(m - base)), f2 = above_0(exp2_(m2 - base));
         m = top;
         l = l * f + take[64] * f2;
 #pragma unroll
@@ -760,7 +778,7 @@ template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void j
             float w = 0.0f;
             if (lane < n) {
                 const float *q = part + (base + lane) * STEP + TILE * D + 16 * sub + row;
-                w = exp2_((base ? q[0] : m0[i]) - (top[i] == -INFINITY ? 0.0f : top[i]));
+                w = above_0(exp2_((base ? q[0] : m0[i]) - (top[i] == -INFINITY ? 0.0f : top[i])));
                 sum[i] += w * (base ? q[TILE] : l0[i]);
             }
             s_w[row][lane] = w;
