@@ -410,6 +410,7 @@ template <int D> struct chunk_shared { chunk_group<D> group[chunk_groups(D)]; in
 template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(const attn_args &a, chunk_shared<D> &shared, int block) {
     constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
     constexpr int KC = D / 8, KR = 64 / KC, GROUPS = chunk_groups(D);      // 16-byte pieces of a K row, K rows per request
+    static_assert(2 * KS == 4 * NI && 4 * DT == 4 * NI);                   // a request beside every fourth product, and every fourth step of the second product
     const int tid = threadIdx.x, lane = tid & 63, wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3, group = wave8 >> 2, n = lane & 31, half = lane >> 5;
     chunk_group<D> &sh = shared.group[group];
     // heads fastest: a head's tiles run on one XCD where the number of heads is a multiple of 8, and share its L2
@@ -587,7 +588,7 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p, o[d], 0, 0, 0);
                 if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p2, o[d], 0, 0, 0);
                 if (k < 2) w[k & 1][d] = v_piece(d, k + 2);
-                if (d % 4 == 0) ask_v(v_from, (buf ^ 1) * BUF, more, (k * DT + d) / 4);
+                if ((k * DT + d) % 4 == 0) ask_v(v_from, (buf ^ 1) * BUF, more, (k * DT + d) / 4);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
