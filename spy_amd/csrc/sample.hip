@@ -50,9 +50,9 @@ static __device__ __forceinline__ float logit_of(u64 x) {
 // e^((l - max) / T) = 2^-y as a multiple of 2^-44, y = (max - l) log2(e) / T.  log2(e) / T in two floats: a rounded one alone would shift all weights of the same
 // distance the same way.  The exponential is good to an ulp.
 struct weigher {
-    float top, c, c_lo, cap;           // cap: distances from here on count as this one, y as 1e20 at most: products beyond a float would have either sign
+    float top, unit, c, c_lo, cap;     // top and distances in units of 1 / unit; cap: distances from here on count as this one, y as 1e20 at most: products beyond a float would have either sign
     __device__ __forceinline__ float far(float l) const {                         // -inf: as good as infinitely far
-        const float d = fminf(top - l, cap);
+        const float d = fminf(fmaf(-l, unit, top), cap);
         return fmaf(d, c, d * c_lo);
     }
     static __device__ __forceinline__ u64 at(float y) {
@@ -349,8 +349,10 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
         return;
     }
     weigher weigh;
-    const double c = 1.4426950408889634074 / (double)temp;
-    weigh.top = top; weigh.c = (float)c; weigh.c_lo = (float)(c - (double)weigh.c);
+    // Beside a large temperature distances past the largest float count: they are taken in units of 2^64, which loses logits that are nothing beside it
+    weigh.unit = temp > 1e18f ? 0x1p-64f : 1.0f;
+    const double c = 1.4426950408889634074 / ((double)temp * (double)weigh.unit);
+    weigh.top = top * weigh.unit; weigh.c = (float)c; weigh.c_lo = (float)(c - (double)weigh.c);
     if (!(weigh.c <= 3.4e38f)) { weigh.c = 3.4e38f; weigh.c_lo = 0.0f; }          // a temperature next to 0
     weigh.cap = weigh.c > 1e-18f ? 1e20f / weigh.c : 3.4e38f;
     const bool by_rank = k > 0 && k < a.n, by_mass = p < 1.0f;
@@ -425,7 +427,7 @@ __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
         __syncthreads();
     }
     bool summed = false;                                                          // the kept weights of this wave's part are in s.part
-    const bool flat = weigh.c < 1e-30f;                                           // a temperature by which -inf is not far enough away by itself
+    const bool flat = weigh.c == 0.0f;                                            // an infinite temperature: -inf is not far away by itself
     if (by_rank || by_mass) {
         const float reach = (float)(SM_BINS - 1) / 32.0f;                         // distances from here on have one bin together
         u64 tail = 0;
