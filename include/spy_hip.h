@@ -193,11 +193,12 @@ int spy_hip_argmax(void *stream, const float *logits, int64_t n, int32_t *out_in
  *   the token drawn is, in order of index, the first kept one at which the running sum of w exceeds uniform * (sum of the kept w).
  * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab at most 2^18.  All five settings are device arrays with one value per
  * row; NULL: temperature 1, no top_k, no min_p, no top_p.  uniform is required: numbers in [0, 1) (below 0 and NaN count as 0, 1 and above as the last number before 1).
- * temperature <= 0 (or NaN) takes the first of the largest logits.  -inf and NaN logits are never drawn; where a logit is +inf, all that are +inf have w = 1 and
+ * temperature <= 0 (or NaN) takes the first of the largest logits, with probability 1.  -inf and NaN logits are never drawn; where a logit is +inf, all that are +inf have w = 1 and
  * the others 0.  A row without a logit above -inf gives token -1 and probability 0.
  * tokens: n_row int32, device; probs: n_row floats or NULL: w of the token / sum of the kept w.
- * Weights are held as multiples of 2^-44 of the largest and added as integers, so that a result depends on no order of additions; tokens whose w is below that
- * have none.  scratch: device memory of spy_hip_sample_scratch_size bytes, 256-byte aligned, this call's alone until the stream has passed it. */
+ * Weights are 32-bit exponentials, held as multiples of 2^-44 of the largest and added as integers, so that a result depends on no order of additions; tokens whose w is
+ * below that have none.  With y = log2(1 / w) one is off by at most (0.7 y + 1) * 2^-23 of itself (the rounding of max l - l, of y, and the exponential's) and 2^-44: the
+ * token differs from the definition's only where top_p or uniform is as close to a border between two tokens.  scratch: device memory of spy_hip_sample_scratch_size bytes, 256-byte aligned, this call's alone until the stream has passed it. */
 typedef struct spy_hip_sample_param {
     const float   *temperature;
     const int32_t *top_k;

@@ -48,7 +48,8 @@ static __device__ __forceinline__ float logit_of(u64 x) {
 }
 
 // e^((l - max) / T) = 2^-y as a multiple of 2^-44, y = (max - l) log2(e) / T.  log2(e) / T in two floats: a rounded one alone would shift all weights of the same
-// distance the same way.  The exponential is good to an ulp.
+// distance the same way.  max - l and y are rounded to 2^-24 of themselves, which moves the weight by up to y ln 2 * 2^-23; the exponential is good to an ulp.  (The distance in
+// two floats and y with its remainder would take off the former: 94 us instead of 82 for 256 rows of 100003, 28.3 instead of 23.9 for 64 of 32000.)
 struct weigher {
     float top, unit, c, c_lo, cap;     // top and distances in units of 1 / unit; cap: distances from here on count as this one, y as 1e20 at most: products beyond a float would have either sign
     __device__ __forceinline__ float far(float l) const {                         // -inf: as good as infinitely far

@@ -45,3 +45,26 @@ def test_small_logits_keep_their_rank_beside_a_large_temperature(hip):
         got, prob = draw(hip, l, uniform=np.array([0.0, 0.99999994], np.float32), temperature=np.float32(1e30), top_k=k)
         kept = np.sort(order[:k])
         assert got.tolist() == [kept[0], kept[-1]] and np.abs(prob - 1 / k).max() <= 2.0 ** -22 / k
+
+
+@pytest.mark.parametrize("temperature", [0.3, 0.7, 1.0, 1.3, 40.0])
+def test_what_a_weight_is_off_by(hip, temperature):
+    """Tokens of every weight down to 2^-40 drawn one by one.  With y = log2(1 / w): max - l is off by 2^-24 of itself, y once more, which is y ln 2 * 2^-23 of the weight,
+    the exponential by an ulp (2^-23), the weight's step is 2^-44; the sum by what its weights are, and the probability is rounded (2^-24)."""
+    rng = np.random.default_rng(7)
+    t = np.float64(np.float32(temperature))
+    n = 400
+    l = np.sort(rng.uniform(-40, 0, n) * np.log(2) * t + 5 * t).astype(np.float32)      # light tokens first, where uniform has fine steps
+    y = (np.float64(l[-1]) - l.astype(np.float64)) * np.log2(np.e) / t
+    w = 2.0 ** -y
+    run = np.cumsum(w)
+    u = ((run - w / 2) / run[-1]).astype(np.float32)
+    off = w * (0.7 * y + 1) * 2.0 ** -23 + 2.0 ** -44
+    clear = np.minimum(w / 2, run[-1] - run + w / 2) > 4 * (np.cumsum(off) + u * off.sum() + run * 2.0 ** -23)      # (some weigh less than all before them are off by)
+    assert clear.sum() > n * 3 // 4 and y[clear].max() > 35
+    got, prob = draw(hip, np.repeat(l[None], n, axis=0), uniform=u, temperature=np.float32(temperature))
+    assert np.array_equal(got[clear], np.arange(n)[clear])
+    tol = (off / w + off.sum() / run[-1] + 2.0 ** -24) * w / run[-1]
+    have = np.abs(prob - w / run[-1])[clear] / tol[clear]
+    print("worst error / bound %.2f, in 2^-23 of the weight %.1f" % (have.max(), (np.abs(prob * run[-1] / w - 1) * 2 ** 23)[clear][y[clear] < 20].max()), flush=True)
+    assert have.max() <= 1
