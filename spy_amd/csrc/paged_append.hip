@@ -80,6 +80,9 @@ static __device__ __forceinline__ void append_rows(const append_args &a, int til
         }
         if (lane == 0) { s_pos[wave] = takes ? pos : INT32_MIN; s_page[wave] = page; }
     }
+    // entries that are wrong but belong to no row: one workgroup's idle wave looks at all (with tiles of V every workgroup that finds none does)
+    if (VROWS && blockIdx.x == 0 && wave == R)
+        for (int i = lane; i < a.b.n_seq; i += 64) pg_sequence(a.b, i, a.err);
     __syncthreads();
     if (a.mode >= 0) {
         for (int i = tid; i < R * npair; i += PA_THREADS) {
