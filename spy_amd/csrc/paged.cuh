@@ -1,6 +1,7 @@
 // What the kernels over a cache in pages share: where a batch's sequences, rows and pages are.
 #pragma once
 
+#include "rows_meet.h"
 #include "scan.cuh"
 
 struct pg_batch {

@@ -232,6 +232,7 @@ extern "C" int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const
         a.turn0 = log2((double)rope->freq_scale) - 2.6514961294723187980432933;             // log2(2 pi)
         a.mscale = rope->attention_factor;
     }
+    SPY_CHECK_ARG(!q || (!pg_rows_meet(q_out, q) && !pg_rows_meet(q_out, k) && !pg_rows_meet(q_out, v)));
     a.q = q ? (const uint8_t *)q->data : nullptr; a.k = (const uint8_t *)k->data; a.v = (const uint8_t *)v->data;
     a.qo = q ? (uint8_t *)q_out->data : nullptr; a.kp = (uint8_t *)k_pages->data; a.vp = (uint8_t *)v_pages->data;
     a.q_h = q ? q->nb[1] : 0; a.q_t = q ? q->nb[2] : 0; a.qo_h = q ? q_out->nb[1] : 0; a.qo_t = q ? q_out->nb[2] : 0;

@@ -913,12 +913,13 @@ extern "C" int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, co
     if (rc) return rc;
     if (q->type != SPY_HIP_F16 || (out->type != SPY_HIP_F32 && out->type != SPY_HIP_F16)) return SPY_HIP_EUNSUPPORTED;
     const int64_t hd = k_pages->ne[0], ps = k_pages->ne[1], G = k_pages->ne[2], n_row = q->ne[2], H = q->ne[1];
-    SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3] && out->data != q->data);
+    SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3]);
     SPY_CHECK_ARG(pg_rows_ok(q, hd, H, n_row) && pg_rows_ok(out, hd, H, n_row) && window >= 0 && fabsf(scale) >= 1e-37f && fabsf(scale) <= 1e24f);
     if (p.scratch) {
         if (scratch_bytes < p.scratch) return SPY_HIP_ENOSPACE;
         SPY_CHECK_ARG(scratch && ((uintptr_t)scratch & 255) == 0);
     }
+    SPY_CHECK_ARG(!pg_rows_meet(out, q));
     attn_args a;
     a.q = (const uint8_t *)q->data; a.kp = (const uint8_t *)k_pages->data; a.vp = (const uint8_t *)v_pages->data; a.out = (uint8_t *)out->data;
     a.q_h = q->nb[1]; a.q_t = q->nb[2]; a.o_h = out->nb[1]; a.o_t = out->nb[2];

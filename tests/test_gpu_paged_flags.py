@@ -42,3 +42,24 @@ def test_append_and_attention_raise_the_flag(hip, new, wrong):
         assert np.array_equal(p.k_at(got_k, s, pos), k[row]) and np.array_equal(p.v_at(got_v, s, pos), v[row])
     P.run_attention(p, q, True)
     assert (P.flag() != 0) == (wrong != "none")
+
+
+@pytest.mark.parametrize("by_head", [False, True])
+def test_append_of_parts_of_one_wide_row(hip, by_head):
+    """q, k, v and q_out side by side in one buffer, as blocks of heads or head by head, which is no overlap: all of q_out is written, and nothing else."""
+    from spy_amd import _lib as H
+    rng = np.random.default_rng(1)
+    p = P.Paged(rng, [(1, 20), (12, 30)], 2, 2, 64, 16)
+    p.upload()
+    wide = rng.standard_normal((p.rows, 9, 64)).astype(np.float16)
+    at = {"q": 0, "k": 1, "v": 2, "qo": 3} if by_head else {"q": 0, "k": 2, "v": 4, "qo": 6}
+    head = 4 if by_head else 1
+    buf = H.DeviceBuffer.from_numpy(wide.view(np.uint16))
+    t = {n: H.tensor(buf, H.F16, [64, 2, p.rows], [2, 128 * head, 9 * 128], offset=128 * o) for n, o in at.items()}
+    B = P.C.byref
+    H.check(H.load().spy_hip_paged_append(None, B(t["q"]), B(t["k"]), B(t["v"]), B(p.batch), None, B(t["qo"]), B(p.t_k), B(p.t_v)), "spy_hip_paged_append")
+    got, n = buf.download(np.float16).reshape(wide.shape), int(p.row_start[-1])
+    want = wide.copy()
+    for h in range(2):
+        want[:n, at["qo"] + head * h] = wide[:n, at["q"] + head * h]
+    assert np.array_equal(got, want) and P.flag() == 0
