@@ -191,7 +191,7 @@ int spy_hip_argmax(void *stream, const float *logits, int64_t n, int32_t *out_in
  *     min_p   those with w >= min_p (0 or less: all; more than 1 counts as 1)
  *     top_p   the fewest whose w add up to top_p times the sum over the tokens that top_k leaves (1 or more: all)
  *   the token drawn is, in order of index, the first kept one at which the running sum of w exceeds uniform * (sum of the kept w).
- * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab at most 2^18.  All five settings are device arrays with one value per
+ * logits: F32 rows {n_vocab, n_row}, nb[0] = 4, rows any multiple of 4 bytes apart, n_vocab at most 2^18, n_row below 2^22.  All five settings are device arrays with one value per
  * row; NULL: temperature 1, no top_k, no min_p, no top_p.  uniform is required: numbers in [0, 1) (below 0 and NaN count as 0, 1 and above as the last number before 1).
  * temperature <= 0 (or NaN) takes the first of the largest logits, with probability 1.  -inf and NaN logits are never drawn; where a logit is +inf, all that are +inf have w = 1 and
  * the others 0.  A row without a logit above -inf gives token -1 and probability 0.
@@ -215,7 +215,8 @@ int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sam
  *      h / (n_head / n_kv_head)).  Sequences may share pages that neither call appends to.
  *      The device arrays are read when the call runs, so that a recorded call can be replayed with other lengths, rows and pages in them.  A sequence that does
  *      not fit -- more new tokens than max_new, more cached ones than max_kv or than page_stride pages hold, rows outside the tensors -- raises the error flag of
- *      spy_hip_take_error and takes no part: its rows are left alone. ----------------- */
+ *      spy_hip_take_error and takes no part: its rows are left alone.  SPY_HIP_EINVAL also for batches whose launch would have 2^32 threads or more (some millions of
+ *      rows or sequences). ----------------- */
 typedef struct spy_hip_paged_batch {
     int32_t n_seq;               /* sequences */
     int32_t max_new, max_kv;     /* no sequence has more new / cached tokens than these (the launches are sized by them) */

@@ -247,7 +247,7 @@ extern "C" int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const
     const bool f16 = k->type == SPY_HIP_F16, tiles = batch->max_new >= 8 && n_row >= 128;
     const int64_t heads = H + G * (tiles ? 1 : 2), per = tiles ? heads : PA_THREADS / (hd / 16), chunks = (heads + per - 1) / per;
     const int64_t row_blocks = (tiles ? (n_row + 3) / 4 : n_row) * chunks, blocks = row_blocks + (tiles ? (n_row / 64 + 2 * (int64_t)batch->n_seq) * G : 0);
-    SPY_CHECK_ARG(blocks < (1ll << 31));
+    SPY_CHECK_ARG(blocks * PA_THREADS < (1ll << 32));                       // threads of a launch
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)blocks), block(PA_THREADS);
     if (tiles) {

@@ -883,7 +883,8 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
         // one workgroup per compute unit fits (512 tokens on 7680: 92 us, 101 with two per unit, 118 with three for four units), 512 keys at least
         attn_share(p.chunk_units, ((int64_t)b->max_kv + 63) / 64 + 1, cu, 8, p.chunk_split, p.chunk_pieces);
     }
-    SPY_CHECK_ARG(p.few_units * p.few_pieces + p.chunk_units * p.chunk_pieces < (1ll << 30) && p.chunk_units * (CHUNK_ROWS / 16) < (1ll << 30));
+    // threads of a launch are a number of 32 bits
+    SPY_CHECK_ARG((p.few_units * p.few_pieces + p.chunk_units * p.chunk_pieces) * (p.chunk_units ? 256 * chunk_groups((int)hd) : 256) < (1ll << 32) && (p.few_units + p.chunk_units * (CHUNK_ROWS / 16)) * 256 < (1ll << 32));
     p.few_bytes = p.few_pieces > 1 ? (size_t)(p.few_units * p.few_pieces * 16 * (hd + 2) * 4) : 0;
     p.scratch = p.few_bytes + (p.chunk_pieces > 1 ? (size_t)(p.chunk_units * p.chunk_pieces * CHUNK_ROWS * (hd + 2) * 4) : 0);
     return 0;

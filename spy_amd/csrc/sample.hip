@@ -580,7 +580,7 @@ extern "C" int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const 
     SPY_CHECK_ARG(logits && param && tokens && logits->data && param->uniform);
     if (logits->type != SPY_HIP_F32) return SPY_HIP_EUNSUPPORTED;
     const int64_t n = logits->ne[0], n_row = logits->ne[1];
-    SPY_CHECK_ARG(n > 0 && n <= SM_VOCAB && n_row > 0 && n_row < (1ll << 31) && logits->ne[2] == 1 && logits->ne[3] == 1 && logits->nb[0] == 4 && logits->nb[1] % 4 == 0);
+    SPY_CHECK_ARG(n > 0 && n <= SM_VOCAB && n_row > 0 && n_row * SM_THREADS < (1ll << 32) && logits->ne[2] == 1 && logits->ne[3] == 1 && logits->nb[0] == 4 && logits->nb[1] % 4 == 0);
     SPY_CHECK_ARG((((uintptr_t)logits->data | (uintptr_t)tokens | (uintptr_t)probs | (uintptr_t)param->temperature | (uintptr_t)param->top_k | (uintptr_t)param->top_p |
                     (uintptr_t)param->min_p | (uintptr_t)param->uniform) & 3) == 0);
     sample_args a;
