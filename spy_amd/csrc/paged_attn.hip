@@ -29,9 +29,9 @@ struct attn_args {
     int G, group;                        // K/V heads, query heads to one
     float c;                             // scale * log2(e)
     int causal, window;                  // window: 0 or how many positions back
-    // Sequences of few rows: tiles of 16 rows per sequence and K/V head, key tiles (of 32) per workgroup, workgroups that share a row's keys at most.  The others:
+    // Sequences of up to `few` rows: one tile of 16 per sequence and K/V head, key tiles (of 32) per workgroup, workgroups that share a row's keys at most.  The others:
     // tiles of CHUNK_ROWS rows over all sequences, key tiles (of 64).
-    int few, few_tiles, few_split, few_pieces, few_blocks;
+    int few, few_split, few_pieces, few_blocks;
     int chunk_tiles, chunk_split, chunk_pieces, chunk_blocks;
     float *few_part, *chunk_part;        // (o, m, l) of the workgroups that share rows
     int *err;
@@ -131,14 +131,12 @@ template <int D, int WAVES> struct few_shared {
 template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void attn_few(const attn_args &a, few_shared<D, WAVES> &sh, int block) {
     constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D, WAVES>::HALF;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quarter = lane >> 4;
-    const int units = a.b.n_seq * a.few_tiles * a.G, piece = block / units, unit = block - piece * units;
-    const int s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
+    const int units = a.b.n_seq * a.G, piece = block / units, unit = block - piece * units, s = unit / a.G, head = unit - s * a.G;
     const pg_seq sq = pg_sequence(a.b, s, a.err);
     if (!sq.ok) return;
-    const row_tile rt(a, sq, tile, 16);
-    if (rt.n_row <= 0 || rt.rows > a.few) return;
-    const int rows = rt.rows, r0 = rt.r0;
-    const int r = min(r0 + n, rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
+    const row_tile rt(a, sq, 0, 16);
+    if (rt.rows > a.few) return;
+    const int rows = rt.rows, r = min(n, rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
     const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all(), begin = rt.lo_any() & ~31, end = rt.end();
     const int n_tile = max((end - begin + 31) >> 5, 0);
     if (piece > 0 && piece * a.few_split >= n_tile) return;
@@ -297,10 +295,10 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
             const float base = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
             for (int w = 0; w < WAVES; w++) sum += sh.l[w][row] * exp2_(sh.m[w][row] - base);
-            if (r0 + row >= rows) continue;
+            if (row >= rows) continue;
             const int dd = h * HALF + d;
             if (whole) {
-                const int t = (r0 + row) / a.group, hh = head * a.group + (r0 + row - t * a.group);
+                const int t = row / a.group, hh = head * a.group + (row - t * a.group);
                 uint8_t *dst = a.out + (int64_t)(sq.row0 + t) * a.o_t + (int64_t)hh * a.o_h;
                 const bool none = mx == -INFINITY && sum == 0.0f;          // sees no key
 #pragma unroll
@@ -817,11 +815,11 @@ template <int D, bool F32OUT, int TILE> static __device__ __forceinline__ void j
 }
 template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_join_kernel(attn_args a, int few_units) {
     if ((int)blockIdx.x < few_units) {
-        const int unit = blockIdx.x, s = unit / (a.few_tiles * a.G), rest = unit - s * a.few_tiles * a.G, tile = rest / a.G, head = rest - tile * a.G;
+        const int unit = blockIdx.x, s = unit / a.G, head = unit - s * a.G;
         const pg_seq sq = pg_sequence(a.b, s, nullptr);
         if (!sq.ok) return;
-        const row_tile rt(a, sq, tile, 16);
-        if (rt.n_row <= 0 || rt.rows > a.few) return;
+        const row_tile rt(a, sq, 0, 16);
+        if (rt.rows > a.few) return;
         const int n_tile = max((rt.end() - (rt.lo_any() & ~31) + 31) >> 5, 0), pieces = (n_tile + a.few_split - 1) / a.few_split;
         if (pieces > 1) join_rows<D, F32OUT, 16>(a, rt, sq, head, 0, pieces, a.few_part + (int64_t)unit * a.few_pieces * 16 * (D + 2));
         return;
@@ -850,8 +848,8 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256 * chunk_groups(D)
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
 // Rows of a sequence that go by tiles of 16, the rest by tiles of 128 (128-wide, 32 heads; by tiles of 16 and of 128): 17 rows on 4096 keys 29.6 and 26.6 us, 64 rows 46.5
 // and 28.8; eight sequences of 17 rows 145 and 106; only one short sequence is faster by tiles of 16 (17 rows on 500 keys: 14.4 and 17.5).
-#define FEW_ROWS 16
-struct attn_plan { int64_t few, few_tiles, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
+#define FEW_ROWS 16        // one tile
+struct attn_plan { int64_t few, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
 // `units` tiles by heads and `key_tiles` tiles of keys: key tiles per workgroup so that `want` workgroups get work, `least` of them at least
 static void attn_share(int64_t units, int64_t key_tiles, int64_t want, int64_t least, int64_t &split, int64_t &pieces) {
     const int64_t n = (want + units - 1) / units;
@@ -871,8 +869,7 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
     // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups.  Few rows: 256 keys at least (one request of 4096 keys,
     // 32 heads: 20 us, 23.5 with 128 keys), else for six workgroups per compute unit (8 requests of up to 30000: 142 us, 150 with two, 151 with three).
     p.few = most > FEW_ROWS && b->n_seq == 1 ? 0 : FEW_ROWS;              // a single sequence that may bring many rows goes one way whatever it brings: no empty launches
-    p.few_tiles = (FEW_ROWS + 15) / 16;
-    p.few_units = p.few ? (int64_t)b->n_seq * p.few_tiles * G : 0;
+    p.few_units = p.few ? (int64_t)b->n_seq * G : 0;
     p.few_split = 1; p.few_pieces = 0;
     if (p.few) attn_share(p.few_units, ((int64_t)b->max_kv + 31) / 32 + 1, 6 * cu, 8, p.few_split, p.few_pieces);
     p.chunk_tiles = p.chunk_units = 0; p.chunk_split = p.chunk_pieces = 1;
@@ -929,7 +926,7 @@ extern "C" int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, co
     a.b.row_start = batch->row_start; a.b.kv_len = batch->kv_len; a.b.pages = batch->pages; a.b.page_stride = batch->page_stride;
     a.b.n_seq = batch->n_seq; a.b.n_row = (int)n_row; a.b.max_new = batch->max_new; a.b.max_kv = batch->max_kv; a.b.n_page = (int)k_pages->ne[3]; a.b.page_log2 = pg_log2(ps);
     a.G = (int)G; a.group = (int)(H / G); a.c = scale * 1.44269504088896341f; a.causal = causal != 0; a.window = window > (1 << 30) ? 0 : window;
-    a.few = (int)p.few; a.few_tiles = (int)p.few_tiles; a.few_split = (int)p.few_split; a.few_pieces = (int)p.few_pieces; a.few_blocks = (int)(p.few_units * p.few_pieces);
+    a.few = (int)p.few; a.few_split = (int)p.few_split; a.few_pieces = (int)p.few_pieces; a.few_blocks = (int)(p.few_units * p.few_pieces);
     a.chunk_tiles = (int)p.chunk_tiles; a.chunk_split = (int)p.chunk_split; a.chunk_pieces = (int)p.chunk_pieces; a.chunk_blocks = (int)(p.chunk_units * p.chunk_pieces);
     a.few_part = (float *)scratch; a.chunk_part = (float *)((uint8_t *)scratch + p.few_bytes); a.err = spy_hip_err_flag_ptr();
     hipStream_t st = (hipStream_t)stream;
