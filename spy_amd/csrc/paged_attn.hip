@@ -115,6 +115,7 @@ static __device__ __forceinline__ v8h ones(uint32_t bits) {
 }
 static __device__ __forceinline__ float kind_value(int kind) { return kind == 2 ? NAN : kind ? -INFINITY : INFINITY; }
 static __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+static __device__ __forceinline__ float larger(float top, float x) { return __builtin_elementwise_maximum(top, fabsf(x)); }       // NaN if either is; two of them are one instruction
 // A factor from one m to another that leaves infinities infinite: what is not above 2^-126 of a larger part adds nothing to it, as with 0
 static __device__ __forceinline__ float above_0(float f) { return fmaxf(f, 0x1p-126f); }
 
@@ -241,11 +242,12 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
         if (kt + WAVES < stop) load_v(v_row(kt + WAVES, pg1));
         pg = pg1; pg1 = pg2;
     }
+    float most = 0.0f;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) unbounded |= !finite(o[d][i]);
-    if (__any(unbounded)) {
+        for (int i = 0; i < 4; i++) most = larger(most, o[d][i]);
+    if (__any(unbounded || !finite(most))) {
 #pragma unroll
         for (int d = 0; d < DT; d++) {
 #pragma unroll
@@ -649,12 +651,12 @@ template <int D, bool F32OUT> static __device__ __forceinline__ void attn_chunk(
         if (idle) while (!step(std::true_type{})) {}
         else while (!step(std::false_type{})) {}
         __syncthreads();
-        bool unbounded = shared.unbounded;
+        float most[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) unbounded |= !finite(o[d][j]);
-        if (__any(unbounded)) {
+            for (int j = 0; j < 16; j++) most[j & 1] = larger(most[j & 1], o[d][j]);
+        if (__any(shared.unbounded || !finite(larger(most[0], most[1])))) {
 #pragma unroll
             for (int d = 0; d < DT; d++) {
 #pragma unroll
