@@ -240,10 +240,12 @@ int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const spy_hip_te
 /* Attention of the batch's new tokens over the pages (which hold them already): MatMul(K, q) -> Softmax(mask, scale) -> MatMul(V^T, P) per sequence and head
  * (attention.cpp:25-302).  q {hd, n_head, n_row} F16, out the same shape F32 or F16, strides and alignment as above.  A token sees the positions below
  * kv_len of its sequence; causal != 0: none behind its own; window > 0: none at or before its own less `window`.  A token that sees no
- * position gets zeros; what lies in the pages at positions it does not see, infinities and NaN too, does not reach its output.  Infinities and NaN in V at positions that it
- * sees are its output in their dimension, whatever they weigh: that infinity, or NaN where there are both or a NaN.  Pages outside 0 .. n_page - 1 hold nothing
- * and raise the error flag.  scale: 1e-37 to 1e24 in magnitude.  out must not overlap q.  Scores, sums and the product are fp32; a probability enters the product as fp16
- * for F16 outputs (off by 2^-11 of itself) and as two fp16 terms for F32 outputs (2^-22), or off by 2^-35 of the row's largest probability where that is more.
+ * position gets zeros; what lies in the pages at positions it does not see, infinities and NaN too, does not reach its output.  Infinities and NaN in V at positions
+ * that it sees are its output in their dimension, whatever they weigh: that infinity, or NaN where there are both or a NaN.  Pages outside 0 .. n_page - 1 hold nothing
+ * and raise the error flag.  scale: 1e-37 to 1e24 in magnitude.  out must not overlap q.
+ * Scores, sums and the product are fp32.  A probability enters the product as two fp16 terms (off by 2^-22 of itself); as one (2^-11) where outputs are F16 and the
+ * sequence has more than 16 rows (new tokens times query heads per K/V head) or is the only one of a batch whose max_new allows it more; in either case off by 2^-35 of the
+ * row's largest probability where that is more.
  * scratch: device memory of spy_hip_paged_attention_scratch_size bytes, 256-byte aligned, this call's alone until the stream has passed it (a captured call: until its
  * graph is done with); its contents need not be set. */
 size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch);

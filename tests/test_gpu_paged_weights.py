@@ -105,3 +105,16 @@ def test_scores_past_the_whole_numbers_of_a_float(hip, scale, new, f32):
             got = P.run_attention(p, q, f32, causal=0, scale=scale)[:int(p.row_start[-1])].astype(np.float64)
             # a sum of weights divided by the same sum: (n / 4 + 192) additions on either side, a weight as it enters the one and the other
             assert np.abs(got - 1).max() <= 2 * (n / 4 + 192) * P.EPS32 + (2.0 ** -22 if f32 else 2 * P.EPS16), (n_seq, q0, np.abs(got - 1).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n_seq", [1, MANY[1]])
+def test_f16_outputs_of_few_rows_are_rounded_f32_outputs(hip, hd, n_seq):
+    """Sequences of few rows take probabilities as two terms for either type: the F16 output is the F32 output rounded, to the bit."""
+    print("f16 as f32: hd %d n_seq %d" % (hd, n_seq), flush=True)
+    rng = np.random.default_rng(hd)
+    k, v = (rng.standard_normal((1700, hd)).astype(np.float16) for _ in range(2))
+    p = _batch(1, n_seq, hd, k, v)
+    q = rng.standard_normal((p.rows, 2, hd)).astype(np.float16)
+    a, b = P.run_attention(p, q, True, causal=0), P.run_attention(p, q, False, causal=0)
+    assert np.array_equal(a[:n_seq].astype(np.float16), b[:n_seq])
