@@ -124,8 +124,8 @@ static __device__ __forceinline__ float above_0(float f) { return fmaxf(f, 0x1p-
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
 // Bound by the bytes of K and V.  The waves take tiles of 32 keys in turn, straight from memory into the registers of the matrix instruction: nothing is shared
-// between waves before the end.  Measured: 64 requests of up to 4096 cached tokens (32 heads to 8, 128 wide, pages of 16) 128 us, 5.1 TB/s; 8 of up to 30000 (64 heads to 8)
-// 137 us, 4.9 TB/s; one of 4096 (32 heads) 15 us, 4.6 TB/s, and 4.5 us for the join.
+// between waves before the end.  Measured: 64 requests of up to 4096 cached tokens (32 heads to 8, 128 wide, pages of 16) 125 us, 5.1 TB/s; 8 of up to 30000 (64 heads to 8)
+// 135 us, 4.9 TB/s; one of 4096 (32 heads) 14 us, 4.8 TB/s, and 4.4 us for the join; 32 of up to 4096 (16 heads to 8, 256 wide, F32 outputs) 140 us, 4.7 TB/s.
 template <int D, int WAVES> struct few_shared {
     static constexpr int HALF = D < 128 ? D : 128;
     float m[WAVES][16], l[WAVES][16];
@@ -318,14 +318,15 @@ template <int D, bool F32OUT, int WAVES> static __device__ __forceinline__ void 
 }
 
 // ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
-// Bound by the matrix cores and the vector instructions of the softmax together: 64 keys by 32 rows take a wave (D = 128) 32 matrix instructions of 33 cycles, and some 215
-// vector instructions of 4.7, 32 of them exponentials of 11; two waves of a SIMD need 4600 of the 5200 cycles that a step takes.  Measured (128 wide, 32 heads): a prompt of
-// 2048 tokens 55 us, 628 TFLOP/s of what its rows see; 512 tokens on 7680 88 us, 754 TFLOP/s; 13 us of the former are spent outside the loop, by two workgroups one after the
-// other.  Tried and not kept (where this had 57 and 91 us): the next tile's scores computed beside this one's exponentials in one instruction stream (58 and 91), a barrier for
-// each group by itself (59 and 98), the groups half a step apart, wave priorities (no difference).
+// Bound by the matrix cores and the vector instructions of the softmax together: 64 keys by 32 rows take a wave (D = 128) 32 matrix instructions of 33 cycles, and some 200
+// vector instructions of 4.7, 32 of them exponentials of 11; two waves of a SIMD need 4400 of the 5200 cycles that a step takes, since the step's barrier puts both into
+// the same phase, where they want the same units.  Measured (128 wide, 32 heads): a prompt of 2048 tokens 55 us, 628 TFLOP/s of what its rows see, with F32 outputs (half as
+// many matrix instructions again) 67; 512 tokens on 7680 87.5 us, 761 TFLOP/s, F32 112; 13 us of the former are spent outside the loop, by two workgroups one after the
+// other.  16 heads of 256, 512 tokens on 3584: 64.5 us, F32 75.8.  Tried and not kept (where this had 57 and 91 us): the next tile's scores computed beside this one's
+// exponentials in one instruction stream (58 and 91), a barrier for each group by itself (59 and 98), wave priorities (no difference).
 // Four waves have 32 rows each; a second group of four has the same rows and every other tile of keys, so that a SIMD always has a second wave, to the end of a long row
 // of keys, and the groups exchange halves of (m, l, o) at the end (one group of 256 rows would leave the short rows of a prompt's triangle without a second wave).
-// (256-wide heads: one group, whose waves have all registers to themselves.)  The 64 keys' K and V^T of a group lie in LDS,
+// (256-wide heads: one group, one wave per SIMD with 500 of its 512 registers in use.)  The 64 keys' K and V^T of a group lie in LDS,
 // requested straight from memory one tile ahead into the other of two buffers.  An LDS row is a row of the matrix instruction's operand (K: instruction row i of 32 is key
 // 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a lane's scores are those of 8 keys that follow each other, as the product wants its
 // probabilities); its 16-byte pieces are stored at their index xor a number of the row, so that the lanes of a read meet different banks.
@@ -850,8 +851,8 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256 * chunk_groups(D)
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------------
-// Rows of a sequence that go by tiles of 16, the rest by tiles of 128 (128-wide, 32 heads; by tiles of 16 and of 128): 17 rows on 4096 keys 29.6 and 26.6 us, 64 rows 46.5
-// and 28.8; eight sequences of 17 rows 145 and 106; only one short sequence is faster by tiles of 16 (17 rows on 500 keys: 14.4 and 17.5).
+// Rows of a sequence that go by a tile of 16, the rest by tiles of 128 (128-wide, 32 heads; by tiles of 16, of which a sequence may have had several then, and of 128): 17 rows on
+// 4096 keys 29.6 and 25.2 us, 64 rows 46.5 and 26.7; eight sequences of 17 rows 145 and 105; only one short sequence is faster by tiles of 16 (17 rows on 500 keys: 14.4 and 17.4).
 #define FEW_ROWS 16        // one tile
 struct attn_plan { int64_t few, few_units, few_split, few_pieces, chunk_tiles, chunk_units, chunk_split, chunk_pieces; size_t few_bytes, scratch; };
 // `units` tiles by heads and `key_tiles` tiles of keys: key tiles per workgroup so that `want` workgroups get work, `least` of them at least
@@ -871,7 +872,7 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
     const int64_t group = H / G, most = (int64_t)b->max_new * group, cu = spy_num_cu();
     SPY_CHECK_ARG(most < (1ll << 30));
     // Keys are shared out in pieces of one size, so that long sequences of a ragged batch take more workgroups.  Few rows: 256 keys at least (one request of 4096 keys,
-    // 32 heads: 20 us, 23.5 with 128 keys), else for six workgroups per compute unit (8 requests of up to 30000: 142 us, 150 with two, 151 with three).
+    // 32 heads: 18.0 us, 19.6 with 128 keys), else for six workgroups per compute unit (8 requests of up to 30000: 141 us, 148 with two, 150 with three).
     p.few = most > FEW_ROWS && b->n_seq == 1 ? 0 : FEW_ROWS;              // a single sequence that may bring many rows goes one way whatever it brings: no empty launches
     p.few_units = p.few ? (int64_t)b->n_seq * G : 0;
     p.few_split = 1; p.few_pieces = 0;
@@ -881,7 +882,7 @@ static int attn_make_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = q->ne[2] * group / CHUNK_ROWS + b->n_seq;
         p.chunk_tiles = each * b->n_seq < all ? each * b->n_seq : all;
         p.chunk_units = p.chunk_tiles * G;
-        // one workgroup per compute unit fits (512 tokens on 7680: 92 us, 101 with two per unit, 118 with three for four units), 512 keys at least
+        // one workgroup per compute unit fits (512 tokens on 7680: 87 us, 95 with two per unit, 119 with four; eight sequences of 17 rows 105, 125 and 139), 512 keys at least
         attn_share(p.chunk_units, ((int64_t)b->max_kv + 63) / 64 + 1, cu, 8, p.chunk_split, p.chunk_pieces);
     }
     // threads of a launch are a number of 32 bits
