@@ -42,7 +42,7 @@ extern "C" {
 /* NumberType ids (orchestration/include/number/number_impl/type.h:12-45) */
 enum spy_hip_type {
     SPY_HIP_F32 = 0, SPY_HIP_F16 = 1, SPY_HIP_Q4_0 = 2, SPY_HIP_Q8_0 = 8,
-    SPY_HIP_Q4_K = 12, SPY_HIP_Q6_K = 14, SPY_HIP_I32 = 26
+    SPY_HIP_Q4_K = 12, SPY_HIP_Q6_K = 14, SPY_HIP_I8 = 24, SPY_HIP_I32 = 26
 };
 
 /* spy::Tensor flattened (tensor.h:23-36, 209-222) */
@@ -251,6 +251,37 @@ int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const spy_hip_te
 size_t spy_hip_paged_attention_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch);
 int spy_hip_paged_attention(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *v_pages, const spy_hip_tensor *out,
                             const spy_hip_paged_batch *batch, float scale, int32_t causal, int32_t window, void *scratch, size_t scratch_bytes);
+/* The same cache in 8 bits, a little over half the bytes: K and V in blocks of 32 elements of a row, as Q8_0 blocks (spy_hip_quantize_q8_0; vec_convert.h:178-261), the whole
+ * numbers and the scales in planes of their own.  K pages I8 {hd, page_size, n_kv_head, n_page} beside K scales F16 {hd / 32, page_size, n_kv_head, n_page}; V^T pages I8 {page_size, hd,
+ * n_kv_head, n_page} beside V scales F16 {page_size, hd / 32, n_kv_head, n_page}.  nb[0] is 1 and 2; nb[1] of the K scales is hd / 16, the other strides are multiples of 16 bytes; data
+ * 16-byte aligned, limits as above.  An element stands for fp16(d * q), the product rounded once.
+ * With m the largest magnitude of a block: d = fp16(m / 127), q = x * (127 / m) to the nearest whole number, halves to even, of the F32 or F16 input (K: turned, in 32 bits).  A block that holds an
+ * infinity or NaN, or whose m / 127 is past the fp16 numbers, has d = NaN and reads back as NaN; one without a magnitude above 1e-36 has q = 0.  Everything else is as for
+ * spy_hip_paged_append, whose q_out this one has. */
+int spy_hip_paged_append_q8(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k, const spy_hip_tensor *v, const spy_hip_paged_batch *batch, const spy_hip_rope_param *rope,
+                            const spy_hip_tensor *q_out, const spy_hip_tensor *k_pages, const spy_hip_tensor *k_scales, const spy_hip_tensor *v_pages, const spy_hip_tensor *v_scales);
+/* spy_hip_paged_attention over that cache: bit for bit what it gives over F16 pages that hold fp16(d * q).  Infinities and NaN are those of these values. */
+size_t spy_hip_paged_attention_q8_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch);
+int spy_hip_paged_attention_q8(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *k_scales, const spy_hip_tensor *v_pages, const spy_hip_tensor *v_scales,
+                               const spy_hip_tensor *out, const spy_hip_paged_batch *batch, float scale, int32_t causal, int32_t window, void *scratch, size_t scratch_bytes);
+/* spy_hip_paged_attention, causal and without a window, for sequences that begin alike: those of a group have their first tokens in common, and what these are is read and multiplied once for all new
+ * tokens of the group instead of once for each sequence.  Groups are runs of sequences of the batch, in device arrays that are read when the call runs.  Sequences before the first
+ * group and behind the last share nothing. */
+typedef struct spy_hip_paged_prefix {
+    int32_t n_group;             /* groups */
+    int32_t max_rows;            /* no group has more new tokens in all ... */
+    int32_t max_prefix;          /* ... and more tokens in common than these (the launches are sized by them) */
+    const int32_t *seq_start;    /* device, n_group + 1 entries, ascending: group g is sequences seq_start[g] .. seq_start[g+1] - 1 */
+    const int32_t *length;       /* device, n_group entries: the first so many positions of every sequence of the group are the same (0: none).  Their pages are those of the group's first
+                                    sequence; in the others' rows of `pages` entries of pages that lie before that many positions are not needed */
+} spy_hip_paged_prefix;
+/* A new token lies behind what its group has in common: a group with a sequence for which that is not so, or that does not fit -- more rows than max_rows, more in common than max_prefix, sequences
+ * outside the batch -- raises the error flag, and that sequence, or the group's sequences, take no part: their rows are left alone.  k_scales and v_scales: NULL with F16 pages, the
+ * scales of I8 pages else.  Results differ from those of spy_hip_paged_attention in the order of the sums (fp32) alone.  Everything else is as there, the scratch of its own size too. */
+size_t spy_hip_paged_attention_shared_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix);
+int spy_hip_paged_attention_shared(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *k_scales, const spy_hip_tensor *v_pages,
+                                   const spy_hip_tensor *v_scales, const spy_hip_tensor *out, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix, float scale, void *scratch,
+                                   size_t scratch_bytes);
 
 /* ---- kernel families used by the operators above and by the fused token loop --------------- */
 

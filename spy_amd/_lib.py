@@ -11,9 +11,9 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SPY_HIP_LIBRARY") or os.path.join(HERE, "libspy_hip.so")     # override: an alternative build of the same ABI
 
-F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, I32 = 0, 1, 2, 8, 12, 14, 26
-TYPE_SIZE = {F32: 4, F16: 2, Q4_0: 18, Q8_0: 34, Q4_K: 144, Q6_K: 210, I32: 4}
-BLOCK_SIZE = {F32: 1, F16: 1, Q4_0: 32, Q8_0: 32, Q4_K: 256, Q6_K: 256, I32: 1}
+F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, I8, I32 = 0, 1, 2, 8, 12, 14, 24, 26
+TYPE_SIZE = {F32: 4, F16: 2, Q4_0: 18, Q8_0: 34, Q4_K: 144, Q6_K: 210, I8: 1, I32: 4}
+BLOCK_SIZE = {F32: 1, F16: 1, Q4_0: 32, Q8_0: 32, Q4_K: 256, Q6_K: 256, I8: 1, I32: 1}
 
 EUNSUPPORTED, EINVAL, ENOSPACE, ETIMEOUT = -1, -2, -3, -4
 
@@ -44,6 +44,11 @@ class PagedBatch(C.Structure):
     """spy_hip_paged_batch"""
     _fields_ = [("n_seq", C.c_int32), ("max_new", C.c_int32), ("max_kv", C.c_int32), ("row_start", C.c_void_p), ("kv_len", C.c_void_p),
                 ("pages", C.c_void_p), ("page_stride", C.c_int64)]
+
+
+class PagedPrefix(C.Structure):
+    """spy_hip_paged_prefix"""
+    _fields_ = [("n_group", C.c_int32), ("max_rows", C.c_int32), ("max_prefix", C.c_int32), ("seq_start", C.c_void_p), ("length", C.c_void_p)]
 
 
 class LlamaLayer(C.Structure):
@@ -118,6 +123,11 @@ SIGNATURES = {
     "spy_hip_paged_append": (_i32, [_vp, _TP, _TP, _TP, C.POINTER(PagedBatch), C.POINTER(RopeParam), _TP, _TP, _TP]),
     "spy_hip_paged_attention_scratch_size": (_sz, [_TP, _TP, C.POINTER(PagedBatch)]),
     "spy_hip_paged_attention": (_i32, [_vp, _TP, _TP, _TP, _TP, C.POINTER(PagedBatch), _f32, _i32, _i32, _vp, _sz]),
+    "spy_hip_paged_append_q8": (_i32, [_vp, _TP, _TP, _TP, C.POINTER(PagedBatch), C.POINTER(RopeParam), _TP, _TP, _TP, _TP, _TP]),
+    "spy_hip_paged_attention_q8_scratch_size": (_sz, [_TP, _TP, C.POINTER(PagedBatch)]),
+    "spy_hip_paged_attention_q8": (_i32, [_vp, _TP, _TP, _TP, _TP, _TP, _TP, C.POINTER(PagedBatch), _f32, _i32, _i32, _vp, _sz]),
+    "spy_hip_paged_attention_shared_scratch_size": (_sz, [_TP, _TP, C.POINTER(PagedBatch), C.POINTER(PagedPrefix)]),
+    "spy_hip_paged_attention_shared": (_i32, [_vp, _TP, _TP, _TP, _TP, _TP, _TP, C.POINTER(PagedBatch), C.POINTER(PagedPrefix), _f32, _vp, _sz]),
     "spy_hip_quantize_q8_0": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64]),
     "spy_hip_quantize_f16": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64]),
     "spy_hip_gemv_q8_0act": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64]),

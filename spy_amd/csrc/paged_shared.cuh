@@ -1,0 +1,40 @@
+// Attention of sequences that begin alike: what a group of them has in common is attended to by all its rows together, the rest by each sequence.
+//
+// For a row, whose keys are those in common, C, and its sequence's own, S: out = (sum over C and S of e^(x_j - m) V_j) / (sum over C and S of e^(x_j - m)).  Both sums are taken in pieces, each
+// with an m of its own, by the kernels of paged_attn.cuh: C with the group as one sequence whose new tokens are all its sequences' and which sees all of C, S from the first position on
+// that is not in common.  A second launch scales the pieces' (o, l) to the largest m and adds them up.
+// What is gained: K and V of C are read once for a group, in tiles of up to 128 rows of the matrix instructions, instead of once for each sequence, which has few.
+#include "paged_attn.cuh"
+
+template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_shared_few_kernel(attn_more a) {
+    __shared__ few_shared<D, 4> sh;
+    const int block = blockIdx.x;
+    const bool common = block < a.common.few_blocks;
+    attn_few<D, F32OUT, 4, MODE>(a, sh, common ? block : block - a.common.few_blocks, common);
+}
+// What takes longest first: chunks over the keys in common, and over a sequence's own, then tiles of few rows
+template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256 * chunk_groups(D)) void attn_shared_mixed_kernel(attn_more a) {
+    __shared__ union { few_shared<D, 4 * chunk_groups(D)> few; std::conditional_t<MODE & ATTN_Q8, chunk_shared_q8<D>, chunk_shared<D>> chunk; } sh;
+    int block = blockIdx.x;
+    if (block < a.common.chunk_blocks + a.chunk_blocks) {
+        const bool common = block < a.common.chunk_blocks;
+        attn_chunk<D, F32OUT, MODE>(a, sh.chunk, common ? block : block - a.common.chunk_blocks, common);
+        return;
+    }
+    block -= a.common.chunk_blocks + a.chunk_blocks;
+    const bool common = block < a.common.few_blocks;
+    attn_few<D, F32OUT, 4 * chunk_groups(D), MODE>(a, sh.few, common ? block : block - a.common.few_blocks, common);
+}
+
+template <int D, bool F32OUT, int MODE> static int attn_shared_launch(const attn_more &a, hipStream_t st) {
+    const unsigned few = a.common.few_blocks + a.few_blocks, chunk = a.common.chunk_blocks + a.chunk_blocks;
+    if (chunk) attn_shared_mixed_kernel<D, F32OUT, MODE><<<dim3(chunk + few), dim3(256 * chunk_groups(D)), 0, st>>>(a);
+    else attn_shared_few_kernel<D, F32OUT, MODE><<<dim3(few), dim3(256), 0, st>>>(a);
+    return SPY_LAUNCH_RC();
+}
+template <int MODE> static int attn_shared_launch(const attn_more &a, int64_t hd, bool f32, hipStream_t st) {
+    if (hd == 64) return f32 ? attn_shared_launch<64, true, MODE>(a, st) : attn_shared_launch<64, false, MODE>(a, st);
+    if (hd == 128) return f32 ? attn_shared_launch<128, true, MODE>(a, st) : attn_shared_launch<128, false, MODE>(a, st);
+    return f32 ? attn_shared_launch<256, true, MODE>(a, st) : attn_shared_launch<256, false, MODE>(a, st);
+}
+int spy_attn_shared_q8(const attn_more &a, int64_t hd, bool f32, hipStream_t st);        // paged_shared_q8.hip

@@ -1,0 +1,137 @@
+// Attention of sequences that begin alike: the plan of a call, and the launch that adds up its pieces (the first launch: paged_shared.cuh).
+#include "paged_shared.cuh"
+
+// A row and head of the output: D / 4 lanes, the heads of a wave of one row
+template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_shared_join_kernel(attn_more a, int waves) {
+    constexpr int L = D / 4, HEADS = 64 / L;                               // lanes to a head, heads to a wave
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63, n_head = a.G * a.group;
+    const int row = wave / waves, h = (wave - row * waves) * HEADS + lane / L, at = lane % L, hq = min(h, n_head - 1);
+    if (row >= a.b.n_row) return;
+    int row1, kv;
+    const int s = row_sequence(a.b, row, lane, row1, kv);
+    if (s < 0) return;
+    pg_span all;
+    const pg_span sq = pg_own(a.b, a.groups, s, nullptr, &all);
+    if (!sq.ok || row < sq.row0) return;
+    // pieces of the keys in common, and of the row's own: as the first launch shares them out
+    const auto pieces_of = [&](const row_tile &rt, bool few, int few_split, int chunk_split) {
+        const int n_tile = few ? (rt.end() - (rt.lo_any() & ~31) + 31) >> 5 : (rt.end() - (rt.lo_any() & ~63) + 63) >> 6, split = few ? few_split : chunk_split;
+        return n_tile > 0 ? (n_tile + split - 1) / split : 0;
+    };
+    int n_common = 0;
+    if (all.ok) {
+        const bool few = all.n_new * a.group <= a.few;
+        n_common = pieces_of(row_tile(a, all, 0, few ? 16 : CHUNK_ROWS, true), few, a.common.few_split, a.common.chunk_split);
+    }
+    const bool few = sq.n_new * a.group <= a.few;
+    const int r = (row - sq.row0) * a.group + hq % a.group;
+    const int n = n_common + pieces_of(row_tile(a, sq, few ? 0 : r / CHUNK_ROWS, few ? 16 : CHUNK_ROWS, false), few, a.few_split, a.chunk_split);
+    const int64_t first = ((int64_t)row * n_head + hq) * a.slots;
+    const auto slot = [&](int p) { return first + (p < n_common ? p : a.own_slot + p - n_common); };
+    // (heads of a wave may have different numbers of pieces: loops end for all of them together)
+    float top = -INFINITY, sum = 0.0f;
+    for (int p = at; __any(p < n); p += L) if (p < n) top = fmaxf(top, a.part_ml[2 * slot(p)]);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, SPY_WAVE));
+    const float base = top == -INFINITY ? 0.0f : top;
+    v4f v = {0, 0, 0, 0};
+    for (int p0 = 0; __any(p0 < n); p0 += L) {
+        float w = 0.0f;
+        if (p0 + at < n) {
+            const float2 ml = *(const float2 *)(a.part_ml + 2 * slot(p0 + at));
+            w = above_0(exp2_(ml.x - base));                               // (infinities stay: what is not above 2^-126 of a larger part adds nothing)
+            sum += w * ml.y;
+        }
+        for (int j = 0; j < L && __any(p0 + j < n); j++) {
+            const float wj = __shfl(w, lane - at + j, SPY_WAVE);
+            if (p0 + j < n) v += wj * *(const v4f *)(a.part_o + slot(p0 + j) * D + 4 * at);
+        }
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, SPY_WAVE);
+    if (h >= n_head) return;
+    const bool none = top == -INFINITY && sum == 0.0f;                     // sees no key
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = none ? 0.0f : v[k] / sum;
+    uint8_t *dst = a.out + (int64_t)row * a.o_t + (int64_t)hq * a.o_h;
+    if (F32OUT) *(v4f *)(dst + at * 16) = v;
+    else *(uint2 *)(dst + at * 8) = make_uint2(f2h(v[0]) | (uint32_t)f2h(v[1]) << 16, f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+}
+
+template <int D, bool F32OUT> static int attn_shared_join(const attn_more &a, hipStream_t st) {
+    const int heads = 256 / D, waves = (a.G * a.group + heads - 1) / heads;        // heads of a wave; waves of a row
+    attn_shared_join_kernel<D, F32OUT><<<dim3((unsigned)(((int64_t)a.b.n_row * waves + 3) / 4)), dim3(256), 0, st>>>(a, waves);
+    return SPY_LAUNCH_RC();
+}
+
+// Own keys as attn_make_plan shares them out; those in common the same way, with groups for sequences.
+struct shared_plan { attn_plan own, common; int64_t slots, own_slot; size_t ml_bytes, scratch; };
+static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *b, const spy_hip_paged_prefix *x, shared_plan &p) {
+    SPY_CHECK_ARG(q && k_pages && q->ne[1] > 0 && q->ne[1] <= 65535 && q->ne[2] > 0 && q->ne[2] < (1 << 28));
+    int rc = pg_check_batch(b);
+    if (!rc) rc = k_pages->type == SPY_HIP_I8 ? pg_check_pages_q8(k_pages, 1) : pg_check_pages(k_pages, 1);
+    if (rc) return rc;
+    SPY_CHECK_ARG(x && x->n_group > 0 && x->n_group <= (1 << 20) && x->max_rows > 0 && x->max_rows <= (1 << 28) && x->max_prefix > 0 && x->max_prefix <= (1 << 30));
+    SPY_CHECK_ARG(x->seq_start && x->length && (((uintptr_t)x->seq_start | (uintptr_t)x->length) & 3) == 0);
+    const int64_t G = k_pages->ne[2], H = q->ne[1], hd = k_pages->ne[0], n_row = q->ne[2];
+    SPY_CHECK_ARG(G <= 65535 && H % G == 0);
+    const int64_t group = H / G, cu = spy_num_cu();
+    const auto share = [&](attn_plan &a, int64_t n, int64_t rows, int64_t keys) {
+        const int64_t most = (rows < n_row ? rows : n_row) * group, tiles = ((keys + 31) / 32 + 1);
+        a.few = FEW_ROWS;
+        a.few_units = n * G;
+        attn_share(a.few_units, tiles, 6 * cu, 8, a.few_split, a.few_pieces);
+        a.chunk_tiles = a.chunk_units = 0; a.chunk_split = a.chunk_pieces = 1;
+        if (most <= FEW_ROWS) return;
+        const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = n_row * group / CHUNK_ROWS + n;
+        a.chunk_tiles = each * n < all ? each * n : all;
+        a.chunk_units = a.chunk_tiles * G;
+        attn_share(a.chunk_units, (keys + 63) / 64 + 1, cu, 8, a.chunk_split, a.chunk_pieces);
+    };
+    share(p.own, b->n_seq, b->max_new, b->max_kv);
+    share(p.common, x->n_group, x->max_rows, x->max_prefix);
+    const auto most = [](int64_t u, int64_t v) { return u > v ? u : v; };
+    p.own_slot = most(p.common.few_pieces, p.common.chunk_pieces);
+    p.slots = p.own_slot + most(p.own.few_pieces, p.own.chunk_pieces);
+    const auto threads = [&](int64_t blocks) { return blocks * 256 * chunk_groups((int)hd) < (1ll << 32); };
+    SPY_CHECK_ARG(threads(p.own.few_units * p.own.few_pieces + p.own.chunk_units * p.own.chunk_pieces + p.common.few_units * p.common.few_pieces + p.common.chunk_units * p.common.chunk_pieces));
+    SPY_CHECK_ARG(n_row * (H + 3) * hd / 4 < (1ll << 32) && n_row * H < (1ll << 31));          // ... and of the second
+    p.ml_bytes = ((size_t)(n_row * H * p.slots) * 8 + 255) / 256 * 256;
+    p.scratch = p.ml_bytes + (size_t)(n_row * H * p.slots * hd) * 4;
+    return 0;
+}
+
+extern "C" size_t spy_hip_paged_attention_shared_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix) {
+    shared_plan p;
+    return attn_make_shared_plan(q, k_pages, batch, prefix, p) ? 0 : p.scratch;
+}
+
+extern "C" int spy_hip_paged_attention_shared(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *k_scales, const spy_hip_tensor *v_pages,
+                                              const spy_hip_tensor *v_scales, const spy_hip_tensor *out, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix, float scale, void *scratch,
+                                              size_t scratch_bytes) {
+    SPY_CHECK_ARG(q && k_pages && v_pages && out);
+    SPY_CHECK_ARG((k_pages->type == SPY_HIP_I8) == (k_scales != nullptr) && (k_scales != nullptr) == (v_scales != nullptr));
+    shared_plan p;
+    attn_more a = {};
+    int rc = attn_make_shared_plan(q, k_pages, batch, prefix, p);
+    if (!rc) rc = attn_check(q, k_pages, k_scales, v_pages, v_scales, out, batch, scale, 1, 0, p.scratch, scratch, scratch_bytes, a);
+    if (rc) return rc;
+    attn_use_plan(p.own, nullptr, a);
+    attn_use_scales(k_scales, v_scales, a);
+    a.few_part = a.chunk_part = nullptr;
+    a.groups.seq_start = prefix->seq_start; a.groups.length = prefix->length;
+    a.groups.n_group = prefix->n_group; a.groups.max_rows = prefix->max_rows; a.groups.max_common = prefix->max_prefix;
+    a.common.few_split = (int)p.common.few_split; a.common.few_pieces = (int)p.common.few_pieces; a.common.few_blocks = (int)(p.common.few_units * p.common.few_pieces);
+    a.common.chunk_tiles = (int)p.common.chunk_tiles; a.common.chunk_split = (int)p.common.chunk_split; a.common.chunk_pieces = (int)p.common.chunk_pieces;
+    a.common.chunk_blocks = (int)(p.common.chunk_units * p.common.chunk_pieces);
+    a.part_ml = (float *)scratch; a.part_o = (float *)((uint8_t *)scratch + p.ml_bytes);
+    a.slots = (int)p.slots; a.own_slot = (int)p.own_slot;
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t hd = k_pages->ne[0];
+    const bool f32 = out->type == SPY_HIP_F32;
+    rc = k_scales ? spy_attn_shared_q8(a, hd, f32, st) : attn_shared_launch<ATTN_SHARED>(a, hd, f32, st);
+    if (rc) return rc;
+    if (hd == 64) return f32 ? attn_shared_join<64, true>(a, st) : attn_shared_join<64, false>(a, st);
+    if (hd == 128) return f32 ? attn_shared_join<128, true>(a, st) : attn_shared_join<128, false>(a, st);
+    return f32 ? attn_shared_join<256, true>(a, st) : attn_shared_join<256, false>(a, st);
+}
