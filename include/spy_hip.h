@@ -207,6 +207,26 @@ typedef struct spy_hip_sample_param {
 } spy_hip_sample_param;
 size_t spy_hip_sample_scratch_size(const spy_hip_tensor *logits);
 int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sample_param *param, int32_t *tokens, float *probs, void *scratch, size_t scratch_bytes);
+/* Verification of drafted tokens -- for hosts that let something cheaper propose tokens (a small model, a lookup) and run the model once over all of them.  Row i of a request is the model's
+ * logits before its i-th drafted token, the row behind the last drafted one those for the token after.  With p_i and q_i the distributions that spy_hip_sample draws from -- of the row's logits with
+ * `param`, and of draft_logits with draft_param --
+ *   drafted token d_i is taken where accept_i * q_i(d_i) < p_i(d_i) and all before it are;
+ *   for the first that is not, a token is drawn from max(p_i - q_i, 0) (from p_i where that leaves nothing), for the row behind the last one, if all are taken, from p_i: in order of
+ *   index, the first at which the running sum exceeds uniform_i * (sum of all).
+ * The tokens that come out are then distributed as if each had been drawn by spy_hip_sample from the model's own rows.
+ * logits, param: as for spy_hip_sample.  draft_logits: the same shape (a request's last row is not read); NULL: a draft is certain, q_i(d_i) = 1.  draft_param: NULL: temperature 1, nothing cut;
+ * its uniform is not looked at.  A drafted token outside the vocabulary is not taken.
+ * drafted: n_row int32, device (a request's last entry is not read); row_start: n_seq + 1 int32, device, ascending: rows row_start[s] .. row_start[s+1] - 1 are request s (none: left alone; one: nothing
+ * drafted, a token is drawn); accept: n_row floats, device, numbers in [0, 1) as uniform.
+ * tokens: n_row int32, device: the taken ones, the one drawn, -1 behind it (may be the memory of `drafted`); accepted: n_seq int32, device: how many are taken; probs: n_row floats or NULL: p_i of
+ * the row's token, 0 where there is none.  A row without a logit above -inf: p is 0 everywhere, and its token -1.  A request whose rows are not among the logits' raises the flag of spy_hip_take_error
+ * and is left alone.
+ * p and q are off by what spy_hip_sample's weights are, p - q by 2^-60 more.  n_row below 2^21 (2^22 without draft_logits).  scratch: spy_hip_sample_verify_scratch_size bytes, 256-byte aligned, this
+ * call's alone until the stream has passed it. */
+size_t spy_hip_sample_verify_scratch_size(const spy_hip_tensor *logits, int32_t n_seq);
+int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits, const spy_hip_sample_param *param, const spy_hip_tensor *draft_logits, const spy_hip_sample_param *draft_param,
+                          const int32_t *drafted, const int32_t *row_start, int32_t n_seq, const float *accept, int32_t *tokens, int32_t *accepted, float *probs, void *scratch,
+                          size_t scratch_bytes);
 
 /* ---- a batch of sequences over a cache in pages: no counterpart in the reference, whose caches hold one sequence
  *      (attention.cpp:180-265).  K pages are {hd, page_size, n_kv_head, n_page} and V^T pages {page_size, hd, n_kv_head, n_page}, F16, nb[0] = 2, the other

@@ -120,6 +120,8 @@ SIGNATURES = {
     "spy_hip_argmax": (_i32, [_vp, _vp, _i64, _vp]),
     "spy_hip_sample_scratch_size": (_sz, [_TP]),
     "spy_hip_sample": (_i32, [_vp, _TP, C.POINTER(SampleParam), _vp, _vp, _vp, _sz]),
+    "spy_hip_sample_verify_scratch_size": (_sz, [_TP, _i32]),
+    "spy_hip_sample_verify": (_i32, [_vp, _TP, C.POINTER(SampleParam), _TP, C.POINTER(SampleParam), _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _sz]),
     "spy_hip_paged_append": (_i32, [_vp, _TP, _TP, _TP, C.POINTER(PagedBatch), C.POINTER(RopeParam), _TP, _TP, _TP]),
     "spy_hip_paged_attention_scratch_size": (_sz, [_TP, _TP, C.POINTER(PagedBatch)]),
     "spy_hip_paged_attention": (_i32, [_vp, _TP, _TP, _TP, _TP, C.POINTER(PagedBatch), _f32, _i32, _i32, _vp, _sz]),

@@ -128,3 +128,31 @@ def test_shared_batches_that_no_launch_can_hold(n_row, seqs, groups, new):
 def test_append_of_more_rows_than_threads(n_row, new):
     a = {n: rows(16, n_row=n_row, at=(i + 1) << 44) for i, n in enumerate(("q", "k", "v", "qo"))}
     assert append(**a, kp=q8("k", G=16), ks=scales("k", G=16), vp=q8("v", G=16), vs=scales("v", G=16), b=batch(n_seq=1, max_new=new)) == H.EINVAL
+
+
+def verify(t=H.F32, n=1000, n_row=5, at=4096, nb=None, uniform=4096, param=True, draft=True, drafted=4096, row_start=4096, n_seq=2, accept=4096, tokens=4096, accepted=4096, probs=None, scratch=4096,
+           room=1 << 30, draft_param=True, **kw):
+    l = H.tensor(at, t, [n, n_row], nb)
+    d = H.tensor(kw.get("draft_at", 8192), kw.get("draft_t", H.F32), [kw.get("draft_n", n), kw.get("draft_row", n_row)])
+    p = H.SampleParam(uniform=uniform, top_p=kw.get("top_p"))
+    q = H.SampleParam(top_p=kw.get("draft_top_p"))
+    return H.load().spy_hip_sample_verify(None, B(l), B(p) if param else None, B(d) if draft else None, B(q) if draft_param else None, drafted, row_start, n_seq, accept, tokens, accepted, probs, scratch,
+                                          room)
+
+
+@pytest.mark.parametrize("kw", [dict(n=0), dict(n_row=0), dict(n=(1 << 18) + 1), dict(at=0), dict(at=4097), dict(nb=[8, 8000]), dict(nb=[4, 4002]), dict(uniform=None), dict(uniform=4098), dict(param=False),
+                                dict(drafted=None), dict(drafted=4097), dict(row_start=None), dict(row_start=4098), dict(n_seq=0), dict(n_seq=-1), dict(n_seq=(1 << 20) + 1), dict(accept=None),
+                                dict(accept=4099), dict(tokens=None), dict(tokens=4097), dict(accepted=None), dict(accepted=4098), dict(probs=4097), dict(scratch=None), dict(scratch=4112),
+                                dict(draft_at=0), dict(draft_at=8194), dict(draft_n=999), dict(draft_row=6), dict(draft_top_p=4098), dict(top_p=4097), dict(n_row=1 << 21), dict(n_row=1 << 22, draft=False)])
+def test_verify_refuses(kw):
+    assert verify(**kw) == H.EINVAL
+
+
+def test_verify_types_and_scratch():
+    assert verify(t=H.F16) == H.EUNSUPPORTED
+    assert verify(draft_t=H.F16) == H.EUNSUPPORTED
+    L = H.load()
+    need = L.spy_hip_sample_verify_scratch_size(B(H.tensor(4096, H.F32, [1000, 5])), 2)
+    assert need > 0
+    assert verify(room=need - 1) == H.ENOSPACE
+    assert L.spy_hip_sample_verify_scratch_size(None, 2) == 0
