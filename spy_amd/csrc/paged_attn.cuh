@@ -160,6 +160,45 @@ static __device__ __forceinline__ float larger(float top, float x) { return __bu
 // A factor from one m to another that leaves infinities infinite: what is not above 2^-126 of a larger part adds nothing to it, as with 0
 static __device__ __forceinline__ float above_0(float f) { return fmaxf(f, 0x1p-126f); }
 
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes per lane from memory to LDS, in lane order from byte `lds` (uniform) on; base uniform, or an address per lane.  Written as instructions so that the compiler does
+// not wait for them at the next LDS read; landed() does.
+// A base that a vector instruction has written may be read five instructions later: the compiler does not look into these.
+// `there` 0: not requested.  (The branch is written out as well: as one of the compiler's it would part the instructions on either side into blocks of their own.)
+static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds, uint32_t there) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\ts_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, %2\n.Lno%=:" :: "s"(lds), "v"(off), "s"(base), "s"(there) : "memory", "m0", "scc");
+}
+static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds, uint32_t there) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, off\n.Lno%=:" :: "s"(lds), "v"(addr), "s"(there) : "memory", "m0", "scc");
+}
+#pragma clang diagnostic pop
+static __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const uint8_t *)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
+}
+static __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+// Arguments are loaded sixteen registers at a time; where they live through the loop over the keys, the compiler runs out of scalar registers, keeps whole groups of
+// sixteen in lanes of a vector register and moves all of one back for each value it needs: 158 of 378 vector instructions per tile.  So the loop's values are scalars
+// of their own, and what is wanted after it is loaded again then (from the kernel's arguments, of which this struct is the first).
+template <class Args> static __device__ __forceinline__ const __attribute__((address_space(4))) Args *args_again() {
+    const __attribute__((address_space(4))) Args *p = (const __attribute__((address_space(4))) Args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+static __device__ __forceinline__ uint32_t alone(uint32_t v) {
+    uint32_t r;
+    asm volatile("s_mov_b32 %0, %1" : "=s"(r) : "s"(uniform(v)));
+    return r;
+}
+static __device__ __forceinline__ int alone(int v) { return (int)alone((uint32_t)v); }
+template <class T> static __device__ __forceinline__ T *alone(T *p) {
+    const uint8_t *r;
+    asm volatile("s_mov_b64 %0, %1" : "=s"(r) : "s"(uniform((const uint8_t *)p)));
+    return (T *)r;
+}
+static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ---- 16 rows per workgroup: single tokens, and a few of them -------------------------------------------------------------------------
 // A row is a new token and one of the query heads that share the K/V head: with a group of heads, or several new tokens, the keys are read once for all of them.
 // Bound by the bytes of K and V.  The waves take tiles of 32 keys in turn, straight from memory into the registers of the matrix instruction: nothing is shared
@@ -170,194 +209,12 @@ template <int D, int WAVES> struct few_shared {
     float m[WAVES][16], l[WAVES][16];
     __attribute__((aligned(16))) float o[WAVES][16][HALF + 4];
 };
-// MODE: see above.  common: the block is one of the keys that the sequences of a group have in common (the groups stand for sequences then)
-template <int D, bool F32OUT, int WAVES, int MODE = ATTN_PLAIN> static __device__ __forceinline__ void attn_few(const attn_args_of<MODE> &a, few_shared<D, WAVES> &sh, int block, bool common = false) {
-    constexpr bool Q8 = MODE & ATTN_Q8, SHARED = MODE & ATTN_SHARED;
-    constexpr int ES = Q8 ? 1 : 2;                                         // bytes of an element in the pages
-    constexpr int KS = D / 32, DT = D / 16, HALF = few_shared<D, WAVES>::HALF;
+// The waves' (m, l, o) to one: the output, or (o, m, l) of the piece
+template <int D, bool F32OUT, int WAVES, int MODE, class Seq> static __device__ __forceinline__ void few_end(const attn_args_of<MODE> &a, few_shared<D, WAVES> &sh, const Seq &sq, int rows, int head, int unit,
+                                                                                                             int piece, bool whole, bool common, float m, float l, v4f (&o)[D / 16]) {
+    constexpr bool SHARED = MODE & ATTN_SHARED;
+    constexpr int HALF = few_shared<D, WAVES>::HALF;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quarter = lane >> 4;
-    int n_unit = a.b.n_seq, split = a.few_split;
-    if constexpr (SHARED) if (common) { n_unit = a.groups.n_group; split = a.common.few_split; }
-    const int units = n_unit * a.G, piece = block / units, unit = block - piece * units, which = unit / a.G, head = unit - which * a.G;
-    const auto sq = [&] {
-        if constexpr (SHARED) return pg_span_of(a.b, a.groups, which, common, a.err);
-        else return pg_sequence(a.b, which, a.err);
-    }();
-    if (!sq.ok) return;
-    const row_tile rt = [&] {
-        if constexpr (SHARED) return row_tile(a, sq, 0, 16, common);
-        else return row_tile(a, sq, 0, 16);
-    }();
-    int s = which;                                                         // whose pages
-    if constexpr (SHARED) s = sq.s;
-    if (rt.rows > a.few) return;
-    const int rows = rt.rows, r = min(n, rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
-    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all(), begin = rt.lo_any() & ~31, end = rt.end();
-    const int n_tile = max((end - begin + 31) >> 5, 0);
-    if ((SHARED || piece > 0) && piece * split >= n_tile) return;
-    const int stop = min((piece + 1) * split, n_tile);
-    const bool whole = !SHARED && n_tile <= split;
-
-    const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
-    v8h fq[KS];
-#pragma unroll
-    for (int k = 0; k < KS; k++) fq[k] = halves(*(const uint4 *)(qrow + (32 * k + 8 * quarter) * 2));
-    const int32_t *table = a.b.pages + (int64_t)s * a.b.page_stride;
-    const int plog = a.b.page_log2, pmask = (1 << plog) - 1, last = (sq.kv - 1) >> plog;
-
-    // Instruction row i of score tile t is key 8 (i / 4) + 4 t + i % 4: a lane's scores are then of keys 8 quarter + 4 t + 0 .. 3, as the product wants them.
-    const uint8_t *kbase = a.kp + (int64_t)head * a.kp_h + (int64_t)(n & 3) * a.kp_p + quarter * 8 * ES, *vbase = a.vp + (int64_t)head * a.vp_h + (int64_t)n * a.vp_d;
-    struct page_pair { int first, second; };                               // of the tile's two groups of 16 keys
-    const auto pages_of = [&](int kt) {
-        const int kb = begin + 32 * min(kt, stop - 1);
-        return page_pair{pg_entry(table, min(kb >> plog, last)), pg_entry(table, min((kb + 16) >> plog, last))};
-    };
-    const auto missing = [&](int page) { return (uint32_t)page >= (uint32_t)a.b.n_page; };
-    const auto place = [&](page_pair g, int q, int64_t step) {             // keys 8 q ..: their page
-        const int page = q & 2 ? g.second : g.first;
-        return (int64_t)(missing(page) ? 0 : page) * step;
-    };
-    typedef std::conditional_t<Q8, uint2, uint4> piece8;                   // eight elements as the pages have them
-    piece8 fk[2][KS], fv[DT];
-    typedef uint32_t k_scales __attribute__((ext_vector_type(KS / 2)));    // of a key: one to a block of 32 elements, which is a step of the scores
-    k_scales dk[2];
-    uint4 dv[D / 32];                                                      // of eight keys, for a block of 32 dimensions
-    const auto load_k = [&](int kt, page_pair g) {
-        const uint8_t *kr = kbase + place(g, n >> 2, a.kp_g) + (int64_t)((begin + 32 * kt + 8 * (n >> 2)) & pmask) * a.kp_p;
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int k = 0; k < KS; k++) fk[t][k] = *(const piece8 *)(kr + 4 * t * a.kp_p + k * 32 * ES);
-        if constexpr (Q8) {
-            const uint8_t *ksr = a.ks + (int64_t)head * a.ks_h + place(g, n >> 2, a.ks_g) + ((begin + 32 * kt + 8 * (n >> 2) & pmask) + (n & 3)) * (D / 16);
-#pragma unroll
-            for (int t = 0; t < 2; t++) dk[t] = *(const k_scales *)(ksr + 4 * t * (D / 16));
-        }
-    };
-    const auto v_row = [&](int kt, page_pair g) { return vbase + place(g, quarter, a.vp_g) + (int64_t)((begin + 32 * kt + 8 * quarter) & pmask) * ES; };
-    const auto v_scales = [&](int kt, page_pair g) {                       // (nothing to look at in pages of fp16)
-        if constexpr (Q8) return a.vs + (int64_t)head * a.vs_h + place(g, quarter, a.vs_g) + (int64_t)((begin + 32 * kt + 8 * quarter) & pmask) * 2;
-        else return (const uint8_t *)nullptr;
-    };
-    const auto load_v = [&](int kt, page_pair g) {
-        const uint8_t *vr = v_row(kt, g), *vsr = v_scales(kt, g);
-#pragma unroll
-        for (int d = 0; d < DT; d++) fv[d] = *(const piece8 *)(vr + 16 * d * a.vp_d);
-        if constexpr (Q8) {
-#pragma unroll
-            for (int d = 0; d < D / 32; d++) dv[d] = *(const uint4 *)(vsr + d * a.vs_b);
-        }
-    };
-    const auto k_piece = [&](int t, int k) {
-        if constexpr (Q8) return dequantized(fk[t][k], all_of(dk[t][k / 2] >> (16 * (k & 1))));
-        else return halves(fk[t][k]);
-    };
-    const auto v_piece = [&](int d) {
-        if constexpr (Q8) return bits(dequantized(fv[d], halves(dv[d / 2])));
-        else return fv[d];
-    };
-
-    float m = -INFINITY, l = 0.0f;
-    v4f o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
-    bool unbounded = false;
-    // K of the next tile is requested when this one's scores are done with the registers, V^T when the product is: memory always has a tile of each wave to fetch
-    const int first = piece * split + wave;
-    page_pair pg = {0, 0}, pg1 = {0, 0};
-    if (first < stop) {
-        pg = pages_of(first);
-        pg1 = pages_of(first + WAVES);
-        load_k(first, pg);
-        load_v(first, pg);
-    }
-    for (int kt = first; kt < stop; kt += WAVES) {
-        const page_pair pg2 = pages_of(kt + 2 * WAVES);
-        const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
-        const bool vbad = missing(quarter & 2 ? pg.second : pg.first);
-        v4f x[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            x[t] = v4f{0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < KS; k++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_piece(t, k), fq[k], x[t], 0, 0, 0);
-        }
-        if (kt + WAVES < stop) load_k(kt + WAVES, pg1);
-        float e[8];                                                        // of this lane's query and keys vk ..
-#pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
-        const bool masked = __any(kb + 32 > hi_all || kb < lo_all || vbad);
-        const int there = vbad ? 0 : end - vk;                             // positions of this lane's eight that the cache has, for this tile's rows
-        if (masked) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = vk + j >= lo && vk + j < hi && !vbad ? e[j] : -INFINITY;
-            if (vbad && vk < end && vk + 8 > rt.lo_any() && a.err) *a.err = 1;     // (a page before the window may be gone)
-            // what lies behind the cache's last position is taken as 0, and so are infinities and NaN, which some rows may see and others not
-            if constexpr (!Q8) {
-#pragma unroll
-                for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), unbounded);
-            }
-        }
-        float top = e[0];
-#pragma unroll
-        for (int j = 1; j < 8; j++) top = fmaxf(top, e[j]);
-        top = quad_reduce(top, [](float p, float q) { return fmaxf(p, q); });
-        top = fmaxf(m, top - (fabsf(top) < 1e7f ? 15.0f : 7.0f));
-        const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_(m - base);
-        m = top;
-        float sum = 0.0f;
-        v8h p, p2;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            e[j] = exp2_(e[j] - base);
-            sum += e[j];
-            p[j] = (_Float16)e[j];
-            p2[j] = (_Float16)(e[j] - (float)p[j]);                        // (for F16 outputs as well: the second product takes no time beside the keys' arrival)
-        }
-        l = l * shrink + sum;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            uint4 w = v_piece(d);
-            if (Q8 && masked) w = bounded(first_of(w, there), unbounded);
-            o[d] *= shrink;
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w), p, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w), p2, o[d], 0, 0, 0);
-        }
-        if (kt + WAVES < stop) load_v(kt + WAVES, pg1);
-        pg = pg1; pg1 = pg2;
-    }
-    float most = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) most = larger(most, o[d][i]);
-    if (__any(unbounded || !finite(most))) {
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[d][i] = finite(o[d][i]) ? o[d][i] : 0.0f;       // (of a row with a score of NaN or +inf: l is NaN)
-#pragma nounroll
-            for (int kind = 0; kind < 3; kind++) {
-                v4f n_seen = {0, 0, 0, 0};
-#pragma nounroll
-                for (int kt = first; kt < stop; kt += WAVES) {
-                    const page_pair g = pages_of(kt);
-                    const int vk = begin + 32 * kt + 8 * quarter;
-                    const bool vbad = missing(quarter & 2 ? g.second : g.first);
-                    uint4 w;
-                    if constexpr (Q8) w = bits(dequantized(*(const uint2 *)(v_row(kt, g) + 16 * d * a.vp_d), halves(*(const uint4 *)(v_scales(kt, g) + d / 2 * a.vs_b))));
-                    else w = *(const uint4 *)(v_row(kt, g) + 16 * d * a.vp_d);
-                    w = first_of(w, vbad ? 0 : end - vk);
-                    uint32_t seen = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
-                    n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), ones(seen), n_seen, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
-            }
-        }
-    }
     l = quad_reduce(l, [](float p, float q) { return p + q; });
     if (quarter == 0) { sh.m[wave][n] = m; sh.l[wave][n] = l; }
     __syncthreads();
@@ -407,6 +264,163 @@ template <int D, bool F32OUT, int WAVES, int MODE = ATTN_PLAIN> static __device_
     }
 }
 
+// MODE: see above.  common: the block is one of the keys that the sequences of a group have in common (the groups stand for sequences then)
+template <int D, bool F32OUT, int WAVES, int MODE = ATTN_PLAIN> static __device__ __forceinline__ void attn_few(const attn_args_of<MODE> &a, few_shared<D, WAVES> &sh, int block, bool common = false) {
+    constexpr bool SHARED = MODE & ATTN_SHARED;
+    constexpr int KS = D / 32, DT = D / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quarter = lane >> 4;
+    int n_unit = a.b.n_seq, split = a.few_split;
+    if constexpr (SHARED) if (common) { n_unit = a.groups.n_group; split = a.common.few_split; }
+    const int units = n_unit * a.G, piece = block / units, unit = block - piece * units, which = unit / a.G, head = unit - which * a.G;
+    const auto sq = [&] {
+        if constexpr (SHARED) return pg_span_of(a.b, a.groups, which, common, a.err);
+        else return pg_sequence(a.b, which, a.err);
+    }();
+    if (!sq.ok) return;
+    const row_tile rt = [&] {
+        if constexpr (SHARED) return row_tile(a, sq, 0, 16, common);
+        else return row_tile(a, sq, 0, 16);
+    }();
+    int s = which;                                                         // whose pages
+    if constexpr (SHARED) s = sq.s;
+    if (rt.rows > a.few) return;
+    const int rows = rt.rows, r = min(n, rows - 1), token = r / a.group, hq = head * a.group + (r - token * a.group);
+    const int hi = rt.hi(token), lo = rt.lo(token), hi_all = rt.hi_all(), lo_all = rt.lo_all(), begin = rt.lo_any() & ~31, end = rt.end();
+    const int n_tile = max((end - begin + 31) >> 5, 0);
+    if ((SHARED || piece > 0) && piece * split >= n_tile) return;
+    const int stop = min((piece + 1) * split, n_tile);
+    const bool whole = !SHARED && n_tile <= split;
+
+    const uint8_t *qrow = a.q + (int64_t)(sq.row0 + token) * a.q_t + (int64_t)hq * a.q_h;
+    v8h fq[KS];
+#pragma unroll
+    for (int k = 0; k < KS; k++) fq[k] = halves(*(const uint4 *)(qrow + (32 * k + 8 * quarter) * 2));
+    const int32_t *table = a.b.pages + (int64_t)s * a.b.page_stride;
+    const int plog = a.b.page_log2, pmask = (1 << plog) - 1, last = (sq.kv - 1) >> plog;
+
+    // Instruction row i of score tile t is key 8 (i / 4) + 4 t + i % 4: a lane's scores are then of keys 8 quarter + 4 t + 0 .. 3, as the product wants them.
+    const uint8_t *kbase = a.kp + (int64_t)head * a.kp_h + (int64_t)(n & 3) * a.kp_p + quarter * 16, *vbase = a.vp + (int64_t)head * a.vp_h + (int64_t)n * a.vp_d;
+    struct page_pair { int first, second; };                               // of the tile's two groups of 16 keys
+    const auto pages_of = [&](int kt) {
+        const int kb = begin + 32 * min(kt, stop - 1);
+        return page_pair{pg_entry(table, min(kb >> plog, last)), pg_entry(table, min((kb + 16) >> plog, last))};
+    };
+    const auto missing = [&](int page) { return (uint32_t)page >= (uint32_t)a.b.n_page; };
+    const auto place = [&](page_pair g, int q, int64_t step) {             // keys 8 q ..: their page
+        const int page = q & 2 ? g.second : g.first;
+        return (int64_t)(missing(page) ? 0 : page) * step;
+    };
+    uint4 fk[2][KS], fv[DT];
+    const auto load_k = [&](int kt, page_pair g) {
+        const uint8_t *kr = kbase + place(g, n >> 2, a.kp_g) + (int64_t)((begin + 32 * kt + 8 * (n >> 2)) & pmask) * a.kp_p;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) fk[t][k] = *(const uint4 *)(kr + 4 * t * a.kp_p + k * 64);
+    };
+    const auto v_row = [&](int kt, page_pair g) { return vbase + place(g, quarter, a.vp_g) + (int64_t)((begin + 32 * kt + 8 * quarter) & pmask) * 2; };
+    const auto load_v = [&](const uint8_t *vr) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) fv[d] = *(const uint4 *)(vr + 16 * d * a.vp_d);
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    v4f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
+    bool unbounded = false;
+    // K of the next tile is requested when this one's scores are done with the registers, V^T when the product is: memory always has a tile of each wave to fetch
+    const int first = piece * split + wave;
+    page_pair pg = {0, 0}, pg1 = {0, 0};
+    if (first < stop) {
+        pg = pages_of(first);
+        pg1 = pages_of(first + WAVES);
+        load_k(first, pg);
+        load_v(v_row(first, pg));
+    }
+    for (int kt = first; kt < stop; kt += WAVES) {
+        const page_pair pg2 = pages_of(kt + 2 * WAVES);
+        const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
+        const bool vbad = missing(quarter & 2 ? pg.second : pg.first);
+        v4f x[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            x[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; k++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fk[t][k]), fq[k], x[t], 0, 0, 0);
+        }
+        if (kt + WAVES < stop) load_k(kt + WAVES, pg1);
+        float e[8];                                                        // of this lane's query and keys vk ..
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * a.c;
+        const bool masked = __any(kb + 32 > hi_all || kb < lo_all || vbad);
+        const int there = vbad ? 0 : end - vk;                             // positions of this lane's eight that the cache has, for this tile's rows
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = vk + j >= lo && vk + j < hi && !vbad ? e[j] : -INFINITY;
+            if (vbad && vk < end && vk + 8 > rt.lo_any() && a.err) *a.err = 1;     // (a page before the window may be gone)
+            // what lies behind the cache's last position is taken as 0, and so are infinities and NaN, which some rows may see and others not
+#pragma unroll
+            for (int d = 0; d < DT; d++) fv[d] = bounded(first_of(fv[d], there), unbounded);
+        }
+        float top = e[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) top = fmaxf(top, e[j]);
+        top = quad_reduce(top, [](float p, float q) { return fmaxf(p, q); });
+        top = fmaxf(m, top - (fabsf(top) < 1e7f ? 15.0f : 7.0f));
+        const float base = top == -INFINITY ? 0.0f : top, shrink = exp2_(m - base);
+        m = top;
+        float sum = 0.0f;
+        v8h p, p2;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            e[j] = exp2_(e[j] - base);
+            sum += e[j];
+            p[j] = (_Float16)e[j];
+            p2[j] = (_Float16)(e[j] - (float)p[j]);                        // (for F16 outputs as well: the second product takes no time beside the keys' arrival)
+        }
+        l = l * shrink + sum;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            o[d] *= shrink;
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fv[d]), p, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(fv[d]), p2, o[d], 0, 0, 0);
+        }
+        if (kt + WAVES < stop) load_v(v_row(kt + WAVES, pg1));
+        pg = pg1; pg1 = pg2;
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = larger(most, o[d][i]);
+    if (__any(unbounded || !finite(most))) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[d][i] = finite(o[d][i]) ? o[d][i] : 0.0f;       // (of a row with a score of NaN or +inf: l is NaN)
+#pragma nounroll
+            for (int kind = 0; kind < 3; kind++) {
+                v4f n_seen = {0, 0, 0, 0};
+#pragma nounroll
+                for (int kt = first; kt < stop; kt += WAVES) {
+                    const page_pair g = pages_of(kt);
+                    const int vk = begin + 32 * kt + 8 * quarter;
+                    const bool vbad = missing(quarter & 2 ? g.second : g.first);
+                    const uint4 w = first_of(*(const uint4 *)(v_row(kt, g) + 16 * d * a.vp_d), vbad ? 0 : end - vk);
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) seen |= (uint32_t)(vk + j >= lo && vk + j < hi && !vbad) << j;
+                    n_seen = __builtin_amdgcn_mfma_f32_16x16x32_f16(of_kind(w, kind), ones(seen), n_seen, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (n_seen[i] != 0.0f) o[d][i] += kind_value(kind);
+            }
+        }
+    }
+    few_end<D, F32OUT, WAVES, MODE>(a, sh, sq, rows, head, unit, piece, whole, common, m, l, o);
+}
+
 // ---- CHUNK_ROWS rows per workgroup: chunks of a prompt --------------------------------------------------------------------------------
 // Bound by the matrix cores and the vector instructions of the softmax together: 64 keys by 32 rows take a wave (D = 128) 32 matrix instructions of 33 cycles, and some 200
 // vector instructions of 4.7, 32 of them exponentials of 11; two waves of a SIMD need 4400 of the 5200 cycles that a step takes, since the step's barrier puts both into
@@ -421,45 +435,6 @@ template <int D, bool F32OUT, int WAVES, int MODE = ATTN_PLAIN> static __device_
 // 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a lane's scores are those of 8 keys that follow each other, as the product wants its
 // probabilities); its 16-byte pieces are stored at their index xor a number of the row, so that the lanes of a read meet different banks.
 typedef float v16f __attribute__((ext_vector_type(16)));
-
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes per lane from memory to LDS, in lane order from byte `lds` (uniform) on; base uniform, or an address per lane.  Written as instructions so that the compiler does
-// not wait for them at the next LDS read; landed() does.
-// A base that a vector instruction has written may be read five instructions later: the compiler does not look into these.
-// `there` 0: not requested.  (The branch is written out as well: as one of the compiler's it would part the instructions on either side into blocks of their own.)
-static __device__ __forceinline__ void to_lds(const void *base, uint32_t off, uint32_t lds, uint32_t there) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\ts_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, %2\n.Lno%=:" :: "s"(lds), "v"(off), "s"(base), "s"(there) : "memory", "m0", "scc");
-}
-static __device__ __forceinline__ void to_lds(const void *addr, uint32_t lds, uint32_t there) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lno%=\n\tglobal_load_lds_dwordx4 %1, off\n.Lno%=:" :: "s"(lds), "v"(addr), "s"(there) : "memory", "m0", "scc");
-}
-#pragma clang diagnostic pop
-static __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
-    const uint64_t v = (uint64_t)p;
-    return (const uint8_t *)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
-}
-static __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-// Arguments are loaded sixteen registers at a time; where they live through the loop over the keys, the compiler runs out of scalar registers, keeps whole groups of
-// sixteen in lanes of a vector register and moves all of one back for each value it needs: 158 of 378 vector instructions per tile.  So the loop's values are scalars
-// of their own, and what is wanted after it is loaded again then (from the kernel's arguments, of which this struct is the first).
-template <class Args> static __device__ __forceinline__ const __attribute__((address_space(4))) Args *args_again() {
-    const __attribute__((address_space(4))) Args *p = (const __attribute__((address_space(4))) Args *)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    return p;
-}
-static __device__ __forceinline__ uint32_t alone(uint32_t v) {
-    uint32_t r;
-    asm volatile("s_mov_b32 %0, %1" : "=s"(r) : "s"(uniform(v)));
-    return r;
-}
-static __device__ __forceinline__ int alone(int v) { return (int)alone((uint32_t)v); }
-template <class T> static __device__ __forceinline__ T *alone(T *p) {
-    const uint8_t *r;
-    asm volatile("s_mov_b64 %0, %1" : "=s"(r) : "s"(uniform((const uint8_t *)p)));
-    return (T *)r;
-}
-static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <int D> static __device__ __forceinline__ int swizzle_k(int row) { return D == 64 ? (row >> 1 & 3) | (((row ^ row >> 3) & 1) << 2) : row & 15; }
 static __device__ __forceinline__ int swizzle_v(int row) { return (row >> 1 & 3) | (((row ^ row >> 3) & 1) << 2); }

@@ -1,14 +1,14 @@
 // Attention over pages of 8 bits: paged_attn.cuh with fp16(d * q) for the elements of K and V, so that its results are those of pages that hold these as fp16, bit for bit.
-#include "paged_attn.cuh"
+#include "paged_few_q8.cuh"
 
 template <int D, bool F32OUT> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_q8_few_kernel(attn_more a) {
-    __shared__ few_shared<D, 4> sh;
-    attn_few<D, F32OUT, 4, ATTN_Q8>(a, sh, blockIdx.x);
+    __shared__ few_q8_shared<D, 4> sh;
+    attn_few_q8<D, F32OUT, 4, ATTN_Q8>(a, sh, blockIdx.x);
 }
 template <int D, bool F32OUT> __global__ __launch_bounds__(256 * chunk_groups(D)) void attn_q8_mixed_kernel(attn_more a) {
-    __shared__ union { few_shared<D, 4 * chunk_groups(D)> few; chunk_shared_q8<D> chunk; } sh;
+    __shared__ union { few_q8_shared<D, 4 * chunk_groups(D)> few; chunk_shared_q8<D> chunk; } sh;
     if ((int)blockIdx.x < a.chunk_blocks) attn_chunk<D, F32OUT, ATTN_Q8>(a, sh.chunk, blockIdx.x);
-    else attn_few<D, F32OUT, 4 * chunk_groups(D), ATTN_Q8>(a, sh.few, blockIdx.x - a.chunk_blocks);
+    else attn_few_q8<D, F32OUT, 4 * chunk_groups(D), ATTN_Q8>(a, sh.few, blockIdx.x - a.chunk_blocks);
 }
 
 extern "C" size_t spy_hip_paged_attention_q8_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch) {

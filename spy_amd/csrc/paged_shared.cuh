@@ -4,17 +4,22 @@
 // with an m of its own, by the kernels of paged_attn.cuh: C with the group as one sequence whose new tokens are all its sequences' and which sees all of C, S from the first position on
 // that is not in common.  A second launch scales the pieces' (o, l) to the largest m and adds them up.
 // What is gained: K and V of C are read once for a group, in tiles of up to 128 rows of the matrix instructions, instead of once for each sequence, which has few.
-#include "paged_attn.cuh"
+#include "paged_few_q8.cuh"
 
+template <int D, int WAVES, int MODE> using shared_few = std::conditional_t<MODE & ATTN_Q8, few_q8_shared<D, WAVES>, few_shared<D, WAVES>>;
+template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinline__ void attn_shared_few(const attn_more &a, shared_few<D, WAVES, MODE> &sh, int block, bool common) {
+    if constexpr (MODE & ATTN_Q8) attn_few_q8<D, F32OUT, WAVES, MODE>(a, sh, block, common);
+    else attn_few<D, F32OUT, WAVES, MODE>(a, sh, block, common);
+}
 template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_shared_few_kernel(attn_more a) {
-    __shared__ few_shared<D, 4> sh;
+    __shared__ shared_few<D, 4, MODE> sh;
     const int block = blockIdx.x;
     const bool common = block < a.common.few_blocks;
-    attn_few<D, F32OUT, 4, MODE>(a, sh, common ? block : block - a.common.few_blocks, common);
+    attn_shared_few<D, F32OUT, 4, MODE>(a, sh, common ? block : block - a.common.few_blocks, common);
 }
 // What takes longest first: chunks over the keys in common, and over a sequence's own, then tiles of few rows
 template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256 * chunk_groups(D)) void attn_shared_mixed_kernel(attn_more a) {
-    __shared__ union { few_shared<D, 4 * chunk_groups(D)> few; std::conditional_t<MODE & ATTN_Q8, chunk_shared_q8<D>, chunk_shared<D>> chunk; } sh;
+    __shared__ union { shared_few<D, 4 * chunk_groups(D), MODE> few; std::conditional_t<MODE & ATTN_Q8, chunk_shared_q8<D>, chunk_shared<D>> chunk; } sh;
     int block = blockIdx.x;
     if (block < a.common.chunk_blocks + a.chunk_blocks) {
         const bool common = block < a.common.chunk_blocks;
@@ -23,7 +28,7 @@ template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256 * chunk
     }
     block -= a.common.chunk_blocks + a.chunk_blocks;
     const bool common = block < a.common.few_blocks;
-    attn_few<D, F32OUT, 4 * chunk_groups(D), MODE>(a, sh.few, common ? block : block - a.common.few_blocks, common);
+    attn_shared_few<D, F32OUT, 4 * chunk_groups(D), MODE>(a, sh.few, common ? block : block - a.common.few_blocks, common);
 }
 
 template <int D, bool F32OUT, int MODE> static int attn_shared_launch(const attn_more &a, hipStream_t st) {
