@@ -1,55 +1,78 @@
 // Attention of sequences that begin alike: the plan of a call, and the launch that adds up its pieces (the first launch: paged_shared.cuh).
 #include "paged_shared.cuh"
 
-// A row and head of the output: D / 4 lanes, the heads of a wave of one row
-template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_shared_join_kernel(attn_more a, int waves) {
-    constexpr int L = D / 4, HEADS = 64 / L;                               // lanes to a head, heads to a wave
-    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63, n_head = a.G * a.group;
-    const int row = wave / waves, h = (wave - row * waves) * HEADS + lane / L, at = lane % L, hq = min(h, n_head - 1);
-    if (row >= a.b.n_row) return;
-    int row1, kv;
-    const int s = row_sequence(a.b, row, lane, row1, kv);
-    if (s < 0) return;
-    pg_span all;
-    const pg_span sq = pg_own(a.b, a.groups, s, nullptr, &all);
-    if (!sq.ok || row < sq.row0) return;
-    // pieces of the keys in common, and of the row's own: as the first launch shares them out
-    const auto pieces_of = [&](const row_tile &rt, bool few, int few_split, int chunk_split) {
-        const int n_tile = few ? (rt.end() - (rt.lo_any() & ~31) + 31) >> 5 : (rt.end() - (rt.lo_any() & ~63) + 63) >> 6, split = few ? few_split : chunk_split;
-        return n_tile > 0 ? (n_tile + split - 1) / split : 0;
-    };
-    int n_common = 0;
-    if (all.ok) {
-        const bool few = all.n_new * a.group <= a.few;
-        n_common = pieces_of(row_tile(a, all, 0, few ? 16 : CHUNK_ROWS, true), few, a.common.few_split, a.common.chunk_split);
-    }
-    const bool few = sq.n_new * a.group <= a.few;
-    const int r = (row - sq.row0) * a.group + hq % a.group;
-    const int n = n_common + pieces_of(row_tile(a, sq, few ? 0 : r / CHUNK_ROWS, few ? 16 : CHUNK_ROWS, false), few, a.few_split, a.chunk_split);
-    const int64_t first = ((int64_t)row * n_head + hq) * a.slots;
-    const auto slot = [&](int p) { return first + (p < n_common ? p : a.own_slot + p - n_common); };
+// A row and head of the output: D / 4 lanes, the heads of a wave of one row.  PARTS: so many waves of the workgroup share the pieces of the same heads.  Latency, and what the first launch wrote:
+// eight pieces of o are requested at a time, the first before the weights are worked out.
+template <int D, bool F32OUT, int PARTS> __global__ __launch_bounds__(256) void attn_shared_join_kernel(attn_more a, int waves) {
+    constexpr int L = D / 4, HEADS = 64 / L, AHEAD = PARTS > 1 ? 8 : 2;                    // lanes to a head, heads to a wave
+    __shared__ v4f s_v[4][64];
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % PARTS, wave = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) / PARTS), lane = threadIdx.x & 63;
+    const int n_head = a.G * a.group, row = wave / waves, h = (wave - row * waves) * HEADS + lane / L, at = lane % L, hq = min(h, n_head - 1);
+    int n_common = 0, n = 0;
+    if (row < a.b.n_row) {
+        int row1, kv;
+        const int s = row_sequence(a.b, row, lane, row1, kv);
+        if (s >= 0) {
+            pg_span all;
+            const pg_span sq = pg_own(a.b, a.groups, s, nullptr, &all);
+            // pieces of the keys in common, and of the row's own: as the first launch shares them out
+            const auto pieces_of = [&](const row_tile &rt, bool few, int few_split, int chunk_split) {
+                const int n_tile = few ? (rt.end() - (rt.lo_any() & ~31) + 31) >> 5 : (rt.end() - (rt.lo_any() & ~63) + 63) >> 6, split = few ? few_split : chunk_split;
+                return n_tile > 0 ? (n_tile + split - 1) / split : 0;
+            };
+            if (sq.ok && row >= sq.row0) {
+                if (all.ok) {
+                    const bool few = all.n_new * a.group <= a.few;
+                    n_common = pieces_of(row_tile(a, all, 0, few ? 16 : CHUNK_ROWS, true), few, a.common.few_split, a.common.chunk_split);
+                }
+                const bool few = sq.n_new * a.group <= a.few;
+                const int r = (row - sq.row0) * a.group + hq % a.group;
+                n = n_common + pieces_of(row_tile(a, sq, few ? 0 : r / CHUNK_ROWS, few ? 16 : CHUNK_ROWS, false), few, a.few_split, a.chunk_split);
+            } else n = -1;
+        } else n = -1;
+    } else n = -1;                                                         // left alone
+    const int64_t first = ((int64_t)min(row, a.b.n_row - 1) * n_head + hq) * a.slots;
+    const auto slot = [&](int p) { p = max(min(p, n - 1), 0); return first + (p < n_common ? p : a.own_slot + p - n_common); };
+    const auto piece = [&](int i) { return part + PARTS * i; };            // the wave's i-th
     // (heads of a wave may have different numbers of pieces: loops end for all of them together)
-    float top = -INFINITY, sum = 0.0f;
-    for (int p = at; __any(p < n); p += L) if (p < n) top = fmaxf(top, a.part_ml[2 * slot(p)]);
+    v4f x[AHEAD];
+    const auto request = [&](int i) {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, SPY_WAVE));
-    const float base = top == -INFINITY ? 0.0f : top;
+        for (int j = 0; j < AHEAD; j++) if (piece(i + j) < n) x[j] = *(const v4f *)(a.part_o + slot(piece(i + j)) * D + 4 * at);
+    };
     v4f v = {0, 0, 0, 0};
-    for (int p0 = 0; __any(p0 < n); p0 += L) {
-        float w = 0.0f;
-        if (p0 + at < n) {
-            const float2 ml = *(const float2 *)(a.part_ml + 2 * slot(p0 + at));
-            w = above_0(exp2_(ml.x - base));                               // (infinities stay: what is not above 2^-126 of a larger part adds nothing)
-            sum += w * ml.y;
-        }
-        for (int j = 0; j < L && __any(p0 + j < n); j++) {
-            const float wj = __shfl(w, lane - at + j, SPY_WAVE);
-            if (p0 + j < n) v += wj * *(const v4f *)(a.part_o + slot(p0 + j) * D + 4 * at);
-        }
-    }
+    float top = -INFINITY, sum = 0.0f;
+    if (__any(n > 0)) {
+        float2 ml = *(const float2 *)(a.part_ml + 2 * slot(at));
+        request(0);
+        for (int p = at; __any(p < n); p += L) if (p < n) top = fmaxf(top, p == at ? ml.x : a.part_ml[2 * slot(p)]);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, SPY_WAVE);
-    if (h >= n_head) return;
+        for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, SPY_WAVE));
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int p0 = 0; __any(p0 < n); p0 += L) {                         // pieces p0 .. p0 + L - 1, a lane the weight of one
+            if (p0) ml = *(const float2 *)(a.part_ml + 2 * slot(p0 + at));
+            const float w = p0 + at < n ? above_0(exp2_(ml.x - base)) : 0.0f;      // (infinities stay: what is not above 2^-126 of a larger part adds nothing)
+            sum += p0 + at < n ? w * ml.y : 0.0f;
+            for (int i = p0 / PARTS; i < (p0 + L) / PARTS && __any(piece(i) < n); i += AHEAD) {
+                if (i) request(i);
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++) {
+                    const float wj = __shfl(w, lane - at + (piece(i + j) - p0) % L, SPY_WAVE);
+                    if (piece(i + j) < n) v += wj * x[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, SPY_WAVE);
+    }
+    if constexpr (PARTS > 1) {
+        s_v[threadIdx.x >> 6][lane] = v;
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int p = 1; p < PARTS; p++) v += s_v[(threadIdx.x >> 6) + p][lane];
+    }
+    if (h >= n_head || n < 0) return;
     const bool none = top == -INFINITY && sum == 0.0f;                     // sees no key
 #pragma unroll
     for (int k = 0; k < 4; k++) v[k] = none ? 0.0f : v[k] / sum;
@@ -60,7 +83,11 @@ template <int D, bool F32OUT> __global__ __launch_bounds__(256) void attn_shared
 
 template <int D, bool F32OUT> static int attn_shared_join(const attn_more &a, hipStream_t st) {
     const int heads = 256 / D, waves = (a.G * a.group + heads - 1) / heads;        // heads of a wave; waves of a row
-    attn_shared_join_kernel<D, F32OUT><<<dim3((unsigned)(((int64_t)a.b.n_row * waves + 3) / 4)), dim3(256), 0, st>>>(a, waves);
+    const int64_t all = (int64_t)a.b.n_row * waves;
+    // Pieces that a row may be expected to have: those of chunks where the batch may bring them.  32 rows of 32 heads with 30 pieces each 14.5 us by a wave, XX by four; 965 rows with two 16 and 42.
+    const int pieces = (a.common.chunk_blocks ? a.common.chunk_pieces : a.common.few_pieces) + (a.chunk_blocks ? a.chunk_pieces : a.few_pieces);
+    if (pieces > 8 && all <= 4096) attn_shared_join_kernel<D, F32OUT, 4><<<dim3((unsigned)all), dim3(256), 0, st>>>(a, waves);
+    else attn_shared_join_kernel<D, F32OUT, 1><<<dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st>>>(a, waves);
     return SPY_LAUNCH_RC();
 }
 
@@ -95,7 +122,7 @@ static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *
     p.slots = p.own_slot + most(p.own.few_pieces, p.own.chunk_pieces);
     const auto threads = [&](int64_t blocks) { return blocks * 256 * chunk_groups((int)hd) < (1ll << 32); };
     SPY_CHECK_ARG(threads(p.own.few_units * p.own.few_pieces + p.own.chunk_units * p.own.chunk_pieces + p.common.few_units * p.common.few_pieces + p.common.chunk_units * p.common.chunk_pieces));
-    SPY_CHECK_ARG(n_row * (H + 3) * hd / 4 < (1ll << 32) && n_row * H < (1ll << 31));          // ... and of the second
+    SPY_CHECK_ARG(n_row * (H + 3) * hd < (1ll << 32) && n_row * H < (1ll << 31));              // ... and of the second
     p.ml_bytes = ((size_t)(n_row * H * p.slots) * 8 + 255) / 256 * 256;
     p.scratch = p.ml_bytes + (size_t)(n_row * H * p.slots * hd) * 4;
     return 0;
