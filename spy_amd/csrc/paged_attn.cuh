@@ -502,15 +502,15 @@ static __device__ __forceinline__ bool find_span(const attn_more &a, bool common
 
 static constexpr __host__ __device__ int chunk_groups(int D) { return D == 256 ? 1 : 2; }
 template <int D> struct chunk_group { __attribute__((aligned(1024))) uint8_t k[2][64 * D * 2], v[2][64 * D * 2]; };
-template <int D> struct chunk_shared { chunk_group<D> group[chunk_groups(D)]; int unbounded; };
-template <int D> struct chunk_shared_q8 : chunk_shared<D> { __attribute__((aligned(16))) uint8_t scales[4 * chunk_groups(D)][D * 4]; };      // of V^T, a wave's own copy
+template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared { chunk_group<D> group[GROUPS]; int unbounded; };
+template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared_q8 : chunk_shared<D, GROUPS> { __attribute__((aligned(16))) uint8_t scales[4 * GROUPS][D * 4]; };      // of V^T, a wave's own copy
 
 // Q8: a tile's whole numbers are in registers while the tile before is computed with, and go to LDS as fp16 values.
-template <int D, bool F32OUT, int MODE = ATTN_PLAIN, class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false) {
+template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D), class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false) {
     constexpr bool Q8 = MODE & ATTN_Q8, SHARED = MODE & ATTN_SHARED;
     constexpr int ES = Q8 ? 1 : 2;                                         // bytes of an element in the pages
     constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
-    constexpr int KC = D / 8, KR = 64 / KC, GROUPS = chunk_groups(D);      // 16-byte pieces of a K row, K rows per request
+    constexpr int KC = D / 8, KR = 64 / KC;                                // 16-byte pieces of a K row, K rows per request
     static_assert(2 * KS == 4 * NI && 4 * DT == 4 * NI);                   // a request beside every fourth product, and every fourth step of the second product
     const int tid = threadIdx.x, lane = tid & 63, wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3, group = wave8 >> 2, n = lane & 31, half = lane >> 5;
     chunk_group<D> &sh = shared.group[group];
@@ -844,7 +844,7 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, class Shared = chunk_shared
     constexpr int HAVE = DT / GROUPS;                                      // output tiles that this wave has in the end, from `d0` on
     const int d0 = group * HAVE;
     if constexpr (GROUPS == 2) {                                           // each group takes one half of the output from the other
-        static_assert(sizeof(chunk_shared<D>) >= 8 * (16 * HAVE + 2) * 256);
+        static_assert(sizeof(chunk_shared<D, GROUPS>) >= 8 * (16 * HAVE + 2) * 256);
         const auto share = [&](int g) { return (float *)&shared + (4 * g + wave) * (16 * HAVE + 2) * 64 + lane; };
         float *const give = share(group);
         const float *const take = share(1 - group);

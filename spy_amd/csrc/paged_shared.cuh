@@ -18,22 +18,22 @@ template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 2
     attn_shared_few<D, F32OUT, 4, MODE>(a, sh, common ? block : block - a.common.few_blocks, common);
 }
 // What takes longest first: chunks over the keys in common, and over a sequence's own, then tiles of few rows
-template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256 * chunk_groups(D)) void attn_shared_mixed_kernel(attn_more a) {
-    __shared__ union { shared_few<D, 4 * chunk_groups(D), MODE> few; std::conditional_t<MODE & ATTN_Q8, chunk_shared_q8<D>, chunk_shared<D>> chunk; } sh;
+template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_shared_mixed_kernel(attn_more a) {
+    __shared__ union { shared_few<D, 4, MODE> few; std::conditional_t<MODE & ATTN_Q8, chunk_shared_q8<D, 1>, chunk_shared<D, 1>> chunk; } sh;
     int block = blockIdx.x;
     if (block < a.common.chunk_blocks + a.chunk_blocks) {
         const bool common = block < a.common.chunk_blocks;
-        attn_chunk<D, F32OUT, MODE>(a, sh.chunk, common ? block : block - a.common.chunk_blocks, common);
+        attn_chunk<D, F32OUT, MODE, 1>(a, sh.chunk, common ? block : block - a.common.chunk_blocks, common);
         return;
     }
     block -= a.common.chunk_blocks + a.chunk_blocks;
     const bool common = block < a.common.few_blocks;
-    attn_shared_few<D, F32OUT, 4 * chunk_groups(D), MODE>(a, sh.few, common ? block : block - a.common.few_blocks, common);
+    attn_shared_few<D, F32OUT, 4, MODE>(a, sh.few, common ? block : block - a.common.few_blocks, common);
 }
 
 template <int D, bool F32OUT, int MODE> static int attn_shared_launch(const attn_more &a, hipStream_t st) {
     const unsigned few = a.common.few_blocks + a.few_blocks, chunk = a.common.chunk_blocks + a.chunk_blocks;
-    if (chunk) attn_shared_mixed_kernel<D, F32OUT, MODE><<<dim3(chunk + few), dim3(256 * chunk_groups(D)), 0, st>>>(a);
+    if (chunk) attn_shared_mixed_kernel<D, F32OUT, MODE><<<dim3(chunk + few), dim3(256), 0, st>>>(a);
     else attn_shared_few_kernel<D, F32OUT, MODE><<<dim3(few), dim3(256), 0, st>>>(a);
     return SPY_LAUNCH_RC();
 }

@@ -92,6 +92,7 @@ template <int D, bool F32OUT> static int attn_shared_join(const attn_more &a, hi
 }
 
 // Own keys as attn_make_plan shares them out; those in common the same way, with groups for sequences.
+#define CW 4
 struct shared_plan { attn_plan own, common; int64_t slots, own_slot; size_t ml_bytes, scratch; };
 static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *b, const spy_hip_paged_prefix *x, shared_plan &p) {
     SPY_CHECK_ARG(q && k_pages && q->ne[1] > 0 && q->ne[1] <= 65535 && q->ne[2] > 0 && q->ne[2] < (1 << 28));
@@ -103,24 +104,27 @@ static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *
     const int64_t G = k_pages->ne[2], H = q->ne[1], hd = k_pages->ne[0], n_row = q->ne[2];
     SPY_CHECK_ARG(G <= 65535 && H % G == 0);
     const int64_t group = H / G, cu = spy_num_cu();
-    const auto share = [&](attn_plan &a, int64_t n, int64_t rows, int64_t keys) {
+    const auto share = [&](attn_plan &a, int64_t count, int64_t rows, int64_t keys) {
         const int64_t most = (rows < n_row ? rows : n_row) * group, tiles = ((keys + 31) / 32 + 1);
         a.few = FEW_ROWS;
-        a.few_units = n * G;
-        attn_share(a.few_units, tiles, 6 * cu, 8, a.few_split, a.few_pieces);
+        a.few_units = count * G;
+        attn_share(a.few_units, tiles, 3 * cu, 8, a.few_split, a.few_pieces);
         a.chunk_tiles = a.chunk_units = 0; a.chunk_split = a.chunk_pieces = 1;
         if (most <= FEW_ROWS) return;
-        const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = n_row * group / CHUNK_ROWS + n;
-        a.chunk_tiles = each * n < all ? each * n : all;
+        const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = n_row * group / CHUNK_ROWS + count;
+        a.chunk_tiles = each * count < all ? each * count : all;
         a.chunk_units = a.chunk_tiles * G;
-        attn_share(a.chunk_units, (keys + 63) / 64 + 1, cu, 8, a.chunk_split, a.chunk_pieces);
+        const int64_t key_tiles = (keys + 63) / 64 + (&a == &p.own), n = (CW * cu / 4 + a.chunk_units - 1) / a.chunk_units;
+        a.chunk_split = n == 1 ? key_tiles : (key_tiles + n - 1) / n;
+        if (a.chunk_split < 8) a.chunk_split = 8;
+        a.chunk_pieces = (key_tiles + a.chunk_split - 1) / a.chunk_split;
     };
     share(p.own, b->n_seq, b->max_new, b->max_kv);
     share(p.common, x->n_group, x->max_rows, x->max_prefix);
     const auto most = [](int64_t u, int64_t v) { return u > v ? u : v; };
     p.own_slot = most(p.common.few_pieces, p.common.chunk_pieces);
     p.slots = p.own_slot + most(p.own.few_pieces, p.own.chunk_pieces);
-    const auto threads = [&](int64_t blocks) { return blocks * 256 * chunk_groups((int)hd) < (1ll << 32); };
+    const auto threads = [&](int64_t blocks) { return blocks * 256 < (1ll << 32); };
     SPY_CHECK_ARG(threads(p.own.few_units * p.own.few_pieces + p.own.chunk_units * p.own.chunk_pieces + p.common.few_units * p.common.few_pieces + p.common.chunk_units * p.common.chunk_pieces));
     SPY_CHECK_ARG(n_row * (H + 3) * hd < (1ll << 32) && n_row * H < (1ll << 31));              // ... and of the second
     p.ml_bytes = ((size_t)(n_row * H * p.slots) * 8 + 255) / 256 * 256;
