@@ -24,6 +24,7 @@
 #define SM_FAST 512            // largest top_k that is looked for among the threads' maxima: twice as many fill the list (64 rows of 32000, by the maxima and by the histogram: top_k 40 11.0 and 26.4 us, 512 18.5 and 27.5)
 #define SM_BITS 44             // weights: multiples of 2^-44; 2^18 of them fit 64 bits
 #define SM_VOCAB (1 << 18)
+#define SM_KEPT 1024           // tokens that a cut keeps a list of
 #define SM_HELD 2048           // logits of a wave's part of the row that lie in LDS
 
 typedef unsigned long long u64;
@@ -233,7 +234,8 @@ static __device__ __forceinline__ u64 draw_at(float u, u64 total) {             
 }
 
 // What a row's settings leave: the tokens up to rank word `last`, their weights added up (0: no token at all), and the weight of one token of interest (0: not left).  top: the largest logit
-struct sample_cut { u64 last, total, weight; float top; uint32_t infinite; };      // (infinite: as sample_row has it)
+// n_kept: so many tokens are left, and their rank words are kept in any order; ~0: not known, nor kept (more than SM_KEPT are never kept).
+struct sample_cut { u64 last, total, weight; float top; uint32_t infinite, n_kept; };      // (infinite: as sample_row has it)
 struct no_cut {};
 
 // The draw from a list of up to 128 tokens that has all that top_k leaves, by one wave: two tokens a lane, ranked by comparing each with all.  Done: a function that is given what
@@ -261,7 +263,7 @@ template <class Done> static __device__ __forceinline__ void draw_from_few(const
     }
     keep = min(keep, number(lane < m && x0 <= last, q < m && x1 <= last));
     const u64 total = upto(keep - 1), want = draw_at(u, total);
-    if constexpr (!std::is_same_v<Done, no_cut>) { done(s.x[keep - 1], total); return; }
+    if constexpr (!std::is_same_v<Done, no_cut>) { done(s.x[keep - 1], total, keep); return; }
     // in order of index: the first with a running sum that reaches `want`
     u64 sum0 = 0, sum1 = 0;
     for (uint32_t j = 0; j < keep; j++) {
@@ -362,8 +364,8 @@ template <class Weight, class Drawn> static __device__ __forceinline__ void draw
 }
 
 
-// Row r by a workgroup: a token drawn, or -- CUT -- what its settings leave, and the weight of token `d` there, to *cut
-template <bool CUT> static __device__ __forceinline__ void sample_row_of(const sample_args &a, uint8_t *smem, int r, int d, sample_cut *cut) {
+// Row r by a workgroup: a token drawn, or -- CUT -- what its settings leave, and the weight of token `d` there, to *cut; the tokens left to `kept`, if not null, as far as they have room
+template <bool CUT> static __device__ __forceinline__ void sample_row_of(const sample_args &a, uint8_t *smem, int r, int d, sample_cut *cut, u64 *kept) {
     sample_shared &s = *(sample_shared *)smem;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     sample_row row;
@@ -386,7 +388,7 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
     __syncthreads();
     for (int w = 0; w < 16; w++) { top = fmaxf(top, s.wave_f[w]); low = fminf(low, s.wave_g[w]); }
     if (top == -INFINITY) {
-        if constexpr (CUT) { if (t == 0) *cut = {0, 0, 0, 0.0f, 0}; }
+        if constexpr (CUT) { if (t == 0) *cut = {0, 0, 0, 0.0f, 0, 0}; }
         else if (t == 0) { a.tokens[r] = -1; if (a.probs) a.probs[r] = 0.0f; }
         return;
     }
@@ -405,14 +407,18 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             if (own == top) atomicMin(&s.bin, first);
         }
         __syncthreads();
-        if constexpr (CUT) { if (t == 0) *cut = {(u64)order_word(top) << 32 | (uint32_t)s.bin, 1ull << SM_BITS, d == s.bin ? 1ull << SM_BITS : 0, top, row.infinite}; }
+        if constexpr (CUT) {
+            const u64 x = (u64)order_word(top) << 32 | (uint32_t)s.bin;
+            if (t == 0) *cut = {x, 1ull << SM_BITS, d == s.bin ? 1ull << SM_BITS : 0, top, row.infinite, 1};
+            if (t == 0 && kept) kept[0] = x;
+        }
         else if (t == 0) { a.tokens[r] = s.bin; if (a.probs) a.probs[r] = 1.0f; }
         return;
     }
     const weigher weigh = weigher_of(temp, top);
-    const auto left = [&](u64 last, u64 total) {                                  // by one thread
+    const auto left = [&](u64 last, u64 total, uint32_t n_kept) {                 // by one thread
         const float l = (uint32_t)d < (uint32_t)a.n ? row.clean(f4{row.g[d], 0.0f, 0.0f, 0.0f})[0] : -INFINITY;
-        *cut = {last, total, l > -INFINITY && rank_word(l, d) <= last ? weigh(l) : 0, top, row.infinite};
+        *cut = {last, total, l > -INFINITY && rank_word(l, d) <= last ? weigh(l) : 0, top, row.infinite, n_kept};
     };
     const bool by_rank = k > 0 && k < a.n, by_mass = p < 1.0f;
     u64 last = ~0ull;                                                             // rank word of the last token kept
@@ -445,7 +451,10 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
         __syncthreads();
         const uint32_t m = s.n_list;
         if (m <= 128) {
-            if constexpr (CUT) { if (wave == 0) draw_from_few(a, s, r, m, k, by_mass, p, last, u, [&](u64 x, u64 total) { if (lane == 0) left(x, total); }); }
+            if constexpr (CUT) { if (wave == 0) draw_from_few(a, s, r, m, k, by_mass, p, last, u, [&](u64 x, u64 total, uint32_t n) {
+                if (lane == 0) left(x, total, n);
+                if (kept) for (uint32_t i = lane; i < n; i += 64) kept[i] = s.x[i];
+            }); }
             else if (wave == 0) draw_from_few(a, s, r, m, k, by_mass, p, last, u, no_cut());
             return;
         }
@@ -460,7 +469,11 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             if ((uint32_t)t < keep && s.x[t] <= last && ((uint32_t)t + 1 == keep || s.x[t + 1] > last)) s.pick_count = t + 1;
             __syncthreads();
             keep = s.pick_count;
-            if constexpr (CUT) { if (t == 0) left(s.x[keep - 1], s.mass[keep - 1]); return; }
+            if constexpr (CUT) {
+                if (t == 0) left(s.x[keep - 1], s.mass[keep - 1], keep);
+                if (kept && (uint32_t)t < keep) kept[t] = s.x[t];
+                return;
+            }
             const u64 total = s.mass[keep - 1], want = draw_at(u, total);
             const bool mine = (uint32_t)t < keep;
             const u64 x = mine ? s.x[t] : 0, w = mine ? s.w[t] : 0;
@@ -488,6 +501,7 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
         __syncthreads();
     }
     bool summed = false;                                                          // the kept weights of this wave's part are in s.part
+    u64 cut_total = 0;                                                            // (of a cut: the kept weights, where `summed`)
     const bool flat = weigh.c == 0.0f;                                            // an infinite temperature: -inf is not far away by itself
     if (by_rank || by_mass) {
         const float reach = (float)(SM_BINS - 1) / 32.0f;                         // distances from here on have one bin together
@@ -527,7 +541,20 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             const float last_l = last == ~0ull ? -INFINITY : logit_of(last);
             const int last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
             u64 sum = 0;
-            row.groups([&](f4 v, int i) {
+            if constexpr (CUT) {                                                  // (the weights before the bin are known)
+                row.groups([&](f4 v, int i) {
+                    bool there[4], any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = flat && !(v[e] > -INFINITY) ? INFINITY : weigh.far(v[e]);
+                        there[e] = (y >= near) & !(y >= upper) & (v[e] > -INFINITY);
+                        any |= there[e];
+                    }
+                    if (__any(any))
+#pragma unroll
+                        for (int e = 0; e < 4; e++) append(s, there[e], v[e], i + e, weigh);
+                });
+            } else row.groups([&](f4 v, int i) {
                 float y[4];
                 bool there[4], any = false;
 #pragma unroll
@@ -553,8 +580,10 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
                         for (int e = 0; e < 4; e++) sum += weigh.at(y[e]);
                 }
             });
-            sum = of_lane(wave_scan(sum), 63);
-            if (lane == 0) s.part[wave] = sum;
+            if constexpr (!CUT) {
+                sum = of_lane(wave_scan(sum), 63);
+                if (lane == 0) s.part[wave] = sum;
+            }
             __syncthreads();
             uint32_t m = s.n_list;
             __syncthreads();
@@ -569,8 +598,10 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             const uint32_t rank = which ? rank_of_mass(s, m, want) : (uint32_t)want - 1;
             const u64 x = s.x[rank];
             upto = before + s.mass[rank];
+            if (CUT && x <= last) { cut_total = upto; summed = true; }
             last = x < last ? x : last;
-            if (which && listed) {
+            if constexpr (CUT) {
+            } else if (which && listed) {
                 if ((uint32_t)t < m && s.x[t] <= last) atomicAdd(&s.part[(uint32_t)s.x[t] / (uint32_t)a.part], s.w[t]);
                 summed = true;
             }
@@ -581,8 +612,8 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
     const bool all_kept = last == ~0ull;
     const float last_l = all_kept ? -INFINITY : logit_of(last);
     const int last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
-    const auto kept = [&](float v, int i) { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); };
-    const auto weight = [&](float v, int i) { return weigh.at(kept(v, i) ? weigh.far(v) : INFINITY); };
+    const auto kept_by = [&](float v, int i) { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); };
+    const auto weight = [&](float v, int i) { return weigh.at(kept_by(v, i) ? weigh.far(v) : INFINITY); };
     if (!summed) {
         u64 sum = 0;
         if (all_kept && !flat) row.each([&](float v, int) { sum += weigh(v); });  // (-inf adds 0)
@@ -590,7 +621,7 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             row.groups([&](f4 v, int i) {
                 bool in[4], some = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++) { in[e] = kept(v[e], i + e); some |= in[e]; }
+                for (int e = 0; e < 4; e++) { in[e] = kept_by(v[e], i + e); some |= in[e]; }
                 if (!__any(some)) return;
 #pragma unroll
                 for (int e = 0; e < 4; e++) sum += weigh.at(in[e] ? weigh.far(v[e]) : INFINITY);
@@ -598,10 +629,10 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
         sum = of_lane(wave_scan(sum), 63);
         if (lane == 0) s.part[wave] = sum;
     }
-    __syncthreads();
+    if (!(CUT && summed)) __syncthreads();
     if constexpr (CUT) {
-        const u64 total = of_lane(row_scan(s.part[lane & 15]), 15);
-        if (t == 0) left(last, total);
+        if (!summed) cut_total = of_lane(row_scan(s.part[lane & 15]), 15);
+        if (t == 0) left(last, cut_total, ~0u);
         return;
     }
     draw_by_parts(a, s, row, held, u, weight, [&](int i, u64 w, u64 total) { a.tokens[r] = i; if (a.probs) a.probs[r] = (float)((double)w / (double)total); });

@@ -3,7 +3,7 @@
 
 __global__ __launch_bounds__(SM_THREADS) void sample_kernel(sample_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    sample_row_of<false>(a, smem, blockIdx.x, 0, nullptr);
+    sample_row_of<false>(a, smem, blockIdx.x, 0, nullptr, nullptr);
 }
 
 extern "C" size_t spy_hip_sample_scratch_size(const spy_hip_tensor *logits) {

@@ -18,6 +18,9 @@ struct verify_args {
     int32_t *tokens, *accepted;
     float *probs;
     sample_cut *cuts;                    // of the target's rows, then of the draft's
+    u64 *kept;                           // of the target's rows: SM_KEPT each
+    u64 *sums;                           // of the requests: VF_PARTS each
+    int32_t *stops;                      // of the requests: the row where its drafts end
     int *err;
 };
 
@@ -36,101 +39,214 @@ __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
     }
     if (row0 < 0 || r < row0 || row1 > a.n_row || (side && r == row1 - 1)) return;
     const int d = r < row1 - 1 ? a.drafted[r] : -1;
-    sample_row_of<true>(side ? a.draft : a.target, smem, r, d, a.cuts + side * (int64_t)a.n_row + r);
+    sample_row_of<true>(side ? a.draft : a.target, smem, r, d, a.cuts + side * (int64_t)a.n_row + r, side ? nullptr : a.kept + (int64_t)r * SM_KEPT);
 }
 
-__global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    sample_shared &s = *(sample_shared *)smem;
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), row0 = a.row_start[blockIdx.x], row1 = a.row_start[blockIdx.x + 1];
+// What settings leave of a row
+struct verify_left {
+    weigher weigh;
+    float last_l;
+    int last_i;
+    bool infinite;
+    __device__ __forceinline__ verify_left(const float *temperature, const sample_cut *c, int r) {
+        const float temp = temperature ? temperature[r] : 1.0f;
+        const u64 last = c->last;
+        weigh = weigher_of(temp > 0.0f ? temp : 1.0f, c->top);                    // (the only token left of a greedy row has the largest logit: any temperature)
+        last_l = last == ~0ull ? -INFINITY : logit_of(last);
+        last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
+        infinite = c->infinite;
+    }
+    __device__ __forceinline__ float clean(float v) const { return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v; }          // (a NaN is never left)
+    __device__ __forceinline__ bool has(float v, int i) const { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); }
+};
+static __device__ __forceinline__ double share_of_all(u64 w, u64 all) { return all ? (double)w / (double)all : 0.0; }
+static __device__ __forceinline__ double verify_p(const verify_args &a, int64_t r) { return share_of_all(a.cuts[r].weight, a.cuts[r].total); }
+
+// Weights of the tokens of row `stop`, where a request's drafts end: of p - q, or -- as_p -- of p
+struct verify_weights {
+    verify_left p, q;
+    const float *gp, *gq;
+    int n, drafted;
+    bool beyond_q, as_p;
+    double one_p, one_q;
+    __device__ __forceinline__ verify_weights(const verify_args &a, int stop, bool at_end)
+        : p(a.target.temperature, a.cuts + stop, stop), q(a.draft.temperature, a.cuts + (at_end || !a.draft.logits ? 0 : a.n_row) + stop, stop) {
+        beyond_q = !at_end && a.draft.logits;
+        as_p = at_end;
+        gp = (const float *)(a.target.logits + stop * a.target.stride);
+        gq = beyond_q ? (const float *)(a.draft.logits + stop * a.draft.stride) : gp;
+        n = a.target.n;
+        drafted = at_end ? -1 : a.drafted[stop];
+        one_p = 1.0 / (double)a.cuts[stop].total;
+        const u64 all_q = beyond_q ? a.cuts[(int64_t)a.n_row + stop].total : 0;
+        one_q = all_q ? 1.0 / (double)all_q : 0.0;
+    }
+    // of a token that p has, with the logits v (as p.clean() has it) and l
+    __device__ __forceinline__ u64 operator()(float v, float l, int i) const {
+        const u64 w = p.weigh(v);
+        if (as_p) return w;
+        if (!beyond_q) return i == drafted ? 0 : w;
+        l = q.clean(l);
+        const double more = (double)w * one_p - (q.has(l, i) ? (double)q.weigh(l) * one_q : 0.0);
+        return more > 0.0 ? (u64)(more * 0x1p60) : 0;
+    }
+    // By a wave: f(weight, token, its logit; 0, 0, 0 where there is none) for the tokens from .. to - 1 that p has, in order of index, a token a lane.  They are looked for first, 256 at a time, in `list`:
+    // a weight takes some hundred instructions, and few tokens of many have one.
+    template <class F> __device__ __forceinline__ void each(int from, int to, uint2 *list, F f) const {
+        const int lane = threadIdx.x & 63;
+        for (int base = from; base < to; base += 256) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = gp[min(base + 64 * j + lane, n - 1)];
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = base + 64 * j + lane;
+                const float v = p.clean(x[j]);
+                const unsigned long long who = __ballot(i < to && p.has(v, i));
+                if (i < to && p.has(v, i)) list[m + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = make_uint2((uint32_t)i, __float_as_uint(v));
+                m += (uint32_t)__popcll(who);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+            for (uint32_t k = 0; k < m; k += 64) {
+                const bool there = k + lane < m;
+                const uint2 e = there ? list[k + lane] : make_uint2(0, 0);
+                const float l = beyond_q && there ? gq[e.x] : 0.0f;
+                f(there ? (*this)(__uint_as_float(e.y), l, (int)e.x) : 0, (int)e.x, __uint_as_float(e.y));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    __device__ __forceinline__ u64 sum(int from, int to, uint2 *list) const {     // by a wave, to every lane
+        u64 all = 0;
+        each(from, to, list, [&](u64 w, int, float) { all += w; });
+        return of_lane(wave_scan(all), 63);
+    }
+};
+#define VF_PARTS 64
+static __device__ __forceinline__ void verify_part(int n, int part, int &from, int &to) {
+    const int size = (n + VF_PARTS - 1) / VF_PARTS;
+    from = min(part * size, n); to = min(from + size, n);
+}
+
+// Where the drafts of a request end, and the weights of each part of that row, added up: a part by each wave
+__global__ __launch_bounds__(256) void verify_sum_kernel(verify_args a) {
+    __shared__ uint2 s_list[4][256];
+    const int request = blockIdx.x / (VF_PARTS / 4), part = blockIdx.x % (VF_PARTS / 4) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wave = part & 3;
+    const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
     if (row0 < 0 || row1 < row0 || row1 > a.n_row) { if (a.err) *a.err = 1; return; }
     if (row0 == row1) return;
-    const bool drawn_from = a.draft.logits != nullptr;                            // else a draft is certain of its token
-    const auto share = [](u64 w, u64 all) { return all ? (double)w / (double)all : 0.0; };
     int stop = row1 - 1;
     for (int base = row0; base < row1 - 1; base += 64) {
         const int r = min(base + lane, row1 - 2);
         const float u = a.accept[r] > 0.0f ? fminf(a.accept[r], 0.99999994f) : 0.0f;
-        const double p = share(a.cuts[r].weight, a.cuts[r].total), q = drawn_from ? share(a.cuts[a.n_row + (int64_t)r].weight, a.cuts[a.n_row + (int64_t)r].total) : 1.0;
+        const double p = verify_p(a, r), q = a.draft.logits ? verify_p(a, (int64_t)a.n_row + r) : 1.0;        // (no distribution: the draft is certain)
         const unsigned long long not_taken = __ballot(!((double)u * q < p));
-        if (not_taken) { stop = min(base + __builtin_amdgcn_readfirstlane(__ffsll(not_taken) - 1), row1 - 2); break; }
+        if (not_taken) { stop = min(base + __ffsll(not_taken) - 1, row1 - 2); break; }
     }
-    const sample_cut c = a.cuts[stop];
-    const bool at_end = stop == row1 - 1;
-    const int drafted = at_end ? -1 : a.drafted[stop];
+    stop = __builtin_amdgcn_readfirstlane(stop);
+    if (part == 0 && lane == 0) a.stops[request] = stop;
+    if (!a.cuts[stop].total || a.cuts[stop].n_kept <= SM_KEPT) return;
+    const verify_weights weights(a, stop, stop == row1 - 1);
+    int from, to;
+    verify_part(weights.n, part, from, to);
+    const u64 sum = weights.sum(from, to, s_list[wave]);
+    if (lane == 0) a.sums[(int64_t)request * VF_PARTS + part] = sum;
+}
+
+__global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) {
+    __shared__ sample_shared s;
+    __shared__ uint2 s_list[16][256];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), request = blockIdx.x;
+    const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
+    if (row0 < 0 || row1 <= row0 || row1 > a.n_row) return;                        // (the launch before has raised the flag)
+    const int stop = __builtin_amdgcn_readfirstlane(a.stops[request]);
+    const u64 c_total = a.cuts[stop].total;
+    const uint32_t n_kept = a.cuts[stop].n_kept;
     for (int r = row0 + t; r < row1; r += SM_THREADS) {
         if (r == stop) continue;
         a.tokens[r] = r < stop ? a.drafted[r] : -1;
-        if (a.probs) a.probs[r] = r < stop ? (float)share(a.cuts[r].weight, a.cuts[r].total) : 0.0f;
+        if (a.probs) a.probs[r] = r < stop ? (float)verify_p(a, r) : 0.0f;
     }
     if (t == 0) {
-        a.accepted[blockIdx.x] = stop - row0;
-        if (!c.total) { a.tokens[stop] = -1; if (a.probs) a.probs[stop] = 0.0f; }
+        a.accepted[request] = stop - row0;
+        if (!c_total) { a.tokens[stop] = -1; if (a.probs) a.probs[stop] = 0.0f; }
     }
-    if (!c.total) return;                                                         // a row without a logit above -inf
-    const sample_args &g = a.target;
-    sample_row row;
-    row.g = (const float *)(g.logits + stop * g.stride);
-    row.n = g.n; row.begin = wave * g.part; row.part = g.part; row.held = g.held; row.infinite = c.infinite;
-    f4 *const held = (f4 *)(smem + sizeof(sample_shared));
-    row.lds = held + wave * (g.held / 4);
-    row.load(0);
-    struct left {                                                                 // what settings leave of a row
-        weigher weigh;
-        float last_l;
-        int last_i;
-        __device__ __forceinline__ left(const sample_args &g, const sample_cut &c, int r) {
-            const float temp = g.temperature ? g.temperature[r] : 1.0f;
-            weigh = weigher_of(temp > 0.0f ? temp : 1.0f, c.top);                 // (the only token left of a greedy row has the largest logit: any temperature)
-            last_l = c.last == ~0ull ? -INFINITY : logit_of(c.last);
-            last_i = (int)(uint32_t)min(c.last & 0xFFFFFFFFull, 0x7FFFFFFFull);
+    if (!c_total) return;                                                         // a row without a logit above -inf
+    verify_weights weights(a, stop, stop == row1 - 1);
+    const float u = a.target.uniform[stop];
+    const auto drawn = [&](int i, float v) { a.tokens[stop] = i; if (a.probs) a.probs[stop] = (float)share_of_all(weights.p.weigh(v), c_total); };
+    if (n_kept <= SM_KEPT) {
+        // one token a thread
+        const bool there = (uint32_t)t < n_kept;
+        const u64 x = there ? a.kept[(int64_t)stop * SM_KEPT + t] : 0;
+        const float v = there ? logit_of(x) : -INFINITY;
+        const int i = (int)(uint32_t)x, range = i >> a.target.range_log2;
+        const float l = there && weights.beyond_q ? weights.gq[i] : 0.0f;
+        s.mass[t] = 0;
+        if (t == 0) s.n_list = 0;
+        u64 w, total, before, all;
+        for (;;) {
+            w = there ? weights(v, l, i) : 0;
+            block_scan(s, w, total);
+            if (weights.as_p || total) break;
+            weights.as_p = true;                                                  // p and q are the same but for their roundings
+            __syncthreads();
         }
-        __device__ __forceinline__ bool has(float v, int i) const { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); }
-    };
-    const left p(g, c, stop);
-    sample_cut cq = {0, 0, 0, 0.0f, 0};
-    const bool beyond_q = !at_end && drawn_from;
-    if (beyond_q) cq = a.cuts[a.n_row + (int64_t)stop];
-    const left q(a.draft, cq, stop);
-    const float *const gq = (const float *)(a.draft.logits + stop * a.draft.stride);
-    const double one_p = 1.0 / (double)c.total, one_q = cq.total ? 1.0 / (double)cq.total : 0.0;
-    bool as_p = at_end;                                                           // from p itself
-    const auto weight = [&](float v, int i) -> u64 {
-        if (!p.has(v, i)) return 0;
-        const u64 w = p.weigh(v);
-        if (as_p) return w;
-        if (!beyond_q) return i == drafted ? 0 : w;
-        float l = gq[i];
-        l = cq.infinite ? (l == INFINITY ? 0.0f : -INFINITY) : l;                 // (a NaN is not left by any setting)
-        const double more = (double)w * one_p - (q.has(l, i) && cq.total ? (double)q.weigh(l) * one_q : 0.0);
-        return more > 0.0 ? (u64)(more * 0x1p60) : 0;
-    };
-    for (;;) {
-        u64 sum = 0;
-        row.groups([&](f4 v, int i) {
-            bool some = false;
-#pragma unroll
-            for (int e = 0; e < 4; e++) some |= p.has(v[e], i + e);
-            if (!__any(some)) return;
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += weight(v[e], i + e);
-        });
-        sum = of_lane(wave_scan(sum), 63);
-        if (lane == 0) s.part[wave] = sum;
+        const u64 want = draw_at(u, total);
+        // in order of index: weights by range of the index, then inside one of the ranges
+        if (w) atomicAdd(&s.mass[range], w);
         __syncthreads();
-        if (as_p || of_lane(row_scan(s.part[lane & 15]), 15)) break;
-        as_p = true;                                                              // p and q are the same but for their roundings
+        const int in = find_bin(s, s.mass[t], want, before, all);
+        const bool mine = w && range == in;
+        if (mine) { const uint32_t k = atomicAdd(&s.n_list, 1u); s.x[k] = (uint32_t)i; s.w[k] = w; }
         __syncthreads();
+        if (mine) {
+            u64 upto = before + w;
+            for (uint32_t j = 0; j < s.n_list; j++) if (s.x[j] < (uint32_t)i) upto += s.w[j];
+            if (upto >= want && upto - w < want) drawn(i, v);
+        }
+        return;
     }
-    const float u = g.uniform[stop];
-    draw_by_parts(g, s, row, held, u, weight, [&](int i, u64, u64) {
-        a.tokens[stop] = i;
-        if (a.probs) a.probs[stop] = (float)share(p.weigh(row.clean(f4{row.g[i], 0.0f, 0.0f, 0.0f})[0]), c.total);
+    u64 sums = wave_scan(a.sums[(int64_t)request * VF_PARTS + lane]);
+    if (!weights.as_p && !of_lane(sums, 63)) {
+        weights.as_p = true;                                                      // as above: the sums once more, four parts by each wave
+        for (int k = 0; k < VF_PARTS / 16; k++) {
+            int from, to;
+            verify_part(weights.n, 16 * k + wave, from, to);
+            const u64 sum = weights.sum(from, to, s_list[wave]);
+            if (lane == 0) s.mass[16 * k + wave] = sum;
+        }
+        __syncthreads();
+        sums = wave_scan(s.mass[lane]);
+    }
+    // the part that the random number falls into, a sixteenth of it by each wave, then a token a lane
+    const u64 want_all = draw_at(u, of_lane(sums, 63));
+    const int part = max(__ffsll(__ballot(sums >= want_all)) - 1, 0);
+    u64 want = want_all - (part ? of_lane(sums, part - 1) : 0);
+    int from, to;
+    verify_part(weights.n, part, from, to);
+    const int size = (to - from + 15) / 16, begin = min(from + wave * size, to), end = min(begin + size, to);
+    const u64 sum = weights.sum(begin, end, s_list[wave]);
+    if (lane == 0) s.part[wave] = sum;
+    __syncthreads();
+    const u64 parts = row_scan(s.part[lane & 15]);
+    if (wave != max(__ffsll(__ballot(parts >= want)) - 1, 0)) return;
+    want -= wave ? of_lane(parts, wave - 1) : 0;
+    u64 before = 0;
+    weights.each(begin, end, s_list[wave], [&](u64 w, int i, float v) {
+        const u64 upto = before + wave_scan(w);
+        if (w && upto >= want && upto - w < want) drawn(i, v);
+        before = of_lane(upto, 63);
     });
 }
 
+static inline size_t verify_cuts(int64_t n_row) { return ((size_t)n_row * 2 * sizeof(sample_cut) + 255) / 256 * 256; }
+static inline size_t verify_scratch(int64_t n_row, int64_t n_seq) { return verify_cuts(n_row) + (size_t)n_row * SM_KEPT * 8 + (size_t)n_seq * (VF_PARTS * 8 + 4); }
 extern "C" size_t spy_hip_sample_verify_scratch_size(const spy_hip_tensor *logits, int32_t n_seq) {
-    return logits && n_seq > 0 && logits->ne[1] > 0 && logits->ne[1] < (1 << 22) ? (size_t)logits->ne[1] * 2 * sizeof(sample_cut) : 0;
+    return logits && n_seq > 0 && logits->ne[1] > 0 && logits->ne[1] < (1 << 22) ? verify_scratch(logits->ne[1], n_seq) : 0;
 }
 
 extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits, const spy_hip_sample_param *param, const spy_hip_tensor *draft_logits, const spy_hip_sample_param *draft_param,
@@ -145,22 +261,24 @@ extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits,
     if (rc) return rc;
     SPY_CHECK_ARG(!draft_logits || (draft_logits->data && draft_logits->ne[0] == logits->ne[0] && draft_logits->ne[1] == logits->ne[1]));
     const int64_t n_row = logits->ne[1], blocks = n_row * (draft_logits ? 2 : 1);
-    SPY_CHECK_ARG(blocks * SM_THREADS < (1ll << 32) && (int64_t)n_seq * SM_THREADS < (1ll << 32));
-    if (scratch_bytes < (size_t)n_row * 2 * sizeof(sample_cut)) return SPY_HIP_ENOSPACE;
+    SPY_CHECK_ARG(blocks * SM_THREADS < (1ll << 32) && (int64_t)n_seq * VF_PARTS * 64 < (1ll << 32));
+    if (scratch_bytes < verify_scratch(n_row, n_seq)) return SPY_HIP_ENOSPACE;
     SPY_CHECK_ARG(scratch && ((uintptr_t)scratch & 255) == 0);
     verify_args a;
     a.target = sample_args_of(logits, param);
     a.draft = draft_logits ? sample_args_of(draft_logits, draft_param) : a.target;
     if (!draft_logits) a.draft.logits = nullptr;
     a.drafted = drafted; a.row_start = row_start; a.accept = accept; a.n_seq = n_seq; a.n_row = (int)n_row;
-    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.err = spy_hip_err_flag_ptr();
+    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.stops = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.err = spy_hip_err_flag_ptr();
     const size_t lds = sample_lds(a.target);
     rc = spy_raise_lds_limit((const void *)verify_cut_kernel, lds);
-    if (!rc) rc = spy_raise_lds_limit((const void *)verify_draw_kernel, lds);
     if (rc) return rc;
     verify_cut_kernel<<<dim3((unsigned)blocks), dim3(SM_THREADS), lds, (hipStream_t)stream>>>(a);
     rc = SPY_LAUNCH_RC();
     if (rc) return rc;
-    verify_draw_kernel<<<dim3((unsigned)n_seq), dim3(SM_THREADS), lds, (hipStream_t)stream>>>(a);
+    verify_sum_kernel<<<dim3((unsigned)(n_seq * (VF_PARTS / 4))), dim3(256), 0, (hipStream_t)stream>>>(a);
+    rc = SPY_LAUNCH_RC();
+    if (rc) return rc;
+    verify_draw_kernel<<<dim3((unsigned)n_seq), dim3(SM_THREADS), 0, (hipStream_t)stream>>>(a);
     return SPY_LAUNCH_RC();
 }
