@@ -505,7 +505,7 @@ template <int D> struct chunk_group { __attribute__((aligned(1024))) uint8_t k[2
 template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared { chunk_group<D> group[GROUPS]; int unbounded; };
 template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared_q8 : chunk_shared<D, GROUPS> { __attribute__((aligned(16))) uint8_t scales[4 * GROUPS][D * 4]; };      // of V^T, a wave's own copy
 
-// Q8: a tile's whole numbers are in registers while the tile before is computed with, and go to LDS as fp16 values.
+// Q8: a tile's whole numbers come to registers two tiles ahead and go to LDS as fp16 values one tile ahead, beside the matrix instructions of the scores, which leave the vector units time for it.
 template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D), class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false) {
     constexpr bool Q8 = MODE & ATTN_Q8, SHARED = MODE & ATTN_SHARED;
     constexpr int ES = Q8 ? 1 : 2;                                         // bytes of an element in the pages
@@ -640,11 +640,20 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
     for (int d = 0; d < DT; d++) o[d] = v16f{0};
     constexpr uint32_t BUF = 64 * D * 2;                                   // bytes of one buffer
     uint32_t k_at = n * (2 * D) + (half ^ swizzle_k<D>(n)) * 16, v_at = n * 128 + (half ^ swizzle_v(n)) * 16;     // this lane's pieces in LDS
+    // Q8: piece j of this wave's, of the tile in the registers, as fp16 to LDS (where there is no such tile, what is in them, to where nobody reads)
+    const auto unpack_piece = [&](int j, int to) __attribute__((always_inline)) {
+        if constexpr (Q8) {
+            const int i = j < NI ? j : j - NI;
+            const uint4 v = j < NI ? bits(dequantized(raw_k[i], all_of(raw_d[i]))) : bits(dequantized(raw_v[i], *(const v8h *)(shared.scales[wave8] + (8 * i + vc) * 16)));
+            *(uint4 *)((j < NI ? sh.k[to] : sh.v[to]) + (4 * i + wave) * 1024 + lane * 16) = v;
+        }
+    };
     const auto compute = [&](int kt, int buf, int bad, bool masked, group_pages next) {
         const int kb = begin + 64 * kt;
         const uint32_t more = there_is(kt + GROUPS);
         // LDS answers after some 130 cycles, four times what an instruction that waits for it takes: operands are asked for in order, well before their use, and the
         // barriers between keep the compiler from moving the requests back to where they are used
+        if constexpr (Q8) landed();                                        // the next tile's numbers and scales
         asm volatile("" : "+v"(k_at), "+v"(v_at));                         // (addresses once more for every tile: the compiler would keep all of them, in registers that it has not)
         const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + d * 4096 + (v_at ^ k * 32)); };
         v16f x[2] = {{0}, {0}};
@@ -662,11 +671,13 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
                 if (i + AHEAD < 2 * KS) fk[i % AHEAD] = k_piece(i + AHEAD);
                 else if (i + AHEAD < 2 * KS + 2 * DT) w[(i + AHEAD - 2 * KS) / DT][(i + AHEAD - 2 * KS) % DT] = v_piece((i + AHEAD - 2 * KS) % DT, (i + AHEAD - 2 * KS) / DT);
                 if (!Q8 && i % 4 == 0) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, more, i / 4);        // the next tile's, one at a time: all at once, they take 1000 cycles to issue
+                if (Q8 && i % 2 == 1) unpack_piece(i / 2, buf ^ 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int i = AHEAD; i < 2 * DT; i++) w[i / DT][i % DT] = v_piece(i % DT, i / DT);
         }
+        if constexpr (Q8) if (kt + 2 * GROUPS < stop) ask_raw(kb + 128 * GROUPS, next);
         // register 8 s + j of tile t: key 32 t + 16 s + 8 half + j.  This lane's query sees register i's where lies(i, first) holds, first: the register 0's from lo on
         const int mine = kb + 8 * half;
         const uint32_t span = max(hi - lo, 0);
@@ -745,28 +756,22 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
         }
         if (any) shared.unbounded = 1;
     };
-    // Q8: the tile's pieces of this wave as fp16 to LDS
-    const auto unpack = [&](int kt, int buf, int bad, bool masked) {
-        if constexpr (Q8) {
-            const int there = bad >> (vc >> 1) & 1 ? 0 : end - (begin + 64 * kt + 8 * vc);
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < NI; i++) {
-                *(uint4 *)(sh.k[buf] + (4 * i + wave) * 1024 + lane * 16) = bits(dequantized(raw_k[i], all_of(raw_d[i])));
-                uint4 v = bits(dequantized(raw_v[i], *(const v8h *)(shared.scales[wave8] + (8 * i + vc) * 16)));
-                if (masked) v = bounded(first_of(v, there), any);
-                *(uint4 *)(sh.v[buf] + (4 * i + wave) * 1024 + lane * 16) = v;
-            }
-            if (any) shared.unbounded = 1;
-        }
-    };
     const int steps = (max(stop - from, 0) + GROUPS - 1) / GROUPS;
     if (steps) {
         int kt = from + group, i = 0, fetched = 0;               // (tiles are numbered from `from` on where their pages are looked up)
         take_entries(first_pages);
         int bad = gone_of(group);
+        int bad_next = 0;                                        // (Q8)
         if constexpr (Q8) {
-            if (kt < stop) ask_raw(begin + 64 * kt, pages_of(group));
+            if (kt < stop) {
+                ask_raw(begin + 64 * kt, pages_of(group));
+                landed();
+#pragma unroll
+                for (int j = 0; j < 2 * NI; j++) unpack_piece(j, 0);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (kt + GROUPS < stop) ask_raw(begin + 64 * (kt + GROUPS), pages_of(group + GROUPS));
+            }
+            bad_next = gone_of(group + GROUPS);
         } else {
             const group_pages now = pages_of(group);
             const uint8_t *const v_from = v_source(begin + 64 * kt, now);
@@ -780,11 +785,10 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
         const auto step = [&](auto idle_) __attribute__((always_inline)) { // one tile; true: it was the last
             const int buf = i & 1, kb = begin + 64 * kt;
             const bool masked = kt < stop && (kb + 64 > hi_all || kb < lo_all || bad);
-            landed();                                                      // what this wave requested of this tile is in LDS ...
-            if constexpr (Q8) { if (kt < stop) unpack(kt, buf, bad, masked); }
-            else if (masked) bound_v(kt, buf, bad);
+            if constexpr (!Q8) landed();                                   // what this wave requested of this tile is in LDS ...
+            if (masked) bound_v(kt, buf, bad);
             __syncthreads();                                               // ... and all of it, and nobody reads the other buffer any more
-            const int ahead = kt - from + GROUPS;
+            const int ahead = kt - from + (Q8 ? 2 : 1) * GROUPS;
             if ((ahead & 15) == group) take_entries(fetched);
             if ((ahead + GROUPS & 15) == group) fetched = entries_of(ahead + GROUPS);
             const group_pages next = pages_of(ahead);
@@ -794,15 +798,21 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
                 for (int g = 0; g < 4; g++) wanted |= (kb + 16 * g < end && kb + 16 * g + 16 > lo_any) << g;
                 if (bad & wanted) *err = 1;
             }
-            if constexpr (Q8) if (kt + GROUPS < stop) ask_raw(kb + 64 * GROUPS, next);
-            if constexpr (idle_ && !Q8) {
+            if constexpr (idle_ && Q8) {
+                landed();
+#pragma unroll
+                for (int j = 0; j < 2 * NI; j++) unpack_piece(j, buf ^ 1);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (kt + 2 * GROUPS < stop) ask_raw(kb + 128 * GROUPS, next);
+            } else if constexpr (idle_) {
                 const uint8_t *const v_from = v_source(kb + 64 * GROUPS, next);
 #pragma unroll
                 for (int j = 0; j < NI; j++) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
 #pragma unroll
                 for (int j = 0; j < NI; j++) ask_v(v_from, (buf ^ 1) * BUF, there_is(kt + GROUPS), j);
             } else if (!idle_ && kt < stop) compute(kt, buf, bad, masked, next);
-            bad = gone_of(ahead);
+            if constexpr (Q8) { bad = bad_next; bad_next = gone_of(ahead); }
+            else bad = gone_of(ahead);
             kt += GROUPS;
             return ++i == steps;
         };
