@@ -480,9 +480,10 @@ static __device__ __forceinline__ bool find_span(const attn_more &a, bool common
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.groups.n_group; base += 64) {
         int n = 0;
+        pg_span q = {};
         if (base + lane < a.groups.n_group) {
             const int g = base + lane;
-            const pg_span q = pg_group(a.b, a.groups, a.groups.seq_start[g], a.groups.seq_start[g + 1], a.groups.length[g], a.err);
+            q = pg_group(a.b, a.groups, a.groups.seq_start[g], a.groups.seq_start[g + 1], a.groups.length[g], a.err);
             const int rows = q.ok ? q.n_new * a.group : 0;
             n = rows > a.few ? (rows + CHUNK_ROWS - 1) / CHUNK_ROWS : 0;
         }
@@ -492,8 +493,9 @@ static __device__ __forceinline__ bool find_span(const attn_more &a, bool common
             const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
             tile = left - __builtin_amdgcn_readlane(sum - n, at);
             count = __builtin_amdgcn_readlane(n, at);
-            sq = pg_group(a.b, a.groups, a.groups.seq_start[base + at], a.groups.seq_start[base + at + 1], a.groups.length[base + at], a.err);
-            return sq.ok;
+            sq.row0 = __builtin_amdgcn_readlane(q.row0, at); sq.n_new = __builtin_amdgcn_readlane(q.n_new, at); sq.kv = __builtin_amdgcn_readlane(q.kv, at);
+            sq.s = __builtin_amdgcn_readlane(q.s, at); sq.from = 0; sq.ok = true;
+            return true;
         }
         left -= __builtin_amdgcn_readlane(sum, 63);
     }
