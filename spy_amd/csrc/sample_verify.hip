@@ -20,7 +20,7 @@ struct verify_args {
     sample_cut *cuts;                    // of the target's rows, then of the draft's
     u64 *kept;                           // of the target's rows: SM_KEPT each
     u64 *sums;                           // of the requests: VF_PARTS each
-    int32_t *stops;                      // of the requests: the row where its drafts end
+    int32_t *stops;                      // of the requests: the row where its drafts end, -1: none
     int *err;
 };
 
@@ -136,8 +136,14 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(verify_args a) {
     __shared__ uint2 s_list[4][256];
     const int request = blockIdx.x / (VF_PARTS / 4), part = blockIdx.x % (VF_PARTS / 4) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wave = part & 3;
     const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
-    if (row0 < 0 || row1 < row0 || row1 > a.n_row) { if (a.err) *a.err = 1; return; }
-    if (row0 == row1) return;
+    int past = 0;                                                                 // rows that the requests before it have taken: where one of them went further, the launch before gave it these rows
+    for (int i = lane; i < request; i += 64) past = max(past, a.row_start[i]);
+    const bool sound = row0 >= 0 && row1 >= row0 && row1 <= a.n_row && !__any(past > row0);
+    if (!sound && a.err) *a.err = 1;
+    if (!sound || row0 == row1) {
+        if (part == 0 && lane == 0) a.stops[request] = -1;
+        return;
+    }
     int stop = row1 - 1;
     for (int base = row0; base < row1 - 1; base += 64) {
         const int r = min(base + lane, row1 - 2);
@@ -160,9 +166,8 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
     __shared__ sample_shared s;
     __shared__ uint2 s_list[16][256];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), request = blockIdx.x;
-    const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
-    if (row0 < 0 || row1 <= row0 || row1 > a.n_row) return;                        // (the launch before has raised the flag)
-    const int stop = __builtin_amdgcn_readfirstlane(a.stops[request]);
+    const int row0 = a.row_start[request], row1 = a.row_start[request + 1], stop = __builtin_amdgcn_readfirstlane(a.stops[request]);
+    if (stop < 0) return;                                                         // without rows, or rows that do not fit
     const u64 c_total = a.cuts[stop].total;
     const uint32_t n_kept = a.cuts[stop].n_kept;
     for (int r = row0 + t; r < row1; r += SM_THREADS) {

@@ -292,6 +292,30 @@ def test_requests_that_do_not_fit_are_left_alone(hip):
     assert P.flag() != 0 and got[1][0] == -7 and np.array_equal(got[0][start[1]:], want[0][start[1]:])
 
 
+@pytest.mark.parametrize("start, alone", [([0, 3, 1, 6], [1, 2]), ([0, 2, 9, 1, 4], [1, 2, 3]), ([5, 7, 0, 4], [1, 2]), ([2, 4, 4, 3, 8], [2, 3])])
+@pytest.mark.parametrize("drafter", [True, False])
+def test_requests_that_begin_before_one_in_front_of_them(hip, start, alone, drafter):
+    """Left alone, whatever their rows; the others are as if by themselves."""
+    from spy_amd import _lib as H
+    rng = np.random.default_rng(8)
+    logits, draft = (rng.standard_normal((8, 1500)).astype(np.float32) for _ in range(2))
+    accept, uniform = rng.random(8).astype(np.float32), rng.random(8).astype(np.float32)
+    drafted = drawn_from(rng, draft)
+    tokens, accepted, probs = run(H, logits, drafted, np.asarray(start, np.int32), accept, uniform, dict(top_p=0.9), draft if drafter else None)
+    assert P.flag() != 0
+    sound = np.zeros(8, bool)
+    for s in range(len(start) - 1):
+        if s in alone:
+            assert accepted[s] == -7
+            continue
+        a, b = start[s], start[s + 1]
+        sound[a:b] = True
+        if a < b:
+            one = np.array([0, b - a])
+            check((tokens[a:b], accepted[s:s + 1], probs[a:b]), logits[a:b], drafted[a:b], one, accept[a:b], uniform[a:b], dict(top_p=0.9), draft[a:b] if drafter else None)
+    assert (tokens[~sound] == -7).all() and (probs[~sound] == -7).all()
+
+
 def test_strided_rows_and_replays(hip):
     """Rows that are parts of wider ones, 4 bytes aligned; a recorded call replayed with other drafts, rows and numbers between eager calls."""
     from spy_amd import _lib as H
