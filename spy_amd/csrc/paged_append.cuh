@@ -87,12 +87,12 @@ static __device__ __forceinline__ int append_tile(const append_args &a, int tile
     return -1;
 }
 
-// Rows, batch and rotation of a call: 0 and `a` without what it says of the pages' memory, or the code that the call is refused with.  hd, ps, G: of the pages, which have been
-// checked, and n_page of them.
+// Rows, batch and rotation of a call: 0 and `a` without what it says of the pages' memory, or the code that the call is refused with.  The pages have been checked, each kind by itself.
 static inline int append_check(append_args &a, const spy_hip_tensor *q, const spy_hip_tensor *k, const spy_hip_tensor *v, const spy_hip_paged_batch *batch, const spy_hip_rope_param *rope,
-                               const spy_hip_tensor *q_out, int64_t hd, int64_t ps, int64_t G, int64_t n_page) {
+                               const spy_hip_tensor *q_out, const spy_hip_tensor *k_pages, const spy_hip_tensor *v_pages) {
     if ((k->type != SPY_HIP_F32 && k->type != SPY_HIP_F16) || v->type != k->type || (q && (q->type != k->type || q_out->type != SPY_HIP_F16))) return SPY_HIP_EUNSUPPORTED;
-    const int64_t n_row = k->ne[2], H = q ? q->ne[1] : 0;
+    const int64_t hd = k_pages->ne[0], ps = k_pages->ne[1], G = k_pages->ne[2], n_row = k->ne[2], H = q ? q->ne[1] : 0;
+    SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3]);
     SPY_CHECK_ARG(n_row > 0 && n_row < (1 << 28) && G <= 65535 && H <= 65535 && pg_rows_ok(k, hd, G, n_row) && pg_rows_ok(v, hd, G, n_row));
     SPY_CHECK_ARG(!q || (H > 0 && H % G == 0 && pg_rows_ok(q, hd, H, n_row) && pg_rows_ok(q_out, hd, H, n_row)));
     a.mode = rope ? rope->mode : -1;
@@ -111,7 +111,7 @@ static inline int append_check(append_args &a, const spy_hip_tensor *q, const sp
     a.q_h = q ? q->nb[1] : 0; a.q_t = q ? q->nb[2] : 0; a.qo_h = q ? q_out->nb[1] : 0; a.qo_t = q ? q_out->nb[2] : 0;
     a.k_h = k->nb[1]; a.k_t = k->nb[2]; a.v_h = v->nb[1]; a.v_t = v->nb[2];
     a.b.row_start = batch->row_start; a.b.kv_len = batch->kv_len; a.b.pages = batch->pages; a.b.page_stride = batch->page_stride;
-    a.b.n_seq = batch->n_seq; a.b.n_row = (int)n_row; a.b.max_new = batch->max_new; a.b.max_kv = batch->max_kv; a.b.n_page = (int)n_page; a.b.page_log2 = pg_log2(ps);
+    a.b.n_seq = batch->n_seq; a.b.n_row = (int)n_row; a.b.max_new = batch->max_new; a.b.max_kv = batch->max_kv; a.b.n_page = (int)k_pages->ne[3]; a.b.page_log2 = pg_log2(ps);
     a.H = (int)H; a.G = (int)G; a.hd = (int)hd; a.err = spy_hip_err_flag_ptr();
     return 0;
 }

@@ -128,11 +128,10 @@ extern "C" int spy_hip_paged_append(void *stream, const spy_hip_tensor *q, const
     if (!rc) rc = pg_check_pages(k_pages, 1);
     if (!rc) rc = pg_check_pages(v_pages, 0);
     if (rc) return rc;
-    const int64_t hd = k_pages->ne[0], ps = k_pages->ne[1], G = k_pages->ne[2], n_row = k->ne[2], H = q ? q->ne[1] : 0;
+    const int64_t hd = k_pages->ne[0], G = k_pages->ne[2], n_row = k->ne[2], H = q ? q->ne[1] : 0;
     append_args a;
-    rc = append_check(a, q, k, v, batch, rope, q_out, hd, ps, G, k_pages->ne[3]);
+    rc = append_check(a, q, k, v, batch, rope, q_out, k_pages, v_pages);
     if (rc) return rc;
-    SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3]);
     a.kp = (uint8_t *)k_pages->data; a.vp = (uint8_t *)v_pages->data;
     a.kp_p = k_pages->nb[1]; a.kp_h = k_pages->nb[2]; a.kp_g = k_pages->nb[3];
     a.vp_d = v_pages->nb[1]; a.vp_h = v_pages->nb[2]; a.vp_g = v_pages->nb[3];

@@ -175,11 +175,10 @@ extern "C" int spy_hip_paged_append_q8(void *stream, const spy_hip_tensor *q, co
     if (!rc) rc = pg_check_scales(k_scales, k_pages, 1);
     if (!rc) rc = pg_check_scales(v_scales, v_pages, 0);
     if (rc) return rc;
-    const int64_t hd = k_pages->ne[0], ps = k_pages->ne[1], G = k_pages->ne[2], n_row = k->ne[2], H = q ? q->ne[1] : 0;
+    const int64_t hd = k_pages->ne[0], G = k_pages->ne[2], n_row = k->ne[2], H = q ? q->ne[1] : 0;
     append_q8_args a;
-    rc = append_check(a, q, k, v, batch, rope, q_out, hd, ps, G, k_pages->ne[3]);
+    rc = append_check(a, q, k, v, batch, rope, q_out, k_pages, v_pages);
     if (rc) return rc;
-    SPY_CHECK_ARG(v_pages->ne[0] == ps && v_pages->ne[1] == hd && v_pages->ne[2] == G && v_pages->ne[3] == k_pages->ne[3]);
     a.kp = (uint8_t *)k_pages->data; a.vp = (uint8_t *)v_pages->data; a.ks = (uint8_t *)k_scales->data; a.vs = (uint8_t *)v_scales->data;
     a.kp_p = k_pages->nb[1]; a.kp_h = k_pages->nb[2]; a.kp_g = k_pages->nb[3]; a.ks_h = k_scales->nb[2]; a.ks_g = k_scales->nb[3];
     a.vp_d = v_pages->nb[1]; a.vp_h = v_pages->nb[2]; a.vp_g = v_pages->nb[3]; a.vs_b = v_scales->nb[1]; a.vs_h = v_scales->nb[2]; a.vs_g = v_scales->nb[3];
