@@ -508,7 +508,26 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
         u64 tail = 0;
         uint32_t n_tail = 0;
         const bool look = by_rank || flat;                                        // (else -inf adds 0, and nothing is counted)
-        row.each([&](float v, int) {
+        if (CUT && !flat) {
+            // by fours and without branches: what is far away adds nothing, at a place of the lane's own
+            row.groups([&](f4 v, int) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = weigh.far(v[e]);
+                    const u64 w = weigh.at(y);
+                    const bool here = y < reach;
+                    const int b = here ? (int)(y * 32.0f) : lane;
+                    const u64 add = here ? w : 0;
+                    tail += w - add;
+                    atomicAdd(&s.mass[b], add);
+                    if (by_rank) {
+                        atomicAdd(&s.count[b], (uint32_t)here);
+                        n_tail += !here & (v[e] > -INFINITY);
+                    }
+                }
+            });
+            if (!by_rank) n_tail = tail != 0;
+        } else row.each([&](float v, int) {
             const bool there = (!look) | (v > -INFINITY);
             const float y = weigh.far(v);
             const u64 w = weigh.at(y);
@@ -542,17 +561,22 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             const int last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
             u64 sum = 0;
             if constexpr (CUT) {                                                  // (the weights before the bin are known)
+                // distances that the bin may hold, a little more
+                const float nearer = flat ? -INFINITY : near / weigh.c * 0.9999f, farther = flat || bin == SM_BINS - 1 ? INFINITY : upper / weigh.c * 1.0001f;
                 row.groups([&](f4 v, int i) {
-                    bool there[4], any = false;
+                    bool some = false;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float y = flat && !(v[e] > -INFINITY) ? INFINITY : weigh.far(v[e]);
-                        there[e] = (y >= near) & !(y >= upper) & (v[e] > -INFINITY);
-                        any |= there[e];
+                        const float far = fmaf(-v[e], weigh.unit, weigh.top);
+                        some |= far == __builtin_amdgcn_fmed3f(far, nearer, farther);
                     }
-                    if (__any(any))
+                    if (some)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) append(s, there[e], v[e], i + e, weigh);
+                        for (int e = 0; e < 4; e++)
+                            if (in(v[e])) {
+                                const uint32_t at = atomicAdd(&s.n_list, 1u);
+                                if (at < SM_LIST) s.x[at] = rank_word(v[e], i + e);
+                            }
                 });
             } else row.groups([&](f4 v, int i) {
                 float y[4];
@@ -592,6 +616,7 @@ template <bool CUT> static __device__ __forceinline__ void sample_row_of(const s
             u64 lo = 0;
             int fine = 0;
             if (!listed) { __syncthreads(); m = narrow(s, row, weigh, in, which == 1, want, before, lo, fine); }
+            if (CUT && listed && (uint32_t)t < m) s.w[t] = weigh(logit_of(s.x[t]));
             rank_list(s, m, [&](u64 x) {
                 return listed ? (int)fminf((weigh.far(logit_of(x)) * 32.0f - (float)bin) * (float)SM_BINS, (float)(SM_BINS - 1)) : (int)((x - lo) >> fine);
             });

@@ -2,9 +2,14 @@
 // draft's distribution and a_i a given random number; the first that is not taken is replaced by one drawn from max(p_i - q_i, 0), and behind the last one that is taken one is drawn from p.
 // Tokens that come out are distributed as the target's alone: min(p, q) of d is what the draft proposes and is taken, and max(p - q, 0) is what p has beyond that.
 //
-// First launch: a workgroup for each row and distribution finds what the settings leave -- the last rank word, the sum of the weights and d's own (sample_row_of<true>).  Second launch: a
-// workgroup for each request finds the row where its drafts end and draws there.  p and q are weights over their sums, in 64 bits; p - q as multiples of 2^-60, so that sums of it are
-// exact in any order.
+// First launch: a workgroup for each row and distribution finds what the settings leave -- the last rank word, the sum of the weights and d's own (sample_row_of<true>), and the tokens themselves where
+// they are 1024 at most.  Second launch: four workgroups for each request find the row where its drafts end and draw there, one of them alone where it has those tokens.  p and q are weights over
+// their sums, in 64 bits; p - q as multiples of 2^-60, so that sums of it are exact in any order, and what comes out is the same each time.
+//
+// Latency and vector instructions: the first launch reads each row once from memory (verify of 32 requests with 1 to 6 rows of 32000 and a drafter's: 37 us, 24.6 of them here), and where top_p alone is set it
+// works out every weight: 160 rows of 100003 by as many workgroups 55 us, 12 for the reads, 24 for the weights (20 instructions a token beside an addition in LDS), 17 for the bin's tokens.  The
+// second is a chain of dependent reads (one request: 6 us) and, where more tokens are left, one pass over the row: 18 us for 64 requests of 100003.  One request with 5 rows of 32000: 21 us in all.  Taking the
+// weights of tokens that are not left as well took 102 us for the large case; three launches, the parts' sums one of their own, 0.3 to 0.8 more than two.
 #include "paged.cuh"
 #include "sample.cuh"
 
@@ -20,13 +25,14 @@ struct verify_args {
     sample_cut *cuts;                    // of the target's rows, then of the draft's
     u64 *kept;                           // of the target's rows: SM_KEPT each
     u64 *sums;                           // of the requests: VF_PARTS each
-    int32_t *stops;                      // of the requests: the row where its drafts end, -1: none
+    int32_t *arrived;                    // of the requests: workgroups that have added up their parts
     int *err;
 };
 
 __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int side = (int)blockIdx.x >= a.n_row, r = blockIdx.x - side * a.n_row, lane = threadIdx.x & 63;
+    for (int i = blockIdx.x * SM_THREADS + threadIdx.x; i < a.n_seq; i += gridDim.x * SM_THREADS) a.arrived[i] = 0;
     int row0 = -1, row1 = -1;                                                     // of the row's request: the first that ends behind it
     for (int base = 0; base < a.n_seq; base += 64) {
         const int s = min(base + lane, a.n_seq - 1), from = a.row_start[s], to = a.row_start[s + 1];
@@ -48,13 +54,12 @@ struct verify_left {
     float last_l;
     int last_i;
     bool infinite;
-    __device__ __forceinline__ verify_left(const float *temperature, const sample_cut *c, int r) {
-        const float temp = temperature ? temperature[r] : 1.0f;
-        const u64 last = c->last;
-        weigh = weigher_of(temp > 0.0f ? temp : 1.0f, c->top);                    // (the only token left of a greedy row has the largest logit: any temperature)
+    __device__ __forceinline__ verify_left(float temp, const sample_cut &c) {
+        const u64 last = c.last;
+        weigh = weigher_of(temp > 0.0f ? temp : 1.0f, c.top);                     // (the only token left of a greedy row has the largest logit: any temperature)
         last_l = last == ~0ull ? -INFINITY : logit_of(last);
         last_i = (int)(uint32_t)min(last & 0xFFFFFFFFull, 0x7FFFFFFFull);
-        infinite = c->infinite;
+        infinite = c.infinite;
     }
     __device__ __forceinline__ float clean(float v) const { return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v; }          // (a NaN is never left)
     __device__ __forceinline__ bool has(float v, int i) const { return (v > -INFINITY) & ((v > last_l) | ((v == last_l) & (i <= last_i))); }
@@ -69,17 +74,15 @@ struct verify_weights {
     int n, drafted;
     bool beyond_q, as_p;
     double one_p, one_q;
-    __device__ __forceinline__ verify_weights(const verify_args &a, int stop, bool at_end)
-        : p(a.target.temperature, a.cuts + stop, stop), q(a.draft.temperature, a.cuts + (at_end || !a.draft.logits ? 0 : a.n_row) + stop, stop) {
+    __device__ __forceinline__ verify_weights(const verify_args &a, int stop, bool at_end, int drafted_, float temp_p, const sample_cut &cut_p, float temp_q, const sample_cut &cut_q) : p(temp_p, cut_p), q(temp_q, cut_q) {
         beyond_q = !at_end && a.draft.logits;
         as_p = at_end;
         gp = (const float *)(a.target.logits + stop * a.target.stride);
         gq = beyond_q ? (const float *)(a.draft.logits + stop * a.draft.stride) : gp;
         n = a.target.n;
-        drafted = at_end ? -1 : a.drafted[stop];
-        one_p = 1.0 / (double)a.cuts[stop].total;
-        const u64 all_q = beyond_q ? a.cuts[(int64_t)a.n_row + stop].total : 0;
-        one_q = all_q ? 1.0 / (double)all_q : 0.0;
+        drafted = at_end ? -1 : drafted_;
+        one_p = 1.0 / (double)cut_p.total;
+        one_q = beyond_q && cut_q.total ? 1.0 / (double)cut_q.total : 0.0;
     }
     // of a token that p has, with the logits v (as p.clean() has it) and l
     __device__ __forceinline__ u64 operator()(float v, float l, int i) const {
@@ -94,10 +97,12 @@ struct verify_weights {
     // a weight takes some hundred instructions, and few tokens of many have one.
     template <class F> __device__ __forceinline__ void each(int from, int to, uint2 *list, F f) const {
         const int lane = threadIdx.x & 63;
-        for (int base = from; base < to; base += 256) {
-            float x[4];
+        float x[4], ahead[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = gp[min(base + 64 * j + lane, n - 1)];
+        for (int j = 0; j < 4; j++) ahead[j] = gp[min(from + 64 * j + lane, n - 1)];
+        for (int base = from; base < to; base += 256) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) { x[j] = ahead[j]; ahead[j] = gp[min(base + 256 + 64 * j + lane, n - 1)]; }
             uint32_t m = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -126,24 +131,24 @@ struct verify_weights {
     }
 };
 #define VF_PARTS 64
+#define VF_BLOCKS (VF_PARTS / 16)
 static __device__ __forceinline__ void verify_part(int n, int part, int &from, int &to) {
     const int size = (n + VF_PARTS - 1) / VF_PARTS;
     from = min(part * size, n); to = min(from + size, n);
 }
 
-// Where the drafts of a request end, and the weights of each part of that row, added up: a part by each wave
-__global__ __launch_bounds__(256) void verify_sum_kernel(verify_args a) {
-    __shared__ uint2 s_list[4][256];
-    const int request = blockIdx.x / (VF_PARTS / 4), part = blockIdx.x % (VF_PARTS / 4) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, wave = part & 3;
+// Four workgroups to a request.  Each finds where its drafts end.  Where the tokens that are left of that row are known, the first one draws; else each wave adds up the weights of a part of the row, and the
+// workgroup that is done last draws (a.arrived: zeroed by the launch before).
+__global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) {
+    __shared__ sample_shared s;
+    __shared__ uint2 s_list[16][256];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), request = blockIdx.x / VF_BLOCKS, block = blockIdx.x % VF_BLOCKS;
     const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
     int past = 0;                                                                 // rows that the requests before it have taken: where one of them went further, the launch before gave it these rows
     for (int i = lane; i < request; i += 64) past = max(past, a.row_start[i]);
     const bool sound = row0 >= 0 && row1 >= row0 && row1 <= a.n_row && !__any(past > row0);
     if (!sound && a.err) *a.err = 1;
-    if (!sound || row0 == row1) {
-        if (part == 0 && lane == 0) a.stops[request] = -1;
-        return;
-    }
+    if (!sound || row0 == row1) return;
     int stop = row1 - 1;
     for (int base = row0; base < row1 - 1; base += 64) {
         const int r = min(base + lane, row1 - 2);
@@ -153,23 +158,26 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(verify_args a) {
         if (not_taken) { stop = min(base + __ffsll(not_taken) - 1, row1 - 2); break; }
     }
     stop = __builtin_amdgcn_readfirstlane(stop);
-    if (part == 0 && lane == 0) a.stops[request] = stop;
-    if (!a.cuts[stop].total || a.cuts[stop].n_kept <= SM_KEPT) return;
-    const verify_weights weights(a, stop, stop == row1 - 1);
-    int from, to;
-    verify_part(weights.n, part, from, to);
-    const u64 sum = weights.sum(from, to, s_list[wave]);
-    if (lane == 0) a.sums[(int64_t)request * VF_PARTS + part] = sum;
-}
-
-__global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) {
-    __shared__ sample_shared s;
-    __shared__ uint2 s_list[16][256];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), request = blockIdx.x;
-    const int row0 = a.row_start[request], row1 = a.row_start[request + 1], stop = __builtin_amdgcn_readfirstlane(a.stops[request]);
-    if (stop < 0) return;                                                         // without rows, or rows that do not fit
-    const u64 c_total = a.cuts[stop].total;
-    const uint32_t n_kept = a.cuts[stop].n_kept;
+    // all that the draw wants of the row, requested together
+    const bool at_end = stop == row1 - 1;
+    const sample_cut cut_p = a.cuts[stop], cut_q = a.cuts[(at_end || !a.draft.logits ? 0 : (int64_t)a.n_row) + stop];
+    const float temp_p = a.target.temperature ? a.target.temperature[stop] : 1.0f, temp_q = a.draft.temperature ? a.draft.temperature[stop] : 1.0f, u = a.target.uniform[stop];
+    const int drafted = a.drafted[stop];
+    const u64 x = a.kept[(int64_t)stop * SM_KEPT + t], c_total = cut_p.total;     // (whatever lies there, where there are fewer)
+    const uint32_t n_kept = cut_p.n_kept;
+    const bool many = c_total && n_kept > SM_KEPT;
+    if (block && !many) return;
+    verify_weights weights(a, stop, at_end, drafted, temp_p, cut_p, temp_q, cut_q);
+    if (many) {
+        int from, to;
+        verify_part(weights.n, 16 * block + wave, from, to);
+        const u64 sum = weights.sum(from, to, s_list[wave]);
+        if (lane == 0) __hip_atomic_store(a.sums + (int64_t)request * VF_PARTS + 16 * block + wave, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (t == 0) s.bin = __hip_atomic_fetch_add(a.arrived + request, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (s.bin != VF_BLOCKS - 1) return;
+    }
     for (int r = row0 + t; r < row1; r += SM_THREADS) {
         if (r == stop) continue;
         a.tokens[r] = r < stop ? a.drafted[r] : -1;
@@ -180,15 +188,12 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
         if (!c_total) { a.tokens[stop] = -1; if (a.probs) a.probs[stop] = 0.0f; }
     }
     if (!c_total) return;                                                         // a row without a logit above -inf
-    verify_weights weights(a, stop, stop == row1 - 1);
-    const float u = a.target.uniform[stop];
     const auto drawn = [&](int i, float v) { a.tokens[stop] = i; if (a.probs) a.probs[stop] = (float)share_of_all(weights.p.weigh(v), c_total); };
     if (n_kept <= SM_KEPT) {
         // one token a thread
         const bool there = (uint32_t)t < n_kept;
-        const u64 x = there ? a.kept[(int64_t)stop * SM_KEPT + t] : 0;
         const float v = there ? logit_of(x) : -INFINITY;
-        const int i = (int)(uint32_t)x, range = i >> a.target.range_log2;
+        const int i = there ? (int)(uint32_t)x : 0, range = i >> a.target.range_log2;
         const float l = there && weights.beyond_q ? weights.gq[i] : 0.0f;
         s.mass[t] = 0;
         if (t == 0) s.n_list = 0;
@@ -215,7 +220,7 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
         }
         return;
     }
-    u64 sums = wave_scan(a.sums[(int64_t)request * VF_PARTS + lane]);
+    u64 sums = wave_scan(__hip_atomic_load(a.sums + (int64_t)request * VF_PARTS + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     if (!weights.as_p && !of_lane(sums, 63)) {
         weights.as_p = true;                                                      // as above: the sums once more, four parts by each wave
         for (int k = 0; k < VF_PARTS / 16; k++) {
@@ -266,7 +271,7 @@ extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits,
     if (rc) return rc;
     SPY_CHECK_ARG(!draft_logits || (draft_logits->data && draft_logits->ne[0] == logits->ne[0] && draft_logits->ne[1] == logits->ne[1]));
     const int64_t n_row = logits->ne[1], blocks = n_row * (draft_logits ? 2 : 1);
-    SPY_CHECK_ARG(blocks * SM_THREADS < (1ll << 32) && (int64_t)n_seq * VF_PARTS * 64 < (1ll << 32));
+    SPY_CHECK_ARG(blocks * SM_THREADS < (1ll << 32) && (int64_t)n_seq * VF_BLOCKS * SM_THREADS < (1ll << 32));
     if (scratch_bytes < verify_scratch(n_row, n_seq)) return SPY_HIP_ENOSPACE;
     SPY_CHECK_ARG(scratch && ((uintptr_t)scratch & 255) == 0);
     verify_args a;
@@ -274,16 +279,13 @@ extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits,
     a.draft = draft_logits ? sample_args_of(draft_logits, draft_param) : a.target;
     if (!draft_logits) a.draft.logits = nullptr;
     a.drafted = drafted; a.row_start = row_start; a.accept = accept; a.n_seq = n_seq; a.n_row = (int)n_row;
-    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.stops = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.err = spy_hip_err_flag_ptr();
+    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.arrived = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.err = spy_hip_err_flag_ptr();
     const size_t lds = sample_lds(a.target);
     rc = spy_raise_lds_limit((const void *)verify_cut_kernel, lds);
     if (rc) return rc;
     verify_cut_kernel<<<dim3((unsigned)blocks), dim3(SM_THREADS), lds, (hipStream_t)stream>>>(a);
     rc = SPY_LAUNCH_RC();
     if (rc) return rc;
-    verify_sum_kernel<<<dim3((unsigned)(n_seq * (VF_PARTS / 4))), dim3(256), 0, (hipStream_t)stream>>>(a);
-    rc = SPY_LAUNCH_RC();
-    if (rc) return rc;
-    verify_draw_kernel<<<dim3((unsigned)n_seq), dim3(SM_THREADS), 0, (hipStream_t)stream>>>(a);
+    verify_draw_kernel<<<dim3((unsigned)n_seq * VF_BLOCKS), dim3(SM_THREADS), 0, (hipStream_t)stream>>>(a);
     return SPY_LAUNCH_RC();
 }
