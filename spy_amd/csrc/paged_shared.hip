@@ -2,7 +2,8 @@
 #include "paged_shared.cuh"
 
 // A row and head of the output: D / 4 lanes, the heads of a wave of one row.  PARTS: so many waves of the workgroup share the pieces of the same heads.  Latency, and what the first launch wrote:
-// eight pieces of o are requested at a time, the first before the weights are worked out.
+// eight pieces of o (two by a wave alone) are requested at a time, the first before the weights are worked out.  A wave for four times the heads took
+// 16 us instead of 15 for 965 rows.
 template <int D, bool F32OUT, int PARTS> __global__ __launch_bounds__(256) void attn_shared_join_kernel(attn_more a, int waves) {
     constexpr int L = D / 4, HEADS = 64 / L, AHEAD = PARTS > 1 ? 8 : 2;                    // lanes to a head, heads to a wave
     __shared__ v4f s_v[4][64];
@@ -84,15 +85,15 @@ template <int D, bool F32OUT, int PARTS> __global__ __launch_bounds__(256) void 
 template <int D, bool F32OUT> static int attn_shared_join(const attn_more &a, hipStream_t st) {
     const int heads = 256 / D, waves = (a.G * a.group + heads - 1) / heads;        // heads of a wave; waves of a row
     const int64_t all = (int64_t)a.b.n_row * waves;
-    // Pieces that a row may be expected to have: those of chunks where the batch may bring them.  32 rows of 32 heads with 30 pieces each 14.5 us by a wave, XX by four; 965 rows with two 16 and 42.
+    // Pieces that a row may be expected to have: those of chunks where the batch may bring them.  32 rows of 32 heads with 30 pieces each 14.5 us by a wave, 6.6 by four; 965 rows with two 16 and 42.
     const int pieces = (a.common.chunk_blocks ? a.common.chunk_pieces : a.common.few_pieces) + (a.chunk_blocks ? a.chunk_pieces : a.few_pieces);
     if (pieces > 8 && all <= 4096) attn_shared_join_kernel<D, F32OUT, 4><<<dim3((unsigned)all), dim3(256), 0, st>>>(a, waves);
     else attn_shared_join_kernel<D, F32OUT, 1><<<dim3((unsigned)((all + 3) / 4)), dim3(256), 0, st>>>(a, waves);
     return SPY_LAUNCH_RC();
 }
 
-// Own keys as attn_make_plan shares them out; those in common the same way, with groups for sequences.
-#define CW 4
+// Own keys much as attn_make_plan shares them out; those in common the same way, with groups for sequences.  Chunks: a workgroup to a compute unit (64 requests behind four prompts of 8000 tokens, 32 behind one of
+// 20000 in 8 bits, and 965 rows behind 2000: 63, 43 and 86 us; two workgroups 72, 51 and 91: more pieces to write and to join); few rows three (61.0 us for the first; six: 63.1).
 struct shared_plan { attn_plan own, common; int64_t slots, own_slot; size_t ml_bytes, scratch; };
 static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *b, const spy_hip_paged_prefix *x, shared_plan &p) {
     SPY_CHECK_ARG(q && k_pages && q->ne[1] > 0 && q->ne[1] <= 65535 && q->ne[2] > 0 && q->ne[2] < (1 << 28));
@@ -114,7 +115,7 @@ static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = n_row * group / CHUNK_ROWS + count;
         a.chunk_tiles = each * count < all ? each * count : all;
         a.chunk_units = a.chunk_tiles * G;
-        const int64_t key_tiles = (keys + 63) / 64 + (&a == &p.own), n = (CW * cu / 4 + a.chunk_units - 1) / a.chunk_units;
+        const int64_t key_tiles = (keys + 63) / 64 + (&a == &p.own), n = (cu + a.chunk_units - 1) / a.chunk_units;
         a.chunk_split = n == 1 ? key_tiles : (key_tiles + n - 1) / n;
         if (a.chunk_split < 8) a.chunk_split = 8;
         a.chunk_pieces = (key_tiles + a.chunk_split - 1) / a.chunk_split;
