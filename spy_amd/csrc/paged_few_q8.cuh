@@ -9,8 +9,10 @@
 
 template <int D, int WAVES> struct few_q8_shared {
     static constexpr int K = 32 * D, V = 32 * D, KD = 2 * D, VD = 2 * D, TILE = K + V + KD + VD;       // bytes: rows of K, [half of the keys][dimension] of V^T, scales
+    static constexpr bool LEAN = D == 256;
+    static constexpr int RING = LEAN ? TILE + KD + VD : 2 * TILE, NEXT = LEAN ? KD + VD : TILE;        // of a wave; from one of what there are two of to the other
     union {
-        __attribute__((aligned(1024))) uint8_t ring[WAVES][2][TILE];
+        __attribute__((aligned(1024))) uint8_t ring[WAVES][RING];
         few_shared<D, WAVES> end;
     };
 };
@@ -64,7 +66,7 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
 
     // A row of K in LDS has its 16-byte pieces at their index xor swizzle(row), so that the 16 rows of an operand lie in different banks (they are keys 8 (i / 4) + 4 t + i % 4)
     const auto swizzle = [](int row) { return D == 256 ? (row & 3) | row >> 3 << 2 : D == 128 ? (row >> 1 & 1) | row >> 3 << 1 : row >> 3; };
-    const uint32_t lds = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.ring[wave][0]);
+    const uint32_t lds = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.ring[wave]);
     uint32_t koff[NI];                                                     // request i: 1024 / D rows, one after the other; from the first of the group of 16 on
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -78,22 +80,27 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
     const bool d_second = d_v ? d_j & 2 : 16 * d_j >= D;
     const uint32_t d_unit = d_v ? 2 : D / 16, d_step = d_v ? vs_g : ks_g;  // bytes of a position, of a page
     const uint8_t *const d_base = d_v ? vs + (uint64_t)(d_j >> 2) * vs_b + (d_j & 1) * 16 + (d_second ? 16 & pmask : 0) * 2 : ks + 16 * d_j % D + (d_second ? 16 & pmask : 0) * (D / 16);
-    const auto ask = [&](int kt, page_pair g, uint32_t buf) {              // buf: bytes of the buffer behind the first
+    const auto present = [&](uint32_t page) { return uniform(page < n_page ? page : 0); };
+    const auto ask_k = [&](int kt, page_pair g, uint32_t buf) {            // K and the scales.  buf: bytes of the buffer behind the first
         const int kb = begin + 32 * kt;
-        const uint32_t pg[2] = {uniform(g.first < n_page ? g.first : 0), uniform(g.second < n_page ? g.second : 0)};
+        const uint32_t pg[2] = {present(g.first), present(g.second)};
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int q = i * (1024 / D) / 16;                             // group of 16 keys
-            to_lds(uniform(kp + (uint64_t)pg[q] * kp_g + (uint64_t)((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds + buf + i * 1024), 1);
-        }
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int q = i / (D / 64), d = i % (D / 64) * 64;
-            to_lds(uniform(vp + (uint64_t)pg[q] * vp_g + ((kb + 16 * q) & pmask) + (uint64_t)d * vp_d), voff, uniform(lds + buf + lay::K + i * 1024), 1);
+            to_lds(uniform(kp + (uint64_t)pg[q] * kp_g + (uint64_t)((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds + (lay::LEAN ? 0 : buf) + i * 1024), 1);
         }
         if (lane < D / 4) to_lds(d_base + (uint64_t)(d_second ? pg[1] : pg[0]) * d_step + (kb & pmask) * d_unit, uniform(lds + buf + lay::K + lay::V), 1);
     };
-    constexpr int ASKED = 2 * NI + 1;
+    const auto ask_v = [&](int kt, page_pair g, uint32_t buf) {
+        const int kb = begin + 32 * kt;
+        const uint32_t pg[2] = {present(g.first), present(g.second)};
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int q = i / (D / 64), d = i % (D / 64) * 64;
+            to_lds(uniform(vp + (uint64_t)pg[q] * vp_g + ((kb + 16 * q) & pmask) + (uint64_t)d * vp_d), voff, uniform(lds + (lay::LEAN ? 0 : buf) + lay::K + i * 1024), 1);
+        }
+    };
+    constexpr int ASKED_K = NI + 1, ASKED_V = NI;
 
     const auto v_values = [&](int kt, page_pair g, int d) {                // as they lie in memory, for the walk that counts what is not finite
         const uint32_t page = quarter & 2 ? g.second : g.first;
@@ -117,17 +124,20 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
         if (first < stop) {
             pg = pages_of(first);
             pg1 = pages_of(first + WAVES);
-            ask(first, pg, 0);
-            if (first + WAVES < stop) ask(first + WAVES, pg1, lay::TILE);
+            ask_k(first, pg, 0);
+            ask_v(first, pg, 0);
+            if (!lay::LEAN && first + WAVES < stop) { ask_k(first + WAVES, pg1, lay::NEXT); ask_v(first + WAVES, pg1, lay::NEXT); }
         }
         uint32_t buf = 0;
         for (int kt = first; kt < stop; kt += WAVES) {
             const page_pair pg2 = pages_of(kt + 2 * WAVES);
             const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
             const bool vbad = (quarter & 2 ? pg.second : pg.first) >= n_page;
-            if (kt + WAVES < stop) landed_but<ASKED>();                    // this tile's requests are answered, the next one's need not be
+            const bool more = kt + WAVES < stop;
+            if constexpr (lay::LEAN) landed_but<ASKED_V>();                // K is there, V need not be
+            else if (more) landed_but<ASKED_K + ASKED_V>();                // this tile's requests are answered, the next one's need not be
             else landed_but<0>();
-            const uint8_t *const tile = sh.ring[wave][0] + buf;
+            const uint8_t *const scales = sh.ring[wave] + lay::K + lay::V + buf, *const tile = sh.ring[wave] + (lay::LEAN ? 0 : buf);
             const int row = 8 * (n >> 2) + (n & 3);
             const uint8_t *const krow = tile + row * D + (quarter & 1) * 8, *const vcol = tile + lay::K + (quarter >> 1) * (16 * D) + n * 16 + (quarter & 1) * 8;
             const int kpiece = ((quarter >> 1) ^ swizzle(row)) * 16;
@@ -135,7 +145,7 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
             k_scales dk[2];
             uint4 dv[D / 32];
 #pragma unroll
-            for (int t = 0; t < 2; t++) dk[t] = *(const k_scales *)(tile + lay::K + lay::V + (row + 4 * t) * (D / 16));
+            for (int t = 0; t < 2; t++) dk[t] = *(const k_scales *)(scales + (row + 4 * t) * (D / 16));
             const auto k_piece = [&](int t, int k) { return dequantized(*(const uint2 *)(krow + 4 * t * D + (kpiece ^ k * 32)), all_of(dk[t][k / 2] >> (16 * (k & 1)))); };
             const auto v_piece = [&](int d) { return bits(dequantized(*(const uint2 *)(vcol + 256 * d), halves(dv[d / 2]))); };
             v4f x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -144,7 +154,11 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
 #pragma unroll
                 for (int t = 0; t < 2; t++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_piece(t, k), fq[k], x[t], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < D / 32; d++) dv[d] = *(const uint4 *)(tile + lay::K + lay::V + lay::KD + d * 64 + quarter * 16);
+            for (int d = 0; d < D / 32; d++) dv[d] = *(const uint4 *)(scales + lay::KD + d * 64 + quarter * 16);
+            if constexpr (lay::LEAN) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // K is not read any more
+                if (more) ask_k(kt + WAVES, pg1, buf ^ lay::NEXT);
+            }
             float e[8];                                                    // of this lane's query and keys vk ..
 #pragma unroll
             for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * c;
@@ -180,6 +194,10 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
                 p2[j] = (_Float16)(e[j] - (float)p[j]);
             }
             l = l * shrink + sum;
+            if constexpr (lay::LEAN) {
+                if (more) landed_but<ASKED_K>();                           // V
+                else landed_but<0>();
+            }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 uint4 w = v_piece(d);
@@ -189,8 +207,9 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w), p2, o[d], 0, 0, 0);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // nothing is read from this buffer any more
-            if (kt + 2 * WAVES < stop) ask(kt + 2 * WAVES, pg2, buf);
-            buf ^= lay::TILE;
+            if constexpr (lay::LEAN) { if (more) ask_v(kt + WAVES, pg1, 0); }
+            else if (kt + 2 * WAVES < stop) { ask_k(kt + 2 * WAVES, pg2, buf); ask_v(kt + 2 * WAVES, pg2, buf); }
+            buf ^= lay::NEXT;
             pg = pg1; pg1 = pg2;
         }
     };

@@ -11,7 +11,7 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
     if constexpr (MODE & ATTN_Q8) attn_few_q8<D, F32OUT, WAVES, MODE>(a, sh, block, common);
     else attn_few<D, F32OUT, WAVES, MODE>(a, sh, block, common);
 }
-template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_shared_few_kernel(attn_more a) {
+template <int D, bool F32OUT, int MODE> __global__ __launch_bounds__(256, D == 256 && !(MODE & ATTN_Q8) ? 1 : 2) void attn_shared_few_kernel(attn_more a) {
     __shared__ shared_few<D, 4, MODE> sh;
     const int block = blockIdx.x;
     const bool common = block < a.common.few_blocks;
