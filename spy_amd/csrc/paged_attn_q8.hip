@@ -1,7 +1,7 @@
 // Attention over pages of 8 bits: paged_attn.cuh with fp16(d * q) for the elements of K and V, so that its results are those of pages that hold these as fp16, bit for bit.
 #include "paged_few_q8.cuh"
 
-template <int D, bool F32OUT> __global__ __launch_bounds__(256, 2) void attn_q8_few_kernel(attn_more a) {
+template <int D, bool F32OUT> __global__ __launch_bounds__(256, 512 / D > 4 ? 4 : 512 / D > 2 ? 3 : 2) void attn_q8_few_kernel(attn_more a) {
     __shared__ few_q8_shared<D, 4> sh;
     attn_few_q8<D, F32OUT, 4, ATTN_Q8>(a, sh, blockIdx.x);
 }

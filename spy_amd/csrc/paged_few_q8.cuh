@@ -1,18 +1,18 @@
 // Tiles of 16 rows over pages of 8 bits: attn_few of paged_attn.cuh with fp16(d * q) for the elements of K and V, the same sums in the same order.
 //
 // A tile of 32 keys goes from memory to LDS as it lies there, by 16 bytes a lane of rows that follow each other, and from LDS to the operands of the matrix instruction: an operand takes 8 bytes from
-// each of 16 rows, and loads of such pieces from memory, which the vector cache takes a few bytes at a time, took as long as all else (157 us for 64 requests of up to 8000 tokens, 32 heads to 8, 128 wide).
-// Each wave has a ring of two tiles of its own: one is computed with while the next one comes, and no wave waits for another before the end.
+// each of 16 rows, and loads of such pieces from memory, which the vector cache takes a few bytes at a time (744 lookups a tile), took as long as all else (64 requests of up to 8000 tokens, 32 heads to 8, 128 wide:
+// 171 us; by way of LDS 144).  Each wave has a tile of its own and waits for no other before the end; the next tile's K is requested when this one's is read, its V when this one's is.
+// Bound by memory, 4.65 TB/s there; one request of 4096 tokens and 32 heads 15.7 us with the second launch, of which 11 are the chain from lengths to the last sum.  With two whole tiles for a wave, 16.2 and
+// 143 us, and 256 wide, where only one wave has room on a SIMD then, 177 us for 32 requests instead of 154 (64 wide, 24 heads to 8: 82.7 and 79.4).
 #pragma once
 
 #include "paged_attn.cuh"
 
 template <int D, int WAVES> struct few_q8_shared {
-    static constexpr int K = 32 * D, V = 32 * D, KD = 2 * D, VD = 2 * D, TILE = K + V + KD + VD;       // bytes: rows of K, [half of the keys][dimension] of V^T, scales
-    static constexpr bool LEAN = D == 256;
-    static constexpr int RING = LEAN ? TILE + KD + VD : 2 * TILE, NEXT = LEAN ? KD + VD : TILE;        // of a wave; from one of what there are two of to the other
+    static constexpr int K = 32 * D, V = 32 * D, KD = 2 * D, DS = 4 * D;                              // bytes: rows of K, [half of the keys][dimension] of V^T; scales: of K, of both
     union {
-        __attribute__((aligned(1024))) uint8_t ring[WAVES][RING];
+        __attribute__((aligned(1024))) uint8_t tile[WAVES][K + V + 2 * DS];                           // (the scales: this tile's and the next one's)
         few_shared<D, WAVES> end;
     };
 };
@@ -66,7 +66,7 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
 
     // A row of K in LDS has its 16-byte pieces at their index xor swizzle(row), so that the 16 rows of an operand lie in different banks (they are keys 8 (i / 4) + 4 t + i % 4)
     const auto swizzle = [](int row) { return D == 256 ? (row & 3) | row >> 3 << 2 : D == 128 ? (row >> 1 & 1) | row >> 3 << 1 : row >> 3; };
-    const uint32_t lds = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.ring[wave]);
+    const uint32_t lds = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sh.tile[wave]);
     uint32_t koff[NI];                                                     // request i: 1024 / D rows, one after the other; from the first of the group of 16 on
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -81,23 +81,23 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
     const uint32_t d_unit = d_v ? 2 : D / 16, d_step = d_v ? vs_g : ks_g;  // bytes of a position, of a page
     const uint8_t *const d_base = d_v ? vs + (uint64_t)(d_j >> 2) * vs_b + (d_j & 1) * 16 + (d_second ? 16 & pmask : 0) * 2 : ks + 16 * d_j % D + (d_second ? 16 & pmask : 0) * (D / 16);
     const auto present = [&](uint32_t page) { return uniform(page < n_page ? page : 0); };
-    const auto ask_k = [&](int kt, page_pair g, uint32_t buf) {            // K and the scales.  buf: bytes of the buffer behind the first
+    const auto ask_k = [&](int kt, page_pair g, uint32_t buf) {            // K, and the scales to the buffer `buf` bytes behind the first
         const int kb = begin + 32 * kt;
         const uint32_t pg[2] = {present(g.first), present(g.second)};
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int q = i * (1024 / D) / 16;                             // group of 16 keys
-            to_lds(uniform(kp + (uint64_t)pg[q] * kp_g + (uint64_t)((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds + (lay::LEAN ? 0 : buf) + i * 1024), 1);
+            to_lds(uniform(kp + (uint64_t)pg[q] * kp_g + (uint64_t)((kb + 16 * q) & pmask) * kp_p), koff[i], uniform(lds + i * 1024), 1);
         }
         if (lane < D / 4) to_lds(d_base + (uint64_t)(d_second ? pg[1] : pg[0]) * d_step + (kb & pmask) * d_unit, uniform(lds + buf + lay::K + lay::V), 1);
     };
-    const auto ask_v = [&](int kt, page_pair g, uint32_t buf) {
+    const auto ask_v = [&](int kt, page_pair g) {
         const int kb = begin + 32 * kt;
         const uint32_t pg[2] = {present(g.first), present(g.second)};
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int q = i / (D / 64), d = i % (D / 64) * 64;
-            to_lds(uniform(vp + (uint64_t)pg[q] * vp_g + ((kb + 16 * q) & pmask) + (uint64_t)d * vp_d), voff, uniform(lds + (lay::LEAN ? 0 : buf) + lay::K + i * 1024), 1);
+            to_lds(uniform(vp + (uint64_t)pg[q] * vp_g + ((kb + 16 * q) & pmask) + (uint64_t)d * vp_d), voff, uniform(lds + lay::K + i * 1024), 1);
         }
     };
     constexpr int ASKED_K = NI + 1, ASKED_V = NI;
@@ -120,24 +120,20 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
         m = -INFINITY; l = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = v4f{0, 0, 0, 0};
-        page_pair pg = {0, 0}, pg1 = {0, 0};
+        page_pair pg = {0, 0};
         if (first < stop) {
             pg = pages_of(first);
-            pg1 = pages_of(first + WAVES);
             ask_k(first, pg, 0);
-            ask_v(first, pg, 0);
-            if (!lay::LEAN && first + WAVES < stop) { ask_k(first + WAVES, pg1, lay::NEXT); ask_v(first + WAVES, pg1, lay::NEXT); }
+            ask_v(first, pg);
         }
         uint32_t buf = 0;
         for (int kt = first; kt < stop; kt += WAVES) {
-            const page_pair pg2 = pages_of(kt + 2 * WAVES);
+            const page_pair next = pages_of(kt + WAVES);
             const int kb = begin + 32 * kt, vk = kb + 8 * quarter;
             const bool vbad = (quarter & 2 ? pg.second : pg.first) >= n_page;
             const bool more = kt + WAVES < stop;
-            if constexpr (lay::LEAN) landed_but<ASKED_V>();                // K is there, V need not be
-            else if (more) landed_but<ASKED_K + ASKED_V>();                // this tile's requests are answered, the next one's need not be
-            else landed_but<0>();
-            const uint8_t *const scales = sh.ring[wave] + lay::K + lay::V + buf, *const tile = sh.ring[wave] + (lay::LEAN ? 0 : buf);
+            landed_but<ASKED_V>();                                         // K is there, V need not be
+            const uint8_t *const tile = sh.tile[wave], *const scales = tile + lay::K + lay::V + buf;
             const int row = 8 * (n >> 2) + (n & 3);
             const uint8_t *const krow = tile + row * D + (quarter & 1) * 8, *const vcol = tile + lay::K + (quarter >> 1) * (16 * D) + n * 16 + (quarter & 1) * 8;
             const int kpiece = ((quarter >> 1) ^ swizzle(row)) * 16;
@@ -155,10 +151,8 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
                 for (int t = 0; t < 2; t++) x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_piece(t, k), fq[k], x[t], 0, 0, 0);
 #pragma unroll
             for (int d = 0; d < D / 32; d++) dv[d] = *(const uint4 *)(scales + lay::KD + d * 64 + quarter * 16);
-            if constexpr (lay::LEAN) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // K is not read any more
-                if (more) ask_k(kt + WAVES, pg1, buf ^ lay::NEXT);
-            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // K is not read any more
+            if (more) ask_k(kt + WAVES, next, buf ^ lay::DS);
             float e[8];                                                    // of this lane's query and keys vk ..
 #pragma unroll
             for (int j = 0; j < 8; j++) e[j] = x[j >> 2][j & 3] * c;
@@ -194,10 +188,8 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
                 p2[j] = (_Float16)(e[j] - (float)p[j]);
             }
             l = l * shrink + sum;
-            if constexpr (lay::LEAN) {
-                if (more) landed_but<ASKED_K>();                           // V
-                else landed_but<0>();
-            }
+            if (more) landed_but<ASKED_K>();                               // V
+            else landed_but<0>();
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 uint4 w = v_piece(d);
@@ -206,11 +198,10 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w), p, o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(w), p2, o[d], 0, 0, 0);
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // nothing is read from this buffer any more
-            if constexpr (lay::LEAN) { if (more) ask_v(kt + WAVES, pg1, 0); }
-            else if (kt + 2 * WAVES < stop) { ask_k(kt + 2 * WAVES, pg2, buf); ask_v(kt + 2 * WAVES, pg2, buf); }
-            buf ^= lay::NEXT;
-            pg = pg1; pg1 = pg2;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // nor V
+            if (more) ask_v(kt + WAVES, next);
+            buf ^= lay::DS;
+            pg = next;
         }
     };
 #pragma unroll
@@ -246,6 +237,6 @@ template <int D, bool F32OUT, int WAVES, int MODE> static __device__ __forceinli
             }
         }
     }
-    __syncthreads();                                                       // the rings are done with
+    __syncthreads();                                                       // the tiles are done with
     few_end<D, F32OUT, WAVES, MODE>(a, sh.end, sq, rows, head, unit, piece, whole, common, m, l, o);
 }
