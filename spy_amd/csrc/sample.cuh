@@ -8,6 +8,7 @@
 //   else: a histogram of the tokens over their distance to the maximum, with a count and a sum of weights in every bin, says in which bin a setting cuts; the bin's
 //     tokens make the list, through finer histograms of X where they are too many.
 // Weights are integers, multiples of 2^-44 of the largest: sums of them are the same in any order, and exact.
+// CUT (sample_verify.hip): what the settings leave is wanted instead of a draw; the sums then come from the bins, and no weight of what lies before the cut is worked out twice.
 // One workgroup per row, which keeps 32768 logits in LDS at a time.  Measured for one row of 32000, and 64 in brackets: greedy 5.5 us (6.1), temperature alone 9.9 (10.6), top_k 40
 // with top_p and min_p 10.2 (11.6), top_k 500 with top_p 17 (18), top_p alone 21 (24), top_k 5000 24 (26), with top_p 28 (30): latency, up to some forty barriers with a
 // few dependent LDS accesses between them, and the slowest row of a batch decides; 256 rows of 100003 with top_p alone 81 us: vector instructions, since a weight of every logit is worked out for the sums by
