@@ -6,7 +6,7 @@
 // they are 1024 at most.  Second launch: four workgroups for each request find the row where its drafts end and draw there, one of them alone where it has those tokens.  p and q are weights over
 // their sums, in 64 bits; p - q as multiples of 2^-60, so that sums of it are exact in any order, and what comes out is the same each time.
 //
-// Latency and vector instructions: the first launch reads each row once from memory (verify of 32 requests with 1 to 6 rows of 32000 and a drafter's: 37 us, 24.6 of them here), and where top_p alone is set it
+// Latency and vector instructions: the first launch reads each row once from memory (verify of 32 requests with 1 to 6 rows of 32000 and a drafter's: 37.6 us, 24.6 of them here), and where top_p alone is set it
 // works out every weight: 160 rows of 100003 by as many workgroups 55 us, 12 for the reads, 24 for the weights (20 instructions a token beside an addition in LDS), 17 for the bin's tokens.  The
 // second is a chain of dependent reads (one request: 6 us) and, where more tokens are left, one pass over the row: 18 us for 64 requests of 100003.  One request with 5 rows of 32000: 21 us in all.  Taking the
 // weights of tokens that are not left as well took 102 us for the large case; three launches, the parts' sums one of their own, 0.3 to 0.8 more than two.
@@ -26,6 +26,7 @@ struct verify_args {
     u64 *kept;                           // of the target's rows: SM_KEPT each
     u64 *sums;                           // of the requests: VF_PARTS each
     int32_t *arrived;                    // of the requests: workgroups that have added up their parts
+    int32_t *owner;                      // of the target's rows: the request that it was looked at for, or -1
     int *err;
 };
 
@@ -33,7 +34,7 @@ __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int side = (int)blockIdx.x >= a.n_row, r = blockIdx.x - side * a.n_row, lane = threadIdx.x & 63;
     for (int i = blockIdx.x * SM_THREADS + threadIdx.x; i < a.n_seq; i += gridDim.x * SM_THREADS) a.arrived[i] = 0;
-    int row0 = -1, row1 = -1;                                                     // of the row's request: the first that ends behind it
+    int row0 = -1, row1 = -1, owner = -1;                                         // the row's request: the first that ends behind it
     for (int base = 0; base < a.n_seq; base += 64) {
         const int s = min(base + lane, a.n_seq - 1), from = a.row_start[s], to = a.row_start[s + 1];
         const unsigned long long past = __ballot(base + lane < a.n_seq && to > r);
@@ -41,9 +42,11 @@ __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
         const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
         row0 = __builtin_amdgcn_readlane(from, at);
         row1 = __builtin_amdgcn_readlane(to, at);
+        owner = row0 >= 0 && r >= row0 && row1 <= a.n_row ? base + at : -1;
         break;
     }
-    if (row0 < 0 || r < row0 || row1 > a.n_row || (side && r == row1 - 1)) return;
+    if (!side && threadIdx.x == 0) a.owner[r] = owner;
+    if (owner < 0 || (side && r == row1 - 1)) return;
     const int d = r < row1 - 1 ? a.drafted[r] : -1;
     sample_row_of<true>(side ? a.draft : a.target, smem, r, d, a.cuts + side * (int64_t)a.n_row + r, side ? nullptr : a.kept + (int64_t)r * SM_KEPT);
 }
@@ -144,11 +147,9 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
     __shared__ uint2 s_list[16][256];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), request = blockIdx.x / VF_BLOCKS, block = blockIdx.x % VF_BLOCKS;
     const int row0 = a.row_start[request], row1 = a.row_start[request + 1];
-    int past = 0;                                                                 // rows that the requests before it have taken: where one of them went further, the launch before gave it these rows
-    for (int i = lane; i < request; i += 64) past = max(past, a.row_start[i]);
-    const bool sound = row0 >= 0 && row1 >= row0 && row1 <= a.n_row && !__any(past > row0);
-    if (!sound && a.err) *a.err = 1;
-    if (!sound || row0 == row1) return;
+    if (row0 < 0 || row1 < row0 || row1 > a.n_row) { if (a.err) *a.err = 1; return; }
+    if (row0 == row1) return;
+    const int owner = a.owner[min(row0 + lane, row1 - 1)];                        // (asked for here, looked at below)
     int stop = row1 - 1;
     for (int base = row0; base < row1 - 1; base += 64) {
         const int r = min(base + lane, row1 - 2);
@@ -158,6 +159,10 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
         if (not_taken) { stop = min(base + __ffsll(not_taken) - 1, row1 - 2); break; }
     }
     stop = __builtin_amdgcn_readfirstlane(stop);
+    // rows that one of the requests before it goes further than are that one's
+    bool taken = __any(owner != request);
+    for (int base = row0 + 64; base < row1; base += 64) taken |= __any(a.owner[min(base + lane, row1 - 1)] != request);
+    if (taken) { if (a.err) *a.err = 1; return; }
     // all that the draw wants of the row, requested together
     const bool at_end = stop == row1 - 1;
     const sample_cut cut_p = a.cuts[stop], cut_q = a.cuts[(at_end || !a.draft.logits ? 0 : (int64_t)a.n_row) + stop];
@@ -254,7 +259,7 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
 }
 
 static inline size_t verify_cuts(int64_t n_row) { return ((size_t)n_row * 2 * sizeof(sample_cut) + 255) / 256 * 256; }
-static inline size_t verify_scratch(int64_t n_row, int64_t n_seq) { return verify_cuts(n_row) + (size_t)n_row * SM_KEPT * 8 + (size_t)n_seq * (VF_PARTS * 8 + 4); }
+static inline size_t verify_scratch(int64_t n_row, int64_t n_seq) { return verify_cuts(n_row) + (size_t)n_row * (SM_KEPT * 8 + 4) + (size_t)n_seq * (VF_PARTS * 8 + 4); }
 extern "C" size_t spy_hip_sample_verify_scratch_size(const spy_hip_tensor *logits, int32_t n_seq) {
     return logits && n_seq > 0 && logits->ne[1] > 0 && logits->ne[1] < (1 << 22) ? verify_scratch(logits->ne[1], n_seq) : 0;
 }
@@ -279,7 +284,7 @@ extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits,
     a.draft = draft_logits ? sample_args_of(draft_logits, draft_param) : a.target;
     if (!draft_logits) a.draft.logits = nullptr;
     a.drafted = drafted; a.row_start = row_start; a.accept = accept; a.n_seq = n_seq; a.n_row = (int)n_row;
-    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.arrived = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.err = spy_hip_err_flag_ptr();
+    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.arrived = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.owner = a.arrived + n_seq; a.err = spy_hip_err_flag_ptr();
     const size_t lds = sample_lds(a.target);
     rc = spy_raise_lds_limit((const void *)verify_cut_kernel, lds);
     if (rc) return rc;
