@@ -507,7 +507,9 @@ template <int D> struct chunk_group { __attribute__((aligned(1024))) uint8_t k[2
 template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared { chunk_group<D> group[GROUPS]; int unbounded; };
 template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared_q8 : chunk_shared<D, GROUPS> { __attribute__((aligned(16))) uint8_t scales[4 * GROUPS][D * 4]; };      // of V^T, a wave's own copy
 
-// Q8: a tile's whole numbers come to registers two tiles ahead and go to LDS as fp16 values one tile ahead, beside the matrix instructions of the scores, which leave the vector units time for it.
+// Q8: a tile's whole numbers come to registers two tiles ahead and go to LDS as fp16 values one tile ahead, beside the matrix instructions of the scores, which leave the vector units time for it (512 tokens on 7680, 32 heads
+// to 8, 128 wide: 106 us; beside the products of their own tile 110 to 113).  The registers that takes are those of operands asked for ahead, half as many as with fp16 pages: as many, 256-wide heads keep 48 registers in memory
+// (512 tokens on 3584, 16 heads to 8: 99 us instead of 84), and 128-wide ones are no faster (106.8).
 template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D), class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false) {
     constexpr bool Q8 = MODE & ATTN_Q8, SHARED = MODE & ATTN_SHARED;
     constexpr int ES = Q8 ? 1 : 2;                                         // bytes of an element in the pages
@@ -659,9 +661,10 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
         asm volatile("" : "+v"(k_at), "+v"(v_at));                         // (addresses once more for every tile: the compiler would keep all of them, in registers that it has not)
         const auto v_piece = [&](int d, int k) { return *(const uint4 *)(sh.v[buf] + d * 4096 + (v_at ^ k * 32)); };
         v16f x[2] = {{0}, {0}};
-        uint4 w[2][DT];
+        constexpr int WB = Q8 ? 1 : 2;                                     // steps of V that are asked for ahead
+        uint4 w[WB][DT];
         {
-            constexpr int AHEAD = KS < 8 ? KS : 8;
+            constexpr int AHEAD = Q8 ? 4 : KS < 8 ? KS : 8;
             v8h fk[AHEAD];
             const auto k_piece = [&](int i) { return *(const v8h *)(sh.k[buf] + (i / KS) * 64 * D + (k_at ^ (i % KS) * 32)); };
 #pragma unroll
@@ -671,13 +674,13 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
             for (int i = 0; i < 2 * KS; i++) {
                 x[i / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk[i % AHEAD], fq[i % KS], x[i / KS], 0, 0, 0);
                 if (i + AHEAD < 2 * KS) fk[i % AHEAD] = k_piece(i + AHEAD);
-                else if (i + AHEAD < 2 * KS + 2 * DT) w[(i + AHEAD - 2 * KS) / DT][(i + AHEAD - 2 * KS) % DT] = v_piece((i + AHEAD - 2 * KS) % DT, (i + AHEAD - 2 * KS) / DT);
+                else if (i + AHEAD < 2 * KS + WB * DT) w[(i + AHEAD - 2 * KS) / DT][(i + AHEAD - 2 * KS) % DT] = v_piece((i + AHEAD - 2 * KS) % DT, (i + AHEAD - 2 * KS) / DT);
                 if (!Q8 && i % 4 == 0) ask_k(kb + 64 * GROUPS, next, (buf ^ 1) * BUF, more, i / 4);        // the next tile's, one at a time: all at once, they take 1000 cycles to issue
                 if (Q8 && i % 2 == 1) unpack_piece(i / 2, buf ^ 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int i = AHEAD; i < 2 * DT; i++) w[i / DT][i % DT] = v_piece(i % DT, i / DT);
+            for (int i = AHEAD; i < WB * DT; i++) w[i / DT][i % DT] = v_piece(i % DT, i / DT);
         }
         if constexpr (Q8) if (kt + 2 * GROUPS < stop) ask_raw(kb + 128 * GROUPS, next);
         // register 8 s + j of tile t: key 32 t + 16 s + 8 half + j.  This lane's query sees register i's where lies(i, first) holds, first: the register 0's from lo on
@@ -738,9 +741,9 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
             }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p, o[d], 0, 0, 0);
-                if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k & 1][d]), p2, o[d], 0, 0, 0);
-                if (k < 2) w[k & 1][d] = v_piece(d, k + 2);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k % WB][d]), p, o[d], 0, 0, 0);
+                if (F32OUT) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(w[k % WB][d]), p2, o[d], 0, 0, 0);
+                if (k + WB < 4) w[k % WB][d] = v_piece(d, k + WB);
                 if (!Q8 && (k * DT + d) % 4 == 0) ask_v(v_from, (buf ^ 1) * BUF, more, (k * DT + d) / 4);
                 __builtin_amdgcn_sched_barrier(0);
             }

@@ -1,6 +1,6 @@
 // Attention over pages of 8 bits: paged_attn.cuh with fp16(d * q) for the elements of K and V, so that its results are those of pages that hold these as fp16, bit for bit.
 // Few rows: paged_few_q8.cuh, bound by memory.  Chunks: attn_chunk of paged_attn.cuh, bound by instructions, with 14 vector instructions to 8 elements on top of what fp16 pages take: 512 tokens on 7680, 32 heads
-// to 8, 128 wide 108 us (fp16 pages: 88), F32 out 133 (112); the cache is half the bytes, which matters for few rows alone.
+// to 8, 128 wide 106 us (fp16 pages: 88), F32 out 128 (112); the cache is half the bytes, which matters for few rows alone.
 #include "paged_few_q8.cuh"
 
 // waves on a SIMD that the tiles in LDS, and the registers, leave room for (128 wide: 131 registers; four waves with 128 took 146.7 us instead of 144.7 for the 64 requests)
