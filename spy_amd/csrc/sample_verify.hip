@@ -284,7 +284,8 @@ extern "C" int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits,
     a.draft = draft_logits ? sample_args_of(draft_logits, draft_param) : a.target;
     if (!draft_logits) a.draft.logits = nullptr;
     a.drafted = drafted; a.row_start = row_start; a.accept = accept; a.n_seq = n_seq; a.n_row = (int)n_row;
-    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.arrived = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.owner = a.arrived + n_seq; a.err = spy_hip_err_flag_ptr();
+    a.tokens = tokens; a.accepted = accepted; a.probs = probs; a.err = spy_hip_err_flag_ptr();
+    a.cuts = (sample_cut *)scratch; a.kept = (u64 *)((uint8_t *)scratch + verify_cuts(n_row)); a.sums = a.kept + n_row * SM_KEPT; a.arrived = (int32_t *)(a.sums + (int64_t)n_seq * VF_PARTS); a.owner = a.arrived + n_seq;
     const size_t lds = sample_lds(a.target);
     rc = spy_raise_lds_limit((const void *)verify_cut_kernel, lds);
     if (rc) return rc;
