@@ -105,11 +105,18 @@ static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *
     const int64_t G = k_pages->ne[2], H = q->ne[1], hd = k_pages->ne[0], n_row = q->ne[2];
     SPY_CHECK_ARG(G <= 65535 && H % G == 0);
     const int64_t group = H / G, cu = spy_num_cu();
+    // Every row has places for the pieces of either kind of tile: those of few rows, of which there may be many, are no more than take 128 MB, or four
+    // (2048 rows of 32 heads on up to 30000 keys: 0.27 GB of scratch instead of 1.6; a chunk of 2048 tokens and eight single ones behind 4000, 32 heads to 8: 270 us instead of 280)
+    const int64_t fit = (128ll << 20) / (n_row * H * hd * 4), room = fit < 4 ? 4 : fit;
     const auto share = [&](attn_plan &a, int64_t count, int64_t rows, int64_t keys) {
         const int64_t most = (rows < n_row ? rows : n_row) * group, tiles = ((keys + 31) / 32 + 1);
         a.few = FEW_ROWS;
         a.few_units = count * G;
         attn_share(a.few_units, tiles, 3 * cu, 8, a.few_split, a.few_pieces);
+        if (a.few_pieces > room) {
+            a.few_split = ((tiles + room - 1) / room + 3) / 4 * 4;
+            a.few_pieces = (tiles + a.few_split - 1) / a.few_split;
+        }
         a.chunk_tiles = a.chunk_units = 0; a.chunk_split = a.chunk_pieces = 1;
         if (most <= FEW_ROWS) return;
         const int64_t each = (most + CHUNK_ROWS - 1) / CHUNK_ROWS, all = n_row * group / CHUNK_ROWS + count;
