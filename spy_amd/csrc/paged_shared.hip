@@ -2,10 +2,11 @@
 #include "paged_shared.cuh"
 
 // A row and head of the output: D / 4 lanes, the heads of a wave of one row.  PARTS: so many waves of the workgroup share the pieces of the same heads.  Latency, and what the first launch wrote:
-// eight pieces of o (two by a wave alone) are requested at a time, the first before the weights are worked out.  A wave for four times the heads took
+// up to eight pieces of o (two by a wave alone) are requested at a time, the first before the weights are worked out.  A wave for four times the heads took
 // 16 us instead of 15 for 965 rows.
 template <int D, bool F32OUT, int PARTS> __global__ __launch_bounds__(256) void attn_shared_join_kernel(attn_more a, int waves) {
-    constexpr int L = D / 4, HEADS = 64 / L, AHEAD = PARTS > 1 ? 8 : 2;                    // lanes to a head, heads to a wave
+    constexpr int L = D / 4, HEADS = 64 / L, AHEAD = PARTS == 1 ? 2 : L / PARTS < 8 ? L / PARTS : 8;        // lanes to a head, heads to a wave, pieces requested at a time
+    static_assert(L % (PARTS * AHEAD) == 0);                               // whole turns for the weights that the lanes of a head have
     __shared__ v4f s_v[4][64];
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % PARTS, wave = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) / PARTS), lane = threadIdx.x & 63;
     const int n_head = a.G * a.group, row = wave / waves, h = (wave - row * waves) * HEADS + lane / L, at = lane % L, hq = min(h, n_head - 1);

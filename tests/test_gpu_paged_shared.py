@@ -24,6 +24,11 @@ CASES = [
     ([(1, 3000)], [0, 1], [2999], 10, 2, 128, 256),              # a group of one
     ([(300, 700), (200, 600)], [0, 2], [400], 5, 5, 128, 1024),
     ([(0, 90), (1, 100), (0, 95)], [0, 3], [90], 4, 2, 128, 16),
+    # more pieces of a row than there are lanes to a head
+    ([(1, 6500), (1, 6450)], [0, 2], [6300], 16, 2, 64, 128),
+    ([(1, 11000), (3, 10900)], [0, 2], [10500], 4, 2, 128, 64),
+    ([(1, 19000), (1, 18900)], [0, 2], [18800], 2, 1, 256, 256),
+    ([(2, 9000), (1, 8000), (1, 700)], [0, 2], [300], 8, 1, 64, 16),
 ]
 
 
