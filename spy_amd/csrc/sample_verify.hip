@@ -10,6 +10,7 @@
 // works out every weight: 160 rows of 100003 by as many workgroups 55 us, 12 for the reads, 24 for the weights (20 instructions a token beside an addition in LDS), 17 for the bin's tokens.  The
 // second is a chain of dependent reads (one request: 6 us) and, where more tokens are left, one pass over the row: 18 us for 64 requests of 100003.  One request with 5 rows of 32000: 21 us in all.  Taking the
 // weights of tokens that are not left as well took 102 us for the large case; three launches, the parts' sums one of their own, 0.3 to 0.8 more than two.
+#include "launch_index.h"
 #include "paged.cuh"
 #include "sample.cuh"
 
@@ -33,7 +34,7 @@ struct verify_args {
 __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int side = (int)blockIdx.x >= a.n_row, r = blockIdx.x - side * a.n_row, lane = threadIdx.x & 63;
-    for (int i = blockIdx.x * SM_THREADS + threadIdx.x; i < a.n_seq; i += gridDim.x * SM_THREADS) a.arrived[i] = 0;
+    for (int64_t i = launch_first(blockIdx.x, SM_THREADS, threadIdx.x); i < a.n_seq; i += launch_step(gridDim.x, SM_THREADS)) a.arrived[i] = 0;
     int row0 = -1, row1 = -1, owner = -1;                                         // the row's request: the first that ends behind it
     for (int base = 0; base < a.n_seq; base += 64) {
         const int s = min(base + lane, a.n_seq - 1), from = a.row_start[s], to = a.row_start[s + 1];
