@@ -178,9 +178,13 @@ __global__ __launch_bounds__(SM_THREADS) void verify_draw_kernel(verify_args a) 
         int from, to;
         verify_part(weights.n, 16 * block + wave, from, to);
         const u64 sum = weights.sum(from, to, s_list[wave]);
-        if (lane == 0) __hip_atomic_store(a.sums + (int64_t)request * VF_PARTS + 16 * block + wave, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (lane == 0) s.part[wave] = sum;
         __syncthreads();
-        if (t == 0) s.bin = __hip_atomic_fetch_add(a.arrived + request, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        // One wave stores the sums of all and counts the workgroup: a release waits for its own wave's stores, and a barrier for nobody's
+        if (wave == 0) {
+            if (lane < 16) __hip_atomic_store(a.sums + (int64_t)request * VF_PARTS + 16 * block + lane, s.part[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lane == 0) s.bin = __hip_atomic_fetch_add(a.arrived + request, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        }
         __syncthreads();
         if (s.bin != VF_BLOCKS - 1) return;
     }

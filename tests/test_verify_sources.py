@@ -1,6 +1,7 @@
 """What the results of the verification of drafts cannot show, or only at sizes that a test has no time for: no GPU needed."""
 import os
 import re
+import shutil
 import subprocess
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -16,3 +17,19 @@ def test_requests_are_shared_out_in_64_bits(tmp_path):
     kernel = open(KERNEL).read()
     assert kernel.count("for (int64_t i = launch_first(blockIdx.x, SM_THREADS, threadIdx.x); i < a.n_seq; i += launch_step(gridDim.x, SM_THREADS)) a.arrived[i] = 0;") == 1
     assert not re.search(r"blockIdx\.x \* SM_THREADS|gridDim\.x \* SM_THREADS", kernel)
+
+
+def test_sums_of_parts_are_stored_before_their_workgroup_is_counted(tmp_path):
+    """The workgroup that is counted last reads the sums of all: the wave that counts has stored its workgroup's sums itself and has waited for the stores.  A release of one wave waits for
+    that wave's stores alone, and a barrier does not wait for those of the others."""
+    flags = re.search(r"^HIPFLAGS \?= ((?:.*\\\n)*.*)$", open(os.path.join(ROOT, "spy_amd", "csrc", "Makefile")).read(), re.M).group(1)
+    flags = [f for f in flags.replace("\\\n", " ").replace("$(ARCH)", "gfx950").replace("$(PRELOAD)", "").split() if f != "-Wall"]
+    out = str(tmp_path / "verify.s")
+    subprocess.run([shutil.which("hipcc") or "/opt/rocm/bin/hipcc"] + flags + ["-w", "--cuda-device-only", "-S", "-o", out, KERNEL], check=True, capture_output=True, timeout=300)
+    text = open(out).read()
+    code = re.search(r"^_Z18verify_draw_kernel\w+:.*?^\.Lfunc_end", text, re.M | re.S).group(0).split("\n")
+    count = [i for i, line in enumerate(code) if re.search(r"\bglobal_atomic_add\b", line)]
+    sums = [i for i, line in enumerate(code) if re.search(r"\bglobal_store_dwordx2\b.* sc1\b", line)]
+    assert len(count) == 1 and len(sums) == 1 and sums[0] < count[0], (sums, count)
+    between = "\n".join(code[sums[0]:count[0]])
+    assert "s_barrier" not in between and re.search(r"s_waitcnt vmcnt\(0\)", between), between
