@@ -297,7 +297,9 @@ typedef struct spy_hip_paged_prefix {
 } spy_hip_paged_prefix;
 /* A new token lies behind what its group has in common: a group with a sequence for which that is not so, or that does not fit -- more rows than max_rows, more in common than max_prefix, sequences
  * outside the batch -- raises the error flag, and that sequence, or the group's sequences, take no part: their rows are left alone.  k_scales and v_scales: NULL with F16 pages, the
- * scales of I8 pages else.  Results differ from those of spy_hip_paged_attention in the order of the sums (fp32) alone.  Everything else is as there, the scratch of its own size too. */
+ * scales of I8 pages else.  A probability enters the product with as many terms as in spy_hip_paged_attention, whatever the rows of the group are: two for F32 outputs and for sequences of up to 16
+ * rows.  (F16 outputs of longer ones, which have one term there, may have two for keys in common, where rows of a short sequence of their group lie in the same tile.)  But for that, results differ
+ * from those of spy_hip_paged_attention in the order of the sums (fp32) alone.  Everything else is as there, the scratch of its own size too. */
 size_t spy_hip_paged_attention_shared_scratch_size(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix);
 int spy_hip_paged_attention_shared(void *stream, const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_tensor *k_scales, const spy_hip_tensor *v_pages,
                                    const spy_hip_tensor *v_scales, const spy_hip_tensor *out, const spy_hip_paged_batch *batch, const spy_hip_paged_prefix *prefix, float scale, void *scratch,

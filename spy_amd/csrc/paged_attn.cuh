@@ -471,7 +471,10 @@ static __device__ __forceinline__ int find_tile(const attn_args &a, int left, in
 }
 
 // ... of what the sequences of groups have in common, or of their own keys
-static __device__ __forceinline__ bool find_span(const attn_more &a, bool common, int left, int &tile, int &count, pg_span &sq) {
+struct span_tile { pg_span sq; int tile, count; };
+static __device__ __forceinline__ bool find_span(const attn_more &a, bool common, int left, span_tile &found) {
+    pg_span &sq = found.sq;
+    int &tile = found.tile, &count = found.count;
     if (!common) {
         const int s = find_tile(a, left, tile, count, sq);
         if (s >= 0) sq = pg_own(a.b, a.groups, s, a.err);
@@ -510,7 +513,8 @@ template <int D, int GROUPS = chunk_groups(D)> struct chunk_shared_q8 : chunk_sh
 // Q8: a tile's whole numbers come to registers two tiles ahead and go to LDS as fp16 values one tile ahead, beside the matrix instructions of the scores, which leave the vector units time for it (512 tokens on 7680, 32 heads
 // to 8, 128 wide: 106 us; beside the products of their own tile 110 to 113).  The registers that takes are those of operands asked for ahead, half as many as with fp16 pages: as many, 256-wide heads keep 48 registers in memory
 // (512 tokens on 3584, 16 heads to 8: 99 us instead of 84), and 128-wide ones are no faster (106.8).
-template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D), class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false) {
+// found: (sequences in groups) the block's tile
+template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D), class Shared = chunk_shared<D>> static __device__ __forceinline__ void attn_chunk(const attn_args_of<MODE> &a, Shared &shared, int block, bool common = false, const span_tile &found = {}) {
     constexpr bool Q8 = MODE & ATTN_Q8, SHARED = MODE & ATTN_SHARED;
     constexpr int ES = Q8 ? 1 : 2;                                         // bytes of an element in the pages
     constexpr int KS = D / 16, DT = D / 32, NI = D / 32;                   // steps of the scores, output tiles, requests of a wave for K (and for V) per tile
@@ -525,7 +529,7 @@ template <int D, bool F32OUT, int MODE = ATTN_PLAIN, int GROUPS = chunk_groups(D
     int tile, count, s;
     std::conditional_t<SHARED, pg_span, pg_seq> sq;
     if constexpr (SHARED) {
-        if (!find_span(a, common, unit / a.G, tile, count, sq)) return;
+        sq = found.sq; tile = found.tile; count = found.count;
         s = sq.s;
     } else {
         s = find_tile(a, unit / a.G, tile, count, sq);

@@ -169,7 +169,8 @@ extern "C" int spy_hip_paged_attention_shared(void *stream, const spy_hip_tensor
     hipStream_t st = (hipStream_t)stream;
     const int64_t hd = k_pages->ne[0];
     const bool f32 = out->type == SPY_HIP_F32;
-    rc = k_scales ? spy_attn_shared_q8(a, hd, f32, st) : attn_shared_launch<ATTN_SHARED>(a, hd, f32, st);
+    const bool two = f32 || (int64_t)batch->max_new * a.group <= a.few;    // (no sequence of many rows: two terms for all)
+    rc = k_scales ? spy_attn_shared_q8(a, hd, two, st) : attn_shared_launch<ATTN_SHARED>(a, hd, two, st);
     if (rc) return rc;
     if (hd == 64) return f32 ? attn_shared_join<64, true>(a, st) : attn_shared_join<64, false>(a, st);
     if (hd == 128) return f32 ? attn_shared_join<128, true>(a, st) : attn_shared_join<128, false>(a, st);
