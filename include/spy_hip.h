@@ -221,7 +221,7 @@ int spy_hip_sample(void *stream, const spy_hip_tensor *logits, const spy_hip_sam
  * tokens: n_row int32, device: the taken ones, the one drawn, -1 behind it (may be the memory of `drafted`); accepted: n_seq int32, device: how many are taken; probs: n_row floats or NULL: p_i of
  * the row's token, 0 where there is none.  A row without a logit above -inf: p is 0 everywhere, and its token -1.  A request whose rows are not among the logits', or
  * that begins before the end of one in front of it, raises the flag of spy_hip_take_error and is left alone.
- * p and q are off by what spy_hip_sample's weights are, p - q by 2^-60 more.  n_row below 2^21 (2^22 without draft_logits).  scratch: spy_hip_sample_verify_scratch_size bytes, 256-byte aligned, this
+ * p and q are off by what spy_hip_sample's weights are, p - q by 2^-50 of the larger of them and 2^-60 more.  n_row below 2^21 (2^22 without draft_logits), n_seq below 2^20.  scratch: spy_hip_sample_verify_scratch_size bytes, 256-byte aligned, this
  * call's alone until the stream has passed it. */
 size_t spy_hip_sample_verify_scratch_size(const spy_hip_tensor *logits, int32_t n_seq);
 int spy_hip_sample_verify(void *stream, const spy_hip_tensor *logits, const spy_hip_sample_param *param, const spy_hip_tensor *draft_logits, const spy_hip_sample_param *draft_param,

@@ -4,7 +4,7 @@
 //
 // First launch: a workgroup for each row and distribution finds what the settings leave -- the last rank word, the sum of the weights and d's own (sample_row_of<true>), and the tokens themselves where
 // they are 1024 at most.  Second launch: four workgroups for each request find the row where its drafts end and draw there, one of them alone where it has those tokens.  p and q are weights over
-// their sums, in 64 bits; p - q as multiples of 2^-60, so that sums of it are exact in any order, and what comes out is the same each time.
+// their sums, in 64 bits; p - q is held as a multiple of 2^-60 (itself off by 2^-50 of the larger of them, verify_share.h), so that sums of it are exact in any order, and what comes out is the same each time.
 //
 // Latency and vector instructions: the first launch reads each row once from memory (verify of 32 requests with 1 to 6 rows of 32000 and a drafter's: 37.6 us, 24.6 of them here), and where top_p alone is set it
 // works out every weight: 160 rows of 100003 by as many workgroups 55 us, 12 for the reads, 24 for the weights (20 instructions a token beside an addition in LDS), 17 for the bin's tokens.  The
@@ -13,6 +13,7 @@
 #include "launch_index.h"
 #include "paged.cuh"
 #include "sample.cuh"
+#include "verify_share.h"
 
 int *spy_hip_err_flag_ptr();
 
@@ -94,8 +95,7 @@ struct verify_weights {
         if (as_p) return w;
         if (!beyond_q) return i == drafted ? 0 : w;
         l = q.clean(l);
-        const double more = (double)w * one_p - (q.has(l, i) ? (double)q.weigh(l) * one_q : 0.0);
-        return more > 0.0 ? (u64)(more * 0x1p60) : 0;
+        return verify_more(w, one_p, q.has(l, i) ? q.weigh(l) : 0, one_q);
     }
     // By a wave: f(weight, token, its logit; 0, 0, 0 where there is none) for the tokens from .. to - 1 that p has, in order of index, a token a lane.  They are looked for first, 256 at a time, in `list`:
     // a weight takes some hundred instructions, and few tokens of many have one.

@@ -33,3 +33,16 @@ def test_sums_of_parts_are_stored_before_their_workgroup_is_counted(tmp_path):
     assert len(count) == 1 and len(sums) == 1 and sums[0] < count[0], (sums, count)
     between = "\n".join(code[sums[0]:count[0]])
     assert "s_barrier" not in between and re.search(r"s_waitcnt vmcnt\(0\)", between), between
+
+
+def test_differences_of_probabilities_are_off_by_what_the_header_says(tmp_path):
+    """2^-50 of the larger probability and 2^-60; 2^-60 alone would not be true."""
+    out = str(tmp_path / "verify_share")
+    subprocess.check_call(["g++", "-O2", "-std=c++20", "-ffp-contract=off", "-o", out, os.path.join(ROOT, "tests", "host", "verify_share.cpp")])
+    r = subprocess.run([out], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+    worst, steps = map(float, r.stdout.split())
+    assert 0 < worst <= 1 and 10 < steps < 1024, r.stdout
+    header = open(os.path.join(ROOT, "include", "spy_hip.h")).read()
+    assert "p - q by 2^-50 of the larger of them and 2^-60 more" in header
+    assert open(KERNEL).read().count("verify_more(w, one_p, ") == 1
