@@ -3,7 +3,7 @@
 // A block with an infinity or NaN, or whose d has no fp16 value, gets d = NaN: it reads back as NaN, as fp16 pages would hold infinities.
 // The whole numbers and the scales lie in planes of their own, so that both are read in whole aligned pieces: a block of 34 bytes is not.
 // A block's maximum is taken by the four lanes that hold it.  One launch, rows and tiles of V as in paged_append.hip: V^T by tiles of 64 positions through LDS, so that 16 positions of a dimension are stored
-// together (from 8 new tokens a sequence and 128 rows on), else byte by byte.  Bound by memory: 2048 tokens of 32 heads each, F32, with q: 30.7 us, 4.4 TB/s; a single token 4.3 us, a launch.
+// together (from 8 new tokens a sequence and 128 rows on), else byte by byte.  Bound by memory: 2048 tokens of 32 heads each, F32, with q: 30.7 us, 4.4 TB/s (F16: 25 us, 3.4 TB/s); a single token 4.3 us, a launch.
 #include "paged_append.cuh"
 
 struct append_q8_args : append_args {

