@@ -1,4 +1,4 @@
-"""What the results of the verification of drafts cannot show, or only at sizes that a test has no time for: no GPU needed."""
+"""What the results of the verification of drafts do not show, and its limits: no GPU needed."""
 import os
 import re
 import shutil
@@ -46,3 +46,12 @@ def test_differences_of_probabilities_are_off_by_what_the_header_says(tmp_path):
     header = open(os.path.join(ROOT, "include", "spy_hip.h")).read()
     assert "p - q by 2^-50 of the larger of them and 2^-60 more" in header
     assert open(KERNEL).read().count("verify_more(w, one_p, ") == 1
+
+
+def test_how_many_requests_a_call_takes():
+    """2^20 - 1, as the header says: the next one's workgroups would be 2^32 threads."""
+    from spy_amd import _lib as H
+    from tests.test_serving_more_args import verify
+    assert verify(n_seq=1 << 20) == H.EINVAL
+    assert verify(n_seq=(1 << 20) - 1, room=1 << 20) == H.ENOSPACE
+    assert "n_seq below 2^20" in open(os.path.join(ROOT, "include", "spy_hip.h")).read()
